@@ -10,6 +10,9 @@ benchmark read like the reference's own:
     check_cuda_inference_memory(desc, inference_batch, hubs, slots_per_hub)
     cuda_probe.*: the test hooks
 
+The operators on torch CUDA tensors beside the network (4-bit microscaled
+matrices, the move sampler) are in azb_ops.py.
+
 The engine is the in-tree libazb200.so; importing this module fails loudly
 when it is missing (there is no CPU fallback).
 """
@@ -50,6 +53,17 @@ class NetDesc(C.Structure):
     @property
     def actions(self):
         return self.area + 1
+
+
+class SampleArgs(C.Structure):
+    """azb_sample_args (include/azb200.h)."""
+
+    _fields_ = [("logits", C.c_void_p), ("type", C.c_int), ("rows", C.c_longlong), ("cols", C.c_longlong),
+                ("ld", C.c_longlong), ("noise", C.c_void_p), ("noise_ld", C.c_longlong), ("legal", C.c_void_p),
+                ("legal_ld", C.c_longlong), ("temperature", C.c_float), ("top_p", C.c_float), ("min_p", C.c_float),
+                ("top_k", C.c_int), ("temperature_rows", C.c_void_p), ("top_p_rows", C.c_void_p),
+                ("min_p_rows", C.c_void_p), ("top_k_rows", C.c_void_p), ("moves", C.c_void_p),
+                ("logprob", C.c_void_p)]
 
 
 _F = C.POINTER(C.c_float)
@@ -120,6 +134,18 @@ def lib() -> C.CDLL:
             L.azb_hub_evaluate_records.argtypes = [C.c_void_p, C.c_int, C.c_void_p, C.c_int, _F, _F] + err
             L.azb_hub_stats.argtypes = [C.c_void_p, C.c_int, C.POINTER(C.c_longlong), C.POINTER(C.c_longlong),
                                         C.POINTER(C.c_longlong), C.POINTER(C.c_double)]
+            V, i, ll = C.c_void_p, C.c_int, C.c_longlong
+            L.azb_infer_device_logits.argtypes = [V]
+            L.azb_infer_device_logits.restype = V
+            L.azb_mx4_sizes.argtypes = [ll, ll, C.POINTER(s), C.POINTER(s)] + err
+            L.azb_mx4_quantise.argtypes = [i, V, i, ll, ll, ll, V, V, V] + err
+            L.azb_mx4_values.argtypes = [i, V, V, ll, ll, V, i, ll, V] + err
+            L.azb_mx4_product.argtypes = [i, V, V, ll, V, V, ll, ll, V, i, V, i, ll, V] + err
+            L.azb_mx4_linear_workspace.argtypes = [ll, ll]
+            L.azb_mx4_linear_workspace.restype = s
+            L.azb_mx4_linear.argtypes = [i, V, i, ll, ll, ll, V, V, ll, V, i, V, i, ll, V, s, V] + err
+            L.azb_sample_moves.argtypes = [i, C.POINTER(SampleArgs), V] + err
+            L.azb_ops_check.argtypes = [i] + err
             L.azb_workspace_bytes.argtypes = [D, C.c_int, C.c_int]
             L.azb_workspace_bytes.restype = s
             L.azb_check_memory.argtypes = [D, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int] + err
@@ -347,6 +373,10 @@ class CudaInference:
 
     def stream(self) -> int:
         return lib().azb_infer_stream(self.h)
+
+    def device_logits(self) -> int:
+        """The device address of the last enqueued pass's logits ([B][actions] float32), for work on stream()."""
+        return lib().azb_infer_device_logits(self.h)
 
     def time(self, B: int, warmup: int, steps: int, with_copies: bool = False, conv: bool = False):
         """(ms for `steps` passes, summed conv-kernel ms or None), CUDA events on the engine's stream."""

@@ -17,30 +17,6 @@ struct azb_runner {
     std::unique_ptr<Runner> impl;
 };
 
-namespace {
-
-void put_text(char* dst, size_t cap, const std::string& s) {
-    if (!dst || cap == 0) return;
-    const size_t n = std::min(cap - 1, s.size());
-    std::memcpy(dst, s.data(), n);
-    dst[n] = '\0';
-}
-
-template <class Fn>
-int guarded(char* err, size_t cap, const char* prefix, Fn fn) {
-    try {
-        fn();
-        return 0;
-    } catch (const std::exception& e) {
-        put_text(err, cap, std::string(prefix) + e.what());
-    } catch (...) {
-        put_text(err, cap, std::string(prefix) + "unknown error");
-    }
-    return -1;
-}
-
-} // namespace
-
 extern "C" {
 
 int azb_cuda_built(void) { return 1; }

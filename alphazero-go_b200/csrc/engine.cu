@@ -3,6 +3,7 @@
 // on one stream: the stem, 2 x blocks fused tensor-core convolutions and the
 // fused heads.
 #include "engine.hpp"
+#include "ops.hpp"
 
 #include <algorithm>
 #include <atomic>
@@ -322,6 +323,19 @@ CUtensorMap make_tensor_map(const void* base, int precision, uint64_t inner, uin
     return m;
 }
 
+
+CUtensorMap make_byte_map(const void* base, uint64_t pitch, uint64_t rows, uint32_t box_rows) {
+    CUtensorMap m;
+    const cuuint64_t dims[2] = {pitch, rows};
+    const cuuint64_t strides[1] = {pitch};
+    const cuuint32_t box[2] = {128, box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUresult r = encode_tiled()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box,
+                                      estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) throw std::runtime_error("cuda: cuTensorMapEncodeTiled failed (" + std::to_string(int(r)) + ")");
+    return m;
+}
 
 // ---------------------------------------------------------------- weights
 

@@ -210,6 +210,7 @@ public:
     cudaStream_t stream() const { return stream_; }
     const Weights& weights() const { return *w_; }
     int* error_host() const { return err_host_; }   // pinned, one int
+    const float* device_logits() const { return ws_->logits; }
     // (total ms of K passes, summed conv-kernel ms)
     // `steps` passes after `warmup`: their total ms; with conv_ms or
     // stage_ms, `steps` more passes with an event around every launch give

@@ -50,13 +50,6 @@ void* scratch_on(int device) {
     return address[device];
 }
 
-void put_text(char* dst, size_t cap, const std::string& s) {
-    if (!dst || cap == 0) return;
-    const size_t n = std::min(cap - 1, s.size());
-    std::memcpy(dst, s.data(), n);
-    dst[n] = '\0';
-}
-
 } // namespace
 
 extern "C" int azb_infer_run_noalloc(azb_infer* h, const float* input, int B, float* logits, float* values,
@@ -96,7 +89,7 @@ extern "C" int azb_infer_run_noalloc(azb_infer* h, const float* input, int B, fl
         }
         return 0;
     } catch (const std::exception& e) {
-        put_text(err, err_cap, std::string("GPU inference failed: ") + e.what());
+        azb::put_text(err, err_cap, std::string("GPU inference failed: ") + e.what());
         return -1;
     }
 }

@@ -173,6 +173,11 @@ int azb_infer_time_stages(azb_infer* h, int B, int steps, double* stage_ms, char
 int azb_infer_read(azb_infer* h, int B, float* logits, float* values, float* ownership, float* probs, char* err,
                    size_t err_cap);
 
+/* The last enqueued pass's logits on the device ([B][area+1], valid until
+ * the handle's next pass), ready for work on azb_infer_stream: for
+ * azb_sample_moves on the engine's own stream. */
+const float* azb_infer_device_logits(azb_infer* h);
+
 /* --------------------------------------------------------------- runner */
 
 typedef struct azb_runner azb_runner;
@@ -256,6 +261,84 @@ int azb_hub_evaluate_records(azb_hub* h, int lane, const uint8_t* records, int B
  * (exactly azb_hub_pass_cap positions) and their summed begin-to-done seconds. */
 int azb_hub_stats(const azb_hub* h, int lane, long long* passes, long long* positions, long long* full_passes,
                   double* gpu_seconds);
+
+/* ------------------------------------------------- device operators */
+
+/* Operators on device memory in the caller's stream (a cudaStream_t; null:
+ * the default stream) of the given device: 4-bit microscaled matrices and
+ * the move sampler. No reference counterpart. Each call checks its arguments
+ * and enqueues one or two kernels; it allocates nothing, does not
+ * synchronise, can be captured into a CUDA graph (after a first call on the
+ * device), keeps no pointer, and leaves the caller's current device as it
+ * was. Matrices are row-major with a row stride `ld` in elements (0: every
+ * row the same; sources only). Element types: */
+enum { AZB_ELEM_F32 = 0, AZB_ELEM_BF16 = 1 };
+
+/* A rows x cols matrix in the 4-bit microscaled form. Blocks of 32 elements
+ * along a row share the scale X = 2^(floor(log2 max|v|) - 2), its exponent at
+ * least -127; an element is v / X rounded to nearest even onto {0, .5, 1,
+ * 1.5, 2, 3, 4, 6}, at most 6 in magnitude. A block holding an infinity or a
+ * NaN is NaN throughout. codes: [rows][16 * ceil(cols / 32)] bytes, element
+ * 2i in the low half of byte i, zero past cols. scales: exponent + 127 (255:
+ * NaN), one byte per block, in tiles of 128 rows x 4 blocks of 512 bytes: row
+ * r, block b at ((r / 128) * ceil(blocks / 4) + b / 4) * 512 + (r % 32) * 16
+ * + (r % 128 / 32) * 4 + b % 4. Both 16-byte aligned. azb_mx4_sizes gives
+ * their sizes in bytes (rows 0..2^22, cols 1..2^26). */
+int azb_mx4_sizes(long long rows, long long cols, size_t* code_bytes, size_t* scale_bytes, char* err, size_t err_cap);
+int azb_mx4_quantise(int device, const void* x, int type, long long rows, long long cols, long long ld, void* codes,
+                     void* scales, void* stream, char* err, size_t err_cap);
+/* The values the matrix holds; exact in either type. */
+int azb_mx4_values(int device, const void* codes, const void* scales, long long rows, long long cols, void* out, int type,
+                   long long ld, void* stream, char* err, size_t err_cap);
+/* out[i][j] = act(sum_k x[i][k] w[j][k] + bias[j]): x is m x k, w n x k, out
+ * m x n, act ReLU (a NaN stays NaN) or nothing, bias fp32 or null. Products
+ * are exact and summed in fp32. */
+int azb_mx4_product(int device, const void* x_codes, const void* x_scales, long long m, const void* w_codes,
+                    const void* w_scales, long long n, long long k, const float* bias, int relu, void* out, int type,
+                    long long ld, void* stream, char* err, size_t err_cap);
+/* The product with x given as plain elements, quantised on the way into the
+ * workspace (azb_mx4_linear_workspace bytes, 256-byte aligned; 0 for sizes
+ * out of range). */
+size_t azb_mx4_linear_workspace(long long m, long long k);
+int azb_mx4_linear(int device, const void* x, int x_type, long long m, long long k, long long x_ld, const void* w_codes,
+                   const void* w_scales, long long n, const float* bias, int relu, void* out, int type, long long ld,
+                   void* workspace, size_t workspace_bytes, void* stream, char* err, size_t err_cap);
+
+/* One move per row of logits. With l the legal, non-NaN logits above -inf and
+ * m their maximum: x = 0 where l = m, else (l - m) / temperature. In
+ * descending order of l (ties: lower column first) top_k keeps the first k
+ * (0 or less: off), top_p of those the shortest prefix whose share of their
+ * mass sum exp(x) reaches p (1 or more: off), min_p those with exp(x) >=
+ * min_p (0 or less: off); the first is always kept. The move is the kept
+ * column with the largest x - log(-log u), u its noise clamped into [2^-25,
+ * 1 - 2^-24] (a NaN: the lowest), ties to the lower column: a draw from the
+ * kept ones' distribution when the noise is uniform on (0, 1). logprob (may
+ * be null) is x[move] - log(sum exp(x)) over all of l. A temperature of 0 or
+ * less, or NaN, takes the first largest logit, logprob 0. A row without any l
+ * gives -1 and -inf. A row's result does not depend on the other rows. */
+typedef struct azb_sample_args {
+    const void* logits;              /* [rows][cols], AZB_ELEM_* */
+    int type;
+    long long rows, cols, ld;
+    const float* noise;              /* [rows][cols]; null only at temperature 0 */
+    long long noise_ld;
+    const uint8_t* legal;            /* [rows][cols], nonzero: legal; null: all */
+    long long legal_ld;
+    float temperature, top_p, min_p; /* for every row, */
+    int top_k;
+    const float* temperature_rows;   /* or one per row where not null */
+    const float* top_p_rows;
+    const float* min_p_rows;
+    const int* top_k_rows;
+    int64_t* moves;                  /* [rows] */
+    float* logprob;                  /* [rows] or null */
+} azb_sample_args;
+int azb_sample_moves(int device, const azb_sample_args* args, void* stream, char* err, size_t err_cap);
+
+/* Waits for the device and reports whether a bounded wait inside a product
+ * kernel ran out since the last call (its outputs are then not valid): 0, or
+ * -1 with "cuda: ...". */
+int azb_ops_check(int device, char* err, size_t err_cap);
 
 /* ------------------------------------------------------- memory checks */
 
