@@ -55,22 +55,20 @@ def _matrix(t: torch.Tensor, what: str):
     return code, rows, cols, ld
 
 
-def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+_stream = torch._C._cuda_getCurrentRawStream   # of a device index: its current stream's handle
 
 
-def _same_device(device, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, not on {device}")
+def _empty(rows: int, cols: int, dtype, device) -> torch.Tensor:
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
 
 
 class Mx4:
-    """A rows x cols matrix in the 4-bit microscaled form: `codes` (uint8
-    [rows, 16 * ceil(cols / 32)]) and `scales` (uint8, in the tensor core's
-    tile order), as azb_mx4_quantise lays them out."""
+    """A rows x cols matrix in the 4-bit microscaled form, as azb_mx4_quantise
+    lays it out: `codes` (uint8 [rows, 16 * ceil(cols / 32)]) and `scales`
+    (uint8, in the tensor core's tile order) in one allocation. Mx4(codes,
+    scales, rows, cols) takes existing ones."""
 
-    __slots__ = ("codes", "scales", "rows", "cols")
+    __slots__ = ("_data", "_split", "_scales", "rows", "cols", "device")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: int):
         need, got = _sizes(rows, cols), (codes.numel(), scales.numel())
@@ -78,38 +76,47 @@ class Mx4:
             raise ValueError(f"Mx4 of {rows} x {cols}: {need} bytes of codes and scales, not {got}")
         if not (codes.is_cuda and codes.is_contiguous() and scales.is_contiguous() and codes.device == scales.device):
             raise ValueError("Mx4: codes and scales must be contiguous and on one GPU")
-        self.codes, self.scales, self.rows, self.cols = codes, scales, rows, cols
+        self._data, self._split, self._scales = codes, need[0], scales
+        self.rows, self.cols, self.device = rows, cols, codes.device
 
     @property
-    def device(self):
-        return self.codes.device
+    def codes(self) -> torch.Tensor:
+        return self._data.flatten()[:self._split].view(self.rows, -1 if self.rows else 0)
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._scales if self._scales is not None else self._data[-(-self._split // 256) * 256:]
+
+    def pointers(self) -> tuple[int, int]:
+        p = self._data.data_ptr()
+        return p, (p + -(-self._split // 256) * 256 if self._scales is None else self._scales.data_ptr())
 
     @property
     def shape(self):
         return (self.rows, self.cols)
 
     def nbytes(self) -> int:
-        return self.codes.numel() + self.scales.numel()
+        return sum(_sizes(self.rows, self.cols))
 
 
-def _sizes(rows: int, cols: int):
-    nc, ns, e = C.c_size_t(), C.c_size_t(), azb200._err()
-    if azb200.lib().azb_mx4_sizes(rows, cols, C.byref(nc), C.byref(ns), e, 1024) != 0:
-        _fail("azb_mx4_sizes", e)
-    return nc.value, ns.value
+def _sizes(rows: int, cols: int) -> tuple[int, int]:
+    """azb_mx4_sizes."""
+    blocks = -(-cols // 32)
+    return rows * blocks * 16, -(-rows // 128) * -(-blocks // 4) * 512
 
 
 def mx4_quantise(x: torch.Tensor) -> Mx4:
     """The 4-bit microscaled form of a matrix."""
     code, rows, cols, ld = _matrix(x, "x")
-    nc, ns = _sizes(rows, cols)
+    device = x.device
     q = object.__new__(Mx4)
-    q.codes = torch.empty((rows, nc // rows if rows else 0), dtype=torch.uint8, device=x.device)
-    q.scales = torch.empty(ns, dtype=torch.uint8, device=x.device)
-    q.rows, q.cols = rows, cols
+    nc, ns = _sizes(rows, cols)
+    q._split, q._scales = nc, None
+    q._data = torch.empty_strided((-(-nc // 256) * 256 + ns,), (1,), dtype=torch.uint8, device=device)
+    q.rows, q.cols, q.device = rows, cols, device
     e = azb200._err()
-    if azb200.lib().azb_mx4_quantise(x.device.index, x.data_ptr(), code, rows, cols, ld, q.codes.data_ptr(),
-                                     q.scales.data_ptr(), _stream(x.device), e, 1024) != 0:
+    if azb200.lib().azb_mx4_quantise(device.index, x.data_ptr(), code, rows, cols, ld, *q.pointers(),
+                                     _stream(device.index), e, 1024) != 0:
         _fail("azb_mx4_quantise", e)
     return q
 
@@ -117,10 +124,11 @@ def mx4_quantise(x: torch.Tensor) -> Mx4:
 def mx4_values(q: Mx4, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values q holds; exact in either type."""
     code = _type(dtype, "dtype")
-    out = torch.empty((q.rows, q.cols), dtype=dtype, device=q.device)
+    device, rows, cols = q.device, q.rows, q.cols
+    out = _empty(rows, cols, dtype, device)
     e = azb200._err()
-    if azb200.lib().azb_mx4_values(q.device.index, q.codes.data_ptr(), q.scales.data_ptr(), q.rows, q.cols,
-                                   out.data_ptr(), code, q.cols, _stream(q.device), e, 1024) != 0:
+    if azb200.lib().azb_mx4_values(device.index, *q.pointers(), rows, cols, out.data_ptr(), code, cols,
+                                   _stream(device.index), e, 1024) != 0:
         _fail("azb_mx4_values", e)
     return out
 
@@ -148,19 +156,21 @@ def mx4_product(x, w: Mx4, *, bias: torch.Tensor | None = None, relu: bool = Fal
     device = x.device
     if bias is not None and (bias.dtype != torch.float32 or bias.shape != (w.rows,) or not bias.is_contiguous()):
         raise ValueError(f"bias: {w.rows} adjacent float32 numbers are needed")
-    _same_device(device, w=w, bias=bias)
+    if w.device != device or (bias is not None and bias.device != device):
+        raise ValueError(f"x is on {device}, w on {w.device}" + (f", bias on {bias.device}" if bias is not None else ""))
     n = w.rows
-    out = torch.empty((m, n), dtype=dtype, device=device)
+    out = _empty(m, n, dtype, device)
     L, e = azb200.lib(), azb200._err()
-    tail = (n, None if bias is None else bias.data_ptr(), int(relu), out.data_ptr(), code, n)
+    b = None if bias is None else bias.data_ptr()
     if quantised:
-        rc = L.azb_mx4_product(device.index, x.codes.data_ptr(), x.scales.data_ptr(), m, w.codes.data_ptr(),
-                               w.scales.data_ptr(), n, k, *tail[1:], _stream(device), e, 1024)
+        rc = L.azb_mx4_product(device.index, *x.pointers(), m, *w.pointers(), n, k, b, relu, out.data_ptr(), code, n,
+                               _stream(device.index), e, 1024)
     else:
-        need = L.azb_mx4_linear_workspace(m, k)
-        ws = torch.empty(need, dtype=torch.uint8, device=device)
-        rc = L.azb_mx4_linear(device.index, x.data_ptr(), x_type, m, k, x_ld, w.codes.data_ptr(), w.scales.data_ptr(),
-                              *tail, ws.data_ptr(), need, _stream(device), e, 1024)
+        nc, ns = _sizes(m, k)
+        need = -(-nc // 256) * 256 + ns   # azb_mx4_linear_workspace
+        ws = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=device)
+        rc = L.azb_mx4_linear(device.index, x.data_ptr(), x_type, m, k, x_ld, *w.pointers(), n, b, relu,
+                              out.data_ptr(), code, n, ws.data_ptr(), need, _stream(device.index), e, 1024)
     if rc != 0:
         _fail("azb_mx4_product", e)
     return out[0] if vector else out
@@ -196,16 +206,18 @@ def sample_moves(logits: torch.Tensor, noise: torch.Tensor | None, *, legal: tor
         if legal.dtype not in (torch.bool, torch.uint8) or legal.shape != logits.shape or (cols > 1 and legal.stride(1) != 1):
             raise ValueError("legal: bool or uint8 of logits' shape, columns adjacent")
         a.legal, a.legal_ld = legal.data_ptr(), legal.stride(0)
-    _same_device(device, noise=noise, legal=legal)
+    for name, t in (("noise", noise), ("legal", legal)):
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, not on {device}")
     a.temperature, a.temperature_rows = _per_row(temperature, "temperature", rows, device, torch.float32)
     a.top_k, a.top_k_rows = _per_row(top_k, "top_k", rows, device, torch.int32)
     a.top_p, a.top_p_rows = _per_row(top_p, "top_p", rows, device, torch.float32)
     a.min_p, a.min_p_rows = _per_row(min_p, "min_p", rows, device, torch.float32)
-    moves = torch.empty(rows, dtype=torch.int64, device=device)
-    logprob = torch.empty(rows, dtype=torch.float32, device=device)
+    moves = torch.empty_strided((rows,), (1,), dtype=torch.int64, device=device)
+    logprob = torch.empty_strided((rows,), (1,), dtype=torch.float32, device=device)
     a.moves, a.logprob = moves.data_ptr(), logprob.data_ptr()
     e = azb200._err()
-    if azb200.lib().azb_sample_moves(device.index, C.byref(a), _stream(device), e, 1024) != 0:
+    if azb200.lib().azb_sample_moves(device.index, a, _stream(device.index), e, 1024) != 0:
         _fail("azb_sample_moves", e)
     return moves, logprob
 

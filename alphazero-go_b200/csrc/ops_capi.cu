@@ -1,7 +1,6 @@
 // C ABI of the operators beside the network (include/azb200.h): argument
 // checks, then one or two launches on the caller's stream. The caller's
 // current device is left as it was.
-#include <climits>
 #include <cmath>
 #include <stdexcept>
 #include <string>
@@ -192,9 +191,9 @@ int azb_sample_moves(int device, const azb_sample_args* p, void* stream, char* e
         const char* fn = "azb_sample_moves";
         require(p, std::string(fn) + ": null argument");
         check_type(p->type, fn);
-        require(p->rows >= 0 && p->rows <= INT_MAX && p->cols >= 1 && p->cols <= (1ll << 30),
+        require(p->rows >= 0 && p->rows <= (1ll << 27) && p->cols >= 1 && p->cols <= (1ll << 30),
                 std::string(fn) + ": " + std::to_string(p->rows) + " rows of " + std::to_string(p->cols) +
-                    " (rows 0..2^31-1, columns 1..2^30)");
+                    " (rows 0..2^27, columns 1..2^30)");
         require(p->ld >= 0 && p->noise_ld >= 0 && p->legal_ld >= 0, std::string(fn) + ": negative row stride");
         require(p->temperature_rows || (p->temperature >= 0.0f && std::isfinite(p->temperature)),
                 std::string(fn) + ": the temperature must be finite and at least 0");

@@ -68,6 +68,8 @@ struct RowParams {
           top_k(a.top_k_rows ? a.top_k_rows[row] : a.top_k) {}
     __device__ bool greedy() const { return !(temperature > 0.0f); }
     __device__ bool filters_p() const { return top_p < 1.0f; }   // false for a NaN
+    // How many the first filter keeps (0 or less: all): top-p 0 keeps one.
+    __device__ int first_k() const { return filters_p() && !(top_p > 0.0f) ? 1 : top_k; }
 };
 
 // Logits with key > key, and the first `ties` with key == key.
@@ -87,7 +89,7 @@ struct Weighed {
 template <class At>
 __device__ Threshold find_threshold(const RowParams& rp, uint32_t top, int valid, float mass, At at) {
     Threshold th{kKeyLow, kAllTies};
-    const int k = rp.filters_p() && !(rp.top_p > 0.0f) ? 1 : rp.top_k;
+    const int k = rp.first_k();
     float kept = mass;   // mass of what is kept so far
     if (k > 0 && k < valid) {
         uint32_t lo = kKeyLow, hi = top + 1;   // count(lo) >= k > count(hi)
@@ -230,131 +232,693 @@ __global__ void __launch_bounds__(128) sample_warp_kernel(const SampleArgs a) {
     }
 }
 
-// -------------------------------------------------------- a block per row
+// ------------------------------------------------------ a cluster per row
+//
+// More columns: a cluster of CTAs per row, each with a slice of the columns
+// in shared memory, so that the logits cross HBM once however many passes
+// the filters need. (A slice too long for that is read again from global
+// memory: kResident false.) The number of CTAs follows from the columns
+// alone, so a row's sums, and with them its result's bits, do not depend on
+// the batch.
+//
+// A filter's threshold is found from a histogram of the upper logits in
+// kBins equal steps of log w, each bin with its count and its mass in fixed
+// point (integers: the order of the atomics does not show). The bin in which
+// the threshold lies is known from its cumulative sums to within their
+// rounding; the logits in it (a list of at most kList) are sorted and the
+// exact cut found among them, on top of the exact count and mass of what lies
+// above. Where the list would be longer (many equal logits, say) the range of
+// keys is halved as in find_threshold.
+//
+// Lower bounds keep most logits out of the histogram: with k <= the number of
+// warps (threads) that hold a logit, the k-th largest is at least the least
+// of their maxima; and logits with w < (1 - p) Z / cols have together less
+// than (1 - p) Z, so the prefix that top-p keeps ends above them.
 
-constexpr int kWideThreads = 1024;
+constexpr int kRowThreads = 512, kRowWarps = kRowThreads / 32, kMaxCluster = 8;
+constexpr int kBins = 512, kList = 256;
+// Gumbel noise -log(-log u) lies in [-2.86, 16.64]: a logit with x < -19.6
+// loses to the maximum whatever their numbers, which need not be read.
+constexpr float kNoChance = -19.6f;
+constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
 
-struct WideShared {
-    float f[32];
-    int n[32];
+__device__ __forceinline__ float ex2(float y) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
+    return r;
+}
+
+__device__ __forceinline__ float logit_of_key(uint32_t key) {
+    return __uint_as_float(key >> 31 ? key ^ 0x80000000u : ~key);
+}
+
+// Descending order of logits, ties by ascending column, as descending numbers.
+__device__ __forceinline__ uint64_t place_of(uint32_t key, int i) { return uint64_t(key) << 32 | uint32_t(~uint32_t(i)); }
+
+struct Part {   // what one CTA knows of its slice
+    float top;             // largest logit
+    float z;               // sum of w relative to `top`
+    float warp_low;        // least of its warps' largest logits
+    float thread_low;      // least of its threads'
+    int valid, warps, threads;   // logits above -inf, warps and threads that hold one
 };
 
-// Every thread's value reduced over the block, in a fixed order.
-__device__ __forceinline__ float block_max(float v, WideShared& sh) {
+struct RowShared {
+    uint32_t hist_n[kBins], hist_w[kBins];   // this CTA's; then the lists
+    uint32_t all_n[kBins], all_w[kBins];     // the cluster's
+    Part part[kMaxCluster];
+    float f[2][kMaxCluster];
+    int n[2][kMaxCluster];
+    unsigned long long best[kMaxCluster];
+    float best_x[kMaxCluster];
+    float wf[kRowWarps], wg[kRowWarps], wh[kRowWarps];
+    int wn[kRowWarps], wm[kRowWarps], wk[kRowWarps];
+    unsigned list_n;
+    int first, last;
+    float kept;
+    uint64_t cut;
+};
+static_assert(kList * 2 * 8 <= int(sizeof(uint32_t)) * kBins * 2, "a CTA's list and the merged one take the histogram's place");
+
+// The address of *p in CTA `rank` of the cluster.
+template <typename P>
+__device__ __forceinline__ uint32_t at_rank(P* p, int rank) { return mapa(smem_u32(p), uint32_t(rank)); }
+__device__ __forceinline__ void put_f(uint32_t a, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory"); }
+__device__ __forceinline__ void put_u(uint32_t a, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
+__device__ __forceinline__ uint32_t get_u(uint32_t a) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void put_l(uint32_t a, unsigned long long v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory"); }
+__device__ __forceinline__ unsigned long long get_l(uint32_t a) {
+    unsigned long long v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sh.f[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = sh.f[threadIdx.x & 31];
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
     return v;
 }
 
-__device__ __forceinline__ Weighed block_add(Weighed v, WideShared& sh) {
-    v.count = int(__reduce_add_sync(0xFFFFFFFFu, unsigned(v.count)));
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v.mass += __shfl_xor_sync(0xFFFFFFFFu, v.mass, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) {
-        sh.f[threadIdx.x >> 5] = v.mass;
-        sh.n[threadIdx.x >> 5] = v.count;
-    }
-    __syncthreads();
-    v.count = int(__reduce_add_sync(0xFFFFFFFFu, unsigned(sh.n[threadIdx.x & 31])));
-    v.mass = sh.f[threadIdx.x & 31];
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v.mass += __shfl_xor_sync(0xFFFFFFFFu, v.mass, o);
-    return v;
-}
-
+// 16 bytes of logits in shared memory.
 template <typename T>
-__global__ void __launch_bounds__(kWideThreads) sample_block_kernel(const SampleArgs a) {
-    __shared__ WideShared sh;
-    const long long row = blockIdx.x;
-    const RowParams rp(a, row);
-    const T* logits = static_cast<const T*>(a.logits) + size_t(row) * size_t(a.ld);
-    const uint8_t* legal = a.legal ? a.legal + size_t(row) * size_t(a.legal_ld) : nullptr;
-    const int t = int(threadIdx.x), step = kWideThreads;
-    float m = neg_inf();
-    for (int i = t; i < a.cols; i += step) m = fmaxf(m, logit_at(a, logits, legal, i));
-    m = block_max(m, sh);
-    if (m == neg_inf()) {
-        if (t == 0) {
-            a.moves[row] = -1;
-            if (a.logprob) a.logprob[row] = neg_inf();
+struct Pack {
+    static constexpr int kWidth = 16 / int(sizeof(T));
+    uint4 q;
+    __device__ __forceinline__ float get(int e) const {
+        if constexpr (sizeof(T) == 2) {
+            const uint32_t u = reinterpret_cast<const uint32_t*>(&q)[e >> 1];
+            return __uint_as_float(e & 1 ? u & 0xFFFF0000u : u << 16);
+        } else {
+            return reinterpret_cast<const float*>(&q)[e];
         }
-        return;
     }
-    const bool greedy = rp.greedy();
-    const float inv_t = greedy ? 1.0f : 1.0f / rp.temperature;
-    float z = 0.0f;
-    Threshold th{key_of(m), kAllTies};
-    int cut = 0x7FFFFFFF;   // columns from here on keep none of the threshold's ties
-    if (!greedy) {
-        auto at = [&](uint32_t key) {
-            Weighed s{0, 0.0f};
-            for (int i = t; i < a.cols; i += step) {
-                const float l = logit_at(a, logits, legal, i);
-                if (key_of(l) >= key) {
-                    ++s.count;
-                    s.mass += expf(scaled(l, m, inv_t));
+    // NaN becomes -inf.
+    __device__ __forceinline__ void clean() {
+        if constexpr (sizeof(T) == 2) {
+            const __nv_bfloat162 low = __floats2bfloat162_rn(neg_inf(), neg_inf());
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                __nv_bfloat162& h = reinterpret_cast<__nv_bfloat162*>(&q)[e];
+                h = __hmax2(h, low);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float& f = reinterpret_cast<float*>(&q)[e];
+                f = fmaxf(f, neg_inf());
+            }
+        }
+    }
+    __device__ __forceinline__ void drop(int e) {
+        if constexpr (sizeof(T) == 2) reinterpret_cast<uint16_t*>(&q)[e] = 0xFF80u;
+        else reinterpret_cast<uint32_t*>(&q)[e] = 0xFF800000u;
+    }
+};
+
+template <typename T, bool kResident>
+struct Slice {
+    using P = Pack<T>;
+    enum : int { W = P::kWidth };
+    const T* src;            // the slice's first logit
+    const uint8_t* legal;    // its legality, or null
+    int n;                   // logits in the slice
+    int shift;               // src's place in its 16 bytes: logit i is element shift + i of `mem`
+    P* mem;                  // resident: the slice, -inf around and where nothing may be chosen
+    bool infinite = false;   // the row's maximum is +inf: its infinite logits stand as 0, the rest as -inf
+
+    __device__ __forceinline__ float direct(int i) const {
+        float l = float(src[i]);
+        if (l != l || (legal && !legal[i])) l = neg_inf();
+        if (infinite) l = l == __uint_as_float(0x7F800000u) ? 0.0f : neg_inf();
+        return l;
+    }
+    __device__ __forceinline__ int packs() const { return (shift + n + W - 1) / W; }
+
+    // Brings the slice in; f(l) for this thread's logits.
+    template <class F>
+    __device__ __forceinline__ void load(F f) {
+        if constexpr (kResident) {
+            const uint4* base = reinterpret_cast<const uint4*>(src - shift);
+            const int np = packs();
+            constexpr int kAhead = 4;
+            for (int v0 = int(threadIdx.x); v0 < np; v0 += kRowThreads * kAhead) {
+                P p[kAhead];
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    const int v = v0 + u * kRowThreads, i = v * W - shift;
+                    if (v < np && i >= 0 && i + W <= n) p[u].q = __ldg(base + v);
+                }
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    const int v = v0 + u * kRowThreads, i = v * W - shift;
+                    if (v >= np) continue;
+                    if (i < 0 || i + W > n) {
+#pragma unroll
+                        for (int e = 0; e < W; ++e) {
+                            p[u].drop(e);
+                            if (i + e >= 0 && i + e < n) reinterpret_cast<T*>(&p[u].q)[e] = src[i + e];
+                        }
+                    }
+                    p[u].clean();
+                    if (legal) {
+#pragma unroll
+                        for (int e = 0; e < W; ++e)
+                            if (i + e >= 0 && i + e < n && !legal[i + e]) p[u].drop(e);
+                    }
+                    mem[v] = p[u];
+#pragma unroll
+                    for (int e = 0; e < W; ++e) f(p[u].get(e));
                 }
             }
-            return block_add(s, sh);
-        };
-        const Weighed all = at(kKeyLow);
-        z = all.mass;
-        th = find_threshold(rp, key_of(m), all.count, all.mass, at);
-        if (th.ties != kAllTies) {   // the column after the last tie kept
-            int lo = 0, hi = a.cols;   // ties before lo < th.ties <= ties before hi
-            while (hi - lo > 1) {
-                const int mid = lo + (hi - lo) / 2;
-                Weighed s{0, 0.0f};
-                for (int i = t; i < mid; i += step) s.count += key_of(logit_at(a, logits, legal, i)) == th.key;
-                if (block_add(s, sh).count >= th.ties) hi = mid;
-                else lo = mid;
-            }
-            cut = hi;
+        } else {
+            for (int i = int(threadIdx.x); i < n; i += kRowThreads) f(direct(i));
         }
     }
-    const float* noise = greedy ? nullptr : a.noise + size_t(row) * size_t(a.noise_ld);
-    float best = neg_inf(), best_x = 0.0f;
-    uint32_t best_i = 0xFFFFFFFFu;
-    for (int i = t; i < a.cols; i += step) {
-        const float l = logit_at(a, logits, legal, i);
-        const uint32_t key = key_of(l);
-        if (key < th.key || (key == th.key && i >= cut)) continue;
-        const float x = scaled(l, m, inv_t);
-        if (l != m && rp.min_p > 0.0f && !greedy && !(expf(x) >= rp.min_p)) continue;
-        const float r = greedy ? 0.0f : race(x, noise[i]);
-        if (r > best) best = r, best_i = uint32_t(i), best_x = x;
+    // f(l, i) for this thread's logits (and some of -inf around the slice).
+    template <class F>
+    __device__ __forceinline__ void each(F f) const {
+        if constexpr (kResident) {
+            const int np = packs();
+            for (int v = int(threadIdx.x); v < np; v += kRowThreads) {
+                const P p = mem[v];
+#pragma unroll
+                for (int e = 0; e < W; ++e) f(p.get(e), v * W - shift + e);
+            }
+        } else {
+            for (int i = int(threadIdx.x); i < n; i += kRowThreads) f(direct(i), i);
+        }
     }
-    // The winner: the largest key's lowest index.
-    __shared__ uint32_t first;
-    __shared__ float first_x;
-    const float top = block_max(best, sh);
-    if (t == 0) first = 0xFFFFFFFFu;
+    // The row's maximum is +inf (every CTA of the cluster learns it at once).
+    __device__ void only_infinite() {
+        infinite = true;
+        if constexpr (kResident) {
+            for (int v = int(threadIdx.x); v < packs(); v += kRowThreads) {
+                P p = mem[v];
+#pragma unroll
+                for (int e = 0; e < W; ++e) {
+                    if (p.get(e) != __uint_as_float(0x7F800000u)) p.drop(e);
+                    else reinterpret_cast<T*>(&p.q)[e] = T(0.0f);
+                }
+                mem[v] = p;
+            }
+        }
+    }
+};
+
+__device__ __forceinline__ void cluster_barrier() {
+    __syncwarp();
+    cluster_sync();
+}
+
+// Count and mass over the cluster, in a fixed order; the same everywhere.
+// `turn` alternates between two sets of slots: a CTA writes a set again only
+// after a barrier that every CTA reaches past its reads of it.
+__device__ __forceinline__ Weighed cluster_add(Weighed v, RowShared& sh, int rank, int ranks, int& turn) {
+    const int warp = int(threadIdx.x) >> 5, lane = int(threadIdx.x) & 31;
+    v.count = int(__reduce_add_sync(0xFFFFFFFFu, unsigned(v.count)));
+    v.mass = warp_sum(v.mass);
     __syncthreads();
-    if (best == top) atomicMin(&first, best_i);
+    if (lane == 0) {
+        sh.wf[warp] = v.mass;
+        sh.wn[warp] = v.count;
+    }
     __syncthreads();
-    if (best == top && best_i == first) first_x = best_x;
+    if (warp == 0) {
+        Weighed s{0, 0.0f};
+        for (int w = 0; w < kRowWarps; ++w) {
+            s.count += sh.wn[w];
+            s.mass += sh.wf[w];
+        }
+        if (lane < ranks) {
+            put_f(at_rank(&sh.f[turn][rank], lane), s.mass);
+            put_u(at_rank(&sh.n[turn][rank], lane), uint32_t(s.count));
+        }
+    }
+    cluster_barrier();
+    Weighed s{0, 0.0f};
+    for (int r = 0; r < ranks; ++r) {
+        s.count += sh.n[turn][r];
+        s.mass += sh.f[turn][r];
+    }
+    turn ^= 1;
+    return s;
+}
+
+struct Inclusive {
+    uint32_t n, w;
+};
+// The histogram's inclusive sums up to bin threadIdx.x (kBins == kRowThreads).
+static_assert(kBins == kRowThreads, "a thread per bin");
+__device__ __forceinline__ Inclusive scan_bins(RowShared& sh) {
+    const int warp = int(threadIdx.x) >> 5, lane = int(threadIdx.x) & 31;
+    Inclusive s{sh.all_n[threadIdx.x], sh.all_w[threadIdx.x]};
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t n = __shfl_up_sync(0xFFFFFFFFu, s.n, o), w = __shfl_up_sync(0xFFFFFFFFu, s.w, o);
+        if (lane >= o) s.n += n, s.w += w;
+    }
+    __syncthreads();
+    if (lane == 31) sh.wn[warp] = int(s.n), sh.wm[warp] = int(s.w);
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) s.n += uint32_t(sh.wn[w]), s.w += uint32_t(sh.wm[w]);
+    return s;
+}
+
+template <typename T, bool kResident>
+__global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const SampleArgs a, const int ranks, const int per) {
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    __shared__ RowShared sh;
+    const int rank = int(blockIdx.x) % ranks, t = int(threadIdx.x), warp = t >> 5, lane = t & 31;
+    const long long row = blockIdx.x / unsigned(ranks);
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // this CTA runs: its memory may be written
+    const RowParams rp(a, row);
+    Slice<T, kResident> sl;
+    const int i0 = min(rank * per, a.cols);
+    sl.src = static_cast<const T*>(a.logits) + size_t(row) * size_t(a.ld) + i0;
+    sl.legal = a.legal ? a.legal + size_t(row) * size_t(a.legal_ld) + i0 : nullptr;
+    sl.n = min(per, a.cols - i0);
+    sl.shift = int(reinterpret_cast<uintptr_t>(sl.src) % 16 / sizeof(T));
+    sl.mem = reinterpret_cast<Pack<T>*>(smem_raw);
+    const float inf = __uint_as_float(0x7F800000u);
+
+    // The slice's largest logit, and the sum of w relative to it.
+    float mine = neg_inf();
+    sl.load([&](float l) { mine = fmaxf(mine, l); });
+    const float of_warp = warp_max(mine);
+    {
+        const bool some = mine > neg_inf();
+        float low = some ? -mine : neg_inf();
+        low = warp_max(low);
+        const int threads = __popc(__ballot_sync(0xFFFFFFFFu, some));
+        if (lane == 0) sh.wf[warp] = of_warp, sh.wg[warp] = low, sh.wn[warp] = threads;
+    }
+    __syncthreads();
+    float m = neg_inf();
+    for (int w = 0; w < kRowWarps; ++w) m = fmaxf(m, sh.wf[w]);
+    const bool greedy = rp.greedy();
+    // w = 2^((l - m) c). The bounds keep 0 * c and -inf * c what they should be.
+    const float c = greedy ? 1.0f : fminf(fmaxf(kLog2e / rp.temperature, 1e-38f), 3e38f);
+    {
+        Weighed s{0, 0.0f};
+        if (!greedy && m > neg_inf()) {
+            if (m == inf) sl.each([&](float l, int) { s.mass += l == inf ? 1.0f : 0.0f; });
+            else if (rp.first_k() > 0)
+                sl.each([&](float l, int) {
+                    s.mass += ex2((l - m) * c);
+                    s.count += l > neg_inf();
+                });
+            else sl.each([&](float l, int) { s.mass += ex2((l - m) * c); });
+        }
+        s.mass = warp_sum(s.mass);
+        s.count = int(__reduce_add_sync(0xFFFFFFFFu, unsigned(s.count)));
+        if (lane == 0) sh.wh[warp] = s.mass, sh.wk[warp] = s.count;
+    }
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // every CTA runs
+    __syncthreads();
+    if (warp == 0 && lane < ranks) {
+        Part p{m, 0.0f, inf, inf, 0, 0, 0};
+        for (int w = 0; w < kRowWarps; ++w) {
+            p.z += sh.wh[w];
+            p.valid += sh.wk[w];
+            p.threads += sh.wn[w];
+            if (sh.wf[w] > neg_inf()) {
+                ++p.warps;
+                p.warp_low = fminf(p.warp_low, sh.wf[w]);
+                p.thread_low = fminf(p.thread_low, -sh.wg[w]);
+            }
+        }
+        const uint32_t to = at_rank(&sh.part[rank], lane);
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(&p);
+        for (int i = 0; i < int(sizeof(Part) / 4); ++i) put_u(to + uint32_t(i) * 4, words[i]);
+    }
+    cluster_barrier();
+    Part all{neg_inf(), 0.0f, inf, inf, 0, 0, 0};
+    for (int r = 0; r < ranks; ++r) all.top = fmaxf(all.top, sh.part[r].top);
+    for (int r = 0; r < ranks; ++r) {
+        const Part& p = sh.part[r];
+        all.z += p.top == all.top ? p.z : p.z * ex2((p.top - all.top) * c);
+        all.valid += p.valid;
+        all.warps += p.warps;
+        all.threads += p.threads;
+        all.warp_low = fminf(all.warp_low, p.warp_low);
+        all.thread_low = fminf(all.thread_low, p.thread_low);
+    }
+    m = all.top;
+    int turn = 0;
+    uint64_t best = 0;       // key of the race and the column, as one number: the largest wins
+    float best_x = 0.0f;
+    const auto run_race = [&](float l, int i, float u) {
+        const float x = (l - m) * c * kLn2;
+        const uint64_t r = place_of(key_of(race(x, u)), i);
+        if (r > best) best = r, best_x = x;
+    };
+
+    if (m == neg_inf()) {
+        // nothing to choose from
+    } else if (greedy) {
+        sl.each([&](float l, int i) {
+            if (l == m && place_of(1u, i0 + i) > best) best = place_of(1u, i0 + i);
+        });
+    } else {
+        if (m == inf) {
+            sl.only_infinite();
+            m = 0.0f;
+            all.valid = int(all.z);
+            all.warp_low = all.thread_low = 0.0f;
+        }
+        const float* noise = a.noise + size_t(row) * size_t(a.noise_ld) + i0;
+        const int k = rp.first_k();
+        const bool by_k = k > 0 && k < all.valid, by_p = rp.filters_p() && rp.top_p > 0.0f && k != 1;
+        uint64_t cut = place_of(kKeyLow, 0x7FFFFFFF);   // the last place kept
+        bool raced = false;
+        if (by_k || by_p) {
+            const auto at = [&](uint32_t key) {
+                Weighed s{0, 0.0f};
+                sl.each([&](float l, int) {
+                    if (key_of(l) >= key) {
+                        ++s.count;
+                        s.mass += ex2((l - m) * c);
+                    }
+                });
+                return cluster_add(s, sh, rank, ranks, turn);
+            };
+            // What the histogram covers: log2 w from `low` to 0.
+            float low;
+            if (by_k) {
+                const float l = k <= all.warps ? all.warp_low : k <= all.threads ? all.thread_low : neg_inf();
+                low = fmaxf((l - m) * c, -40.0f);
+            } else {
+                low = fmaxf(__log2f((1.0f - rp.top_p) * 0.99f * all.z / float(a.cols)), -40.0f);
+            }
+            low = fminf(low, -1e-3f);
+            const float steps = float(kBins - 1) / -low;   // bins per unit of log2 w; the last bin holds `low`
+            const float fixed = 2147483648.0f / all.z;     // all masses together stay below 2^31 + cols / 2
+            const auto bin_of = [&](float y) { return int(-y * steps); };
+            sh.hist_n[t] = 0;
+            sh.hist_w[t] = 0;
+            __syncthreads();
+            sl.each([&](float l, int) {
+                const float y = (l - m) * c;
+                if (y >= low) {
+                    const int b = bin_of(y);
+                    atomicAdd(&sh.hist_n[b], 1u);
+                    atomicAdd(&sh.hist_w[b], __float2uint_rn(ex2(y) * fixed));
+                }
+            });
+            cluster_barrier();
+            {   // this CTA adds its share of the bins over the cluster, for everyone
+                const int share = kBins / ranks;
+                if (t < share) {
+                    const int b = rank * share + t;
+                    uint32_t n = 0, w = 0;
+                    for (int r = 0; r < ranks; ++r) {
+                        n += get_u(at_rank(&sh.hist_n[b], r));
+                        w += get_u(at_rank(&sh.hist_w[b], r));
+                    }
+                    for (int r = 0; r < ranks; ++r) {
+                        put_u(at_rank(&sh.all_n[b], r), n);
+                        put_u(at_rank(&sh.all_w[b], r), w);
+                    }
+                }
+            }
+            cluster_barrier();
+            const Inclusive upto = scan_bins(sh);
+            uint64_t* list = reinterpret_cast<uint64_t*>(sh.hist_n);
+            uint64_t* merged = list + kList;
+            // The cut of one filter: the first `count` logits, or the shortest
+            // prefix of mass `target`. False: the histogram does not settle it.
+            // kept: the mass of what the cut is taken from.
+            const auto settle = [&](int count, double target, float* kept) -> bool {
+                __syncthreads();
+                if (t == 0) sh.first = sh.last = kBins, sh.list_n = 0;
+                __syncthreads();
+                if (count > 0) {
+                    if (upto.n >= uint32_t(count) && upto.n - sh.all_n[t] < uint32_t(count)) sh.first = sh.last = t;
+                } else {
+                    // A fixed-point sum is off by half a unit a logit, and by the
+                    // masses' own rounding, a few 2^-22 of it.
+                    const double goal = target * double(fixed), slack = 0.5 * double(upto.n) + 4096.0;
+                    if (double(upto.w) + slack >= goal) atomicMin(&sh.first, t);
+                    if (double(upto.w) - slack >= goal) atomicMin(&sh.last, t);
+                }
+                __syncthreads();
+                int first = sh.first;
+                const int last = sh.last;
+                if (last >= kBins) return false;
+                __syncthreads();
+                // Few enough down to the cut: all of them are listed, and raced there.
+                if (t == last) sh.list_n = upto.n;
+                if (t == first) sh.wk[0] = int(upto.n - sh.all_n[t]);
+                __syncthreads();
+                const uint32_t down = sh.list_n, above = uint32_t(sh.wk[0]);
+                const bool whole = down <= uint32_t(kList);
+                if (!whole && down - above > uint32_t(kList)) return false;
+                if (whole) first = 0;
+                __syncthreads();
+                if (t == 0) sh.list_n = 0;
+                __syncthreads();
+                Weighed s{0, 0.0f};
+                sl.each([&](float l, int i) {
+                    const float y = (l - m) * c;
+                    if (y >= low) {
+                        const int b = bin_of(y);
+                        if (b < first) {
+                            ++s.count;
+                            s.mass += ex2(y);
+                        } else if (b <= last) {
+                            list[atomicAdd(&sh.list_n, 1u)] = place_of(key_of(l), i0 + i);
+                        }
+                    }
+                });
+                s = cluster_add(s, sh, rank, ranks, turn);   // (also: every list is written)
+                // All lists here, then in order.
+                int n = 0;
+                uint64_t mineplace = 0;
+                for (int r = 0; r < ranks; ++r) {
+                    const int rn = int(get_u(at_rank(&sh.list_n, r)));
+                    if (t >= n && t < n + rn) mineplace = get_l(at_rank(&list[t - n], r));
+                    n += rn;
+                }
+                if (t < n) merged[t] = mineplace;
+                __syncthreads();
+                int before = 0;
+                if (t < n)
+                    for (int j = 0; j < n; ++j) before += merged[j] > mineplace;
+                __syncthreads();
+                if (t < n) merged[before] = mineplace;
+                __syncthreads();
+                // The sums run down the sorted list: the same for every CTA and
+                // run. A lane takes kList / 32 neighbours.
+                if (warp == 0) {
+                    constexpr int kEach = kList / 32;
+                    double w[kEach], sum = 0.0;
+#pragma unroll
+                    for (int j = 0; j < kEach; ++j) {
+                        const int at_ = lane * kEach + j;
+                        w[j] = at_ < n ? double(ex2((logit_of_key(uint32_t(merged[at_] >> 32)) - m) * c)) : 0.0;
+                    }
+                    const int live = count > 0 ? min(n, count - s.count) : n;   // of the list, what top-k keeps
+#pragma unroll
+                    for (int j = 0; j < kEach; ++j) sum += lane * kEach + j < live ? w[j] : 0.0;
+                    double ahead = sum;   // up to and with this lane's
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const double d = __shfl_up_sync(0xFFFFFFFFu, ahead, o);
+                        if (lane >= o) ahead += d;
+                    }
+                    const double total = double(s.mass) + __shfl_sync(0xFFFFFFFFu, ahead, 31);
+                    double before_me = double(s.mass) + __shfl_up_sync(0xFFFFFFFFu, ahead, 1);
+                    if (lane == 0) before_me = double(s.mass);
+                    int stay = live;
+                    if (count == 0 || (whole && by_p)) {
+                        if (count > 0) target = double(rp.top_p) * total;
+                        int here = 0;
+#pragma unroll
+                        for (int j = 0; j < kEach; ++j) {
+                            here += lane * kEach + j < live && before_me < target;
+                            before_me += w[j];
+                        }
+                        stay = int(__reduce_add_sync(0xFFFFFFFFu, unsigned(here)));
+                    }
+                    if (lane == 0) {
+                        sh.cut = stay > 0 ? merged[stay - 1] : merged[0] + 1;
+                        sh.kept = float(total);
+                    }
+                }
+                __syncthreads();
+                *kept = sh.kept;
+                if (sh.cut > cut) cut = sh.cut;
+                if (whole) {
+                    raced = true;
+                    if (rank == 0 && t < n) {
+                        const uint64_t place = merged[t];   // (rank 0: i0 is 0)
+                        const float l = logit_of_key(uint32_t(place >> 32));
+                        const int i = int(~uint32_t(place));
+                        if (place >= cut && (l == m || !(rp.min_p > 0.0f) || ex2((l - m) * c) >= rp.min_p))
+                            run_race(l, i, noise[i]);
+                    }
+                }
+                return true;
+            };
+            float kept = all.z;
+            bool settled = true;
+            if (by_k) settled = settle(k, 0.0, &kept);
+            if (settled && by_p && !raced) {
+                if (by_k) cluster_barrier();   // the first cut's lists have been read
+                settled = settle(0, double(rp.top_p) * double(kept), &kept);
+            }
+            if (!settled) {
+                const Weighed every = at(kKeyLow);
+                RowParams only = rp;
+                const Threshold th = find_threshold(only, key_of(m), every.count, every.mass, at);
+                int end = a.cols;   // the column after the threshold's last tie kept
+                if (th.ties != kAllTies) {
+                    int lo = 0;     // ties before lo < th.ties <= ties before end
+                    while (end - lo > 1) {
+                        const int mid = lo + (end - lo) / 2;
+                        Weighed s{0, 0.0f};
+                        sl.each([&](float l, int i) { s.count += i0 + i < mid && key_of(l) == th.key; });
+                        if (cluster_add(s, sh, rank, ranks, turn).count >= th.ties) end = mid;
+                        else lo = mid;
+                    }
+                }
+                cut = place_of(th.key, end - 1);
+            }
+        }
+        if (!raced) {
+            const uint32_t cut_key = uint32_t(cut >> 32);
+            float low = kNoChance * kLog2e;
+            if (rp.min_p > 0.0f) low = fmaxf(low, fminf(__log2f(rp.min_p) - 1e-3f, 0.0f));
+            const auto stays = [&](float l, int i) {
+                const float y = (l - m) * c;
+                if (!(y >= low)) return false;
+                const uint32_t key = key_of(l);
+                if (key < cut_key || place_of(key, i0 + i) < cut) return false;
+                return l == m || !(rp.min_p > 0.0f) || ex2(y) >= rp.min_p;
+            };
+            if constexpr (kResident) {
+                // Every kept logit's number is asked for before the first is used.
+                using P = Pack<T>;
+                constexpr int kAhead = 16 / P::kWidth;
+                const int np = sl.packs();
+                for (int v0 = t; v0 < np; v0 += kRowThreads * kAhead) {
+                    float u[kAhead * P::kWidth];
+                    uint32_t in = 0;
+#pragma unroll
+                    for (int g = 0; g < kAhead; ++g) {
+                        const int v = v0 + g * kRowThreads;
+                        if (v < np) {
+                            const P p = sl.mem[v];
+#pragma unroll
+                            for (int e = 0; e < P::kWidth; ++e) {
+                                const int i = v * P::kWidth - sl.shift + e;
+                                if (stays(p.get(e), i)) {
+                                    in |= 1u << (g * P::kWidth + e);
+                                    u[g * P::kWidth + e] = __ldg(noise + i);
+                                }
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int g = 0; g < kAhead; ++g) {
+                        const int v = v0 + g * kRowThreads;
+#pragma unroll
+                        for (int e = 0; e < P::kWidth; ++e)
+                            if (in >> (g * P::kWidth + e) & 1u)
+                                run_race(sl.mem[v].get(e), i0 + v * P::kWidth - sl.shift + e, u[g * P::kWidth + e]);
+                    }
+                }
+            } else {
+                sl.each([&](float l, int i) {
+                    if (stays(l, i)) run_race(l, i0 + i, noise[i]);
+                });
+            }
+        }
+    }
+
+    // The cluster's winner.
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        const uint64_t b = __shfl_xor_sync(0xFFFFFFFFu, best, o);
+        const float x = __shfl_xor_sync(0xFFFFFFFFu, best_x, o);
+        if (b > best) best = b, best_x = x;
+    }
+    __shared__ uint64_t warp_best[kRowWarps];
+    if (lane == 0) warp_best[warp] = best, sh.wg[warp] = best_x;
     __syncthreads();
     if (t == 0) {
-        a.moves[row] = (long long)first;
-        if (a.logprob) a.logprob[row] = greedy ? 0.0f : first_x - logf(z);
+        for (int w = 0; w < kRowWarps; ++w)
+            if (warp_best[w] > best) best = warp_best[w], best_x = sh.wg[w];
+        put_l(at_rank(&sh.best[rank], 0), best);
+        put_f(at_rank(&sh.best_x[rank], 0), best_x);
     }
+    cluster_barrier();
+    if (rank == 0 && t == 0) {
+        for (int r = 0; r < ranks; ++r)
+            if (sh.best[r] > best) best = sh.best[r], best_x = sh.best_x[r];
+        a.moves[row] = best ? (long long)uint32_t(~uint32_t(best)) : -1;
+        if (a.logprob) a.logprob[row] = !best ? neg_inf() : greedy ? 0.0f : best_x - logf(all.z);
+    }
+}
+
+template <typename T, bool kResident>
+cudaError_t launch_rows(const SampleArgs& a, int ranks, int per, size_t smem, cudaStream_t s) {
+    if (const cudaError_t e = open_smem<sample_row_kernel<T, kResident>>(smem); e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(a.rows * ranks));
+    cfg.blockDim = dim3(kRowThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {unsigned(ranks), 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, sample_row_kernel<T, kResident>, a, ranks, per);
 }
 
 template <typename T>
 cudaError_t launch_sample_t(const SampleArgs& a, cudaStream_t s) {
     const int grid = int((a.rows + 3) / 4);
-    if (a.cols <= 128) sample_warp_kernel<T, 4><<<grid, 128, 0, s>>>(a);
-    else if (a.cols <= 384) sample_warp_kernel<T, 12><<<grid, 128, 0, s>>>(a);
-    else if (a.cols <= 1024) sample_warp_kernel<T, 32><<<grid, 128, 0, s>>>(a);
-    else sample_block_kernel<T><<<int(a.rows), kWideThreads, 0, s>>>(a);
-    return cudaGetLastError();
+    if (a.cols <= 1024) {
+        if (a.cols <= 128) sample_warp_kernel<T, 4><<<grid, 128, 0, s>>>(a);
+        else if (a.cols <= 384) sample_warp_kernel<T, 12><<<grid, 128, 0, s>>>(a);
+        else sample_warp_kernel<T, 32><<<grid, 128, 0, s>>>(a);
+        return cudaGetLastError();
+    }
+    const int ranks = a.cols <= 4096 ? 1 : a.cols <= 8192 ? 2 : a.cols <= 16384 ? 4 : kMaxCluster;
+    const int per = (a.cols + ranks - 1) / ranks;
+    const size_t smem = size_t(per) * sizeof(T) + 32;   // up to 16 bytes of alignment at either end
+    return smem <= (size_t(200) << 10) ? launch_rows<T, true>(a, ranks, per, smem, s) : launch_rows<T, false>(a, ranks, per, 0, s);
 }
 
 }  // namespace

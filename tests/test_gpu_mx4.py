@@ -150,11 +150,10 @@ def test_strided_outputs_leave_the_rest_alone(ops, torch):
     x, w = gpu(torch, normals(5, 9, 70), "float32"), gpu(torch, normals(6, 37, 70), "float32")
     qx, qw = ops.mx4_quantise(x), ops.mx4_quantise(w)
     out = torch.full((9, 101), -7.0, device="cuda")
-    raw(ops, "azb_mx4_values", 0, qx.codes.data_ptr(), qx.scales.data_ptr(), 9, 70, out.data_ptr(), 0, 101, None)
+    raw(ops, "azb_mx4_values", 0, *qx.pointers(), 9, 70, out.data_ptr(), 0, 101, None)
     assert same(host(out[:, :70]), quantised(x.cpu().numpy())) and bool((out[:, 70:] == -7).all())
     out.fill_(-7.0)
-    raw(ops, "azb_mx4_product", 0, qx.codes.data_ptr(), qx.scales.data_ptr(), 9, qw.codes.data_ptr(),
-        qw.scales.data_ptr(), 37, 70, None, 0, out.data_ptr(), 0, 101, None)
+    raw(ops, "azb_mx4_product", 0, *qx.pointers(), 9, *qw.pointers(), 37, 70, None, 0, out.data_ptr(), 0, 101, None)
     assert torch.equal(out[:, :37], ops.mx4_product(qx, qw)) and bool((out[:, 37:] == -7).all())
 
 
@@ -271,7 +270,7 @@ def test_refusals(ops, torch):
         (lambda: ops.mx4_product(x[:, :32], w), "x has 32 columns, w 64"),
         (lambda: ops.mx4_product(x, x), "an Mx4 is needed"),
         (lambda: ops.mx4_product(x, w, bias=torch.ones(3, device="cuda")), "bias: 4 adjacent"),
-        (lambda: ops.mx4_product(x, w, bias=torch.ones(4)), "bias is on cpu"),
+        (lambda: ops.mx4_product(x, w, bias=torch.ones(4)), "bias on cpu"),
         (lambda: ops.mx4_product(x.cpu(), w), "CUDA tensor"),
     ]:
         with pytest.raises(ValueError, match=text):
