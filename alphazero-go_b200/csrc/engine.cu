@@ -324,17 +324,26 @@ CUtensorMap make_tensor_map(const void* base, int precision, uint64_t inner, uin
 }
 
 
-CUtensorMap make_byte_map(const void* base, uint64_t pitch, uint64_t rows, uint32_t box_rows) {
+CUtensorMap make_map_2d(CUtensorMapDataType type, const void* base, uint64_t inner, uint64_t rows, uint64_t row_bytes,
+                        uint32_t box_inner, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
     CUtensorMap m;
-    const cuuint64_t dims[2] = {pitch, rows};
-    const cuuint64_t strides[1] = {pitch};
-    const cuuint32_t box[2] = {128, box_rows};
+    const cuuint64_t dims[2] = {inner, rows};
+    const cuuint64_t strides[1] = {row_bytes};
+    const cuuint32_t box[2] = {box_inner, box_rows};
     const cuuint32_t estr[2] = {1, 1};
-    const CUresult r = encode_tiled()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box,
-                                      estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUresult r = encode_tiled()(&m, type, 2, const_cast<void*>(base), dims, strides, box, estr,
+                                      CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) throw std::runtime_error("cuda: cuTensorMapEncodeTiled failed (" + std::to_string(int(r)) + ")");
     return m;
+}
+
+CUtensorMap make_byte_map(const void* base, uint64_t pitch, uint64_t rows, uint32_t box_rows) {
+    return make_map_2d(CU_TENSOR_MAP_DATA_TYPE_UINT8, base, pitch, rows, pitch, 128, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+CUtensorMap make_scale_map(const void* base, uint64_t tiles) {
+    return make_map_2d(CU_TENSOR_MAP_DATA_TYPE_UINT32, base, 128, tiles, 512, 128, 2, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 // ---------------------------------------------------------------- weights

@@ -24,8 +24,9 @@ __device__ int g_mx4_error;   // KernelError of a product whose bounded wait ran
 
 // ---------------------------------------------------------- conversions
 
-// Eight magnitudes' worth of E2M1 codes, element 0 in the low four bits.
-__device__ __forceinline__ uint32_t pack_e2m1(const float (&v)[8]) {
+// Eight values' E2M1 codes (round to nearest even, at most 6), value 0's in
+// the low four bits.
+__device__ __forceinline__ uint32_t pack_e2m1(const float* v) {
     uint32_t r;
     asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
         "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
@@ -38,7 +39,7 @@ __device__ __forceinline__ uint32_t pack_e2m1(const float (&v)[8]) {
     return r;
 }
 
-__device__ __forceinline__ void unpack_e2m1(uint32_t codes, float (&v)[8]) {
+__device__ __forceinline__ void unpack_e2m1(uint32_t codes, float* v) {
     uint32_t h[4];
     asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
         "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
@@ -56,48 +57,84 @@ __device__ __forceinline__ void unpack_e2m1(uint32_t codes, float (&v)[8]) {
     }
 }
 
-// Elements [c, c + 8) of a row as floats; zeros past cols. kVec: the row is
-// 16-byte aligned and c + 8 <= cols.
-template <typename T, bool kVec>
-__device__ __forceinline__ void load8(const T* row, long long c, long long cols, float (&v)[8]) {
-    if constexpr (kVec && sizeof(T) == 2) {
-        const uint4 q = __ldg(reinterpret_cast<const uint4*>(row + c));
-        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&q);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = __bfloat1622float2(h[i]);
-            v[2 * i] = f.x;
-            v[2 * i + 1] = f.y;
-        }
-    } else if constexpr (kVec) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(row + c));
-        const float4 b = __ldg(reinterpret_cast<const float4*>(row + c) + 1);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? float(row[c + i]) : 0.0f;
-    }
+// kBytes (2 to 16) from global memory into the words at dst.
+template <int kBytes>
+__device__ __forceinline__ void load_piece(uint32_t* dst, const void* src) {
+    if constexpr (kBytes == 16) *reinterpret_cast<uint4*>(dst) = __ldg(static_cast<const uint4*>(src));
+    else if constexpr (kBytes == 8) *reinterpret_cast<uint2*>(dst) = __ldg(static_cast<const uint2*>(src));
+    else if constexpr (kBytes == 4) *dst = __ldg(static_cast<const uint32_t*>(src));
 }
 
-template <typename T, bool kVec>
-__device__ __forceinline__ void store8(T* row, long long c, long long cols, const float (&v)[8]) {
-    if constexpr (kVec && sizeof(T) == 2) {
-        uint4 q;
-        __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&q);
+// kN neighbouring elements of a row as they lie in memory (kN T in words).
+template <typename T, int kN>
+struct Run {
+    static constexpr int kWords = kN * int(sizeof(T)) / 4;
+    uint32_t u[kWords];
+
+    // Elements [c, c + kN), zeros past `cols`; kBytes: what the row's
+    // alignment lets one load take.
+    template <int kBytes>
+    __device__ __forceinline__ void load(const T* row, long long c, long long cols) {
+        if (kBytes >= 4 && c + kN <= cols) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-        *reinterpret_cast<uint4*>(row + c) = q;
-    } else if constexpr (kVec) {
-        float4* p = reinterpret_cast<float4*>(row + c);
-        p[0] = make_float4(v[0], v[1], v[2], v[3]);
-        p[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
+            for (int i = 0; i < kWords; i += kBytes / 4)
+                load_piece<kBytes>(u + i, reinterpret_cast<const uint8_t*>(row + c) + 4 * i);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (c + i < cols) row[c + i] = T(v[i]);
+            for (int i = 0; i < kWords; ++i) {
+                if constexpr (sizeof(T) == 4) {
+                    u[i] = c + i < cols ? __ldg(reinterpret_cast<const uint32_t*>(row + c) + i) : 0u;
+                } else {
+                    const uint16_t* h = reinterpret_cast<const uint16_t*>(row + c) + 2 * i;
+                    u[i] = c + 2 * i < cols ? __ldg(h) : 0u;
+                    if (c + 2 * i + 1 < cols) u[i] |= uint32_t(__ldg(h + 1)) << 16;
+                }
+            }
+        }
     }
-}
+    // The largest magnitude's exponent field (255: an infinity or a NaN).
+    // Magnitudes compare as their bits do.
+    __device__ __forceinline__ uint32_t top_field() const {
+        if constexpr (sizeof(T) == 4) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) top = max(top, u[i] & 0x7FFFFFFFu);
+            return top >> 23;
+        } else {
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) top = __vmaxu2(top, u[i] & 0x7FFF7FFFu);
+            return max(top >> 16, top & 0xFFFFu) >> 7;
+        }
+    }
+    // Codes of elements [8 i, 8 i + 8) over the scale 2^(code - 127). The
+    // product with the scale's reciprocal is exact (in bfloat16 too) unless it
+    // is far below the smallest magnitude's half.
+    __device__ __forceinline__ uint32_t codes(int i, uint32_t code) const {
+        if (code == 255) return 0u;
+        float y[8];
+        if constexpr (sizeof(T) == 4) {
+            const float inv = __uint_as_float((254u - code) << 23);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(u[8 * i + e]) * inv;
+        } else {
+            const uint32_t h = (254u - code) << 7, hh = h | h << 16;
+            const __nv_bfloat162 inv = *reinterpret_cast<const __nv_bfloat162*>(&hh);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const __nv_bfloat162 t = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&u[4 * i + e]), inv);
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(&t);
+                y[2 * e] = __uint_as_float(w << 16);
+                y[2 * e + 1] = __uint_as_float(w & 0xFFFF0000u);
+            }
+        }
+        return pack_e2m1(y);
+    }
+};
+
+// The scale code (exponent + 127) of a block whose largest magnitude has this
+// exponent field.
+__device__ __forceinline__ uint32_t scale_code(uint32_t field) { return field == 255 ? 255u : field > 2 ? field - 2 : 0u; }
 
 __device__ __forceinline__ size_t scale_offset(const MxShape& s, long long row, long long block) {
     return size_t((row >> 7) * s.scale_tiles() + (block >> 2)) * 512 + size_t(row & 31) * 16 +
@@ -106,103 +143,118 @@ __device__ __forceinline__ size_t scale_offset(const MxShape& s, long long row, 
 
 // ---------------------------------------------------------- quantisation
 
-// One thread takes 8 elements, four neighbours one block: a warp's load is
-// 256 consecutive elements. The block's maximum is an integer maximum of
-// magnitudes (an infinity or NaN has the largest), over the four threads.
-// A warp item is kCastSpan elements of one row, all loads in flight before
-// the first is used. Rows up to the next multiple of 128 and blocks up to
-// the next multiple of 4 are visited too: their scales are set to zero.
-constexpr int kCastThreads = 256, kCastUnroll = 4, kCastSpan = 256 * kCastUnroll;
+// A thread takes 16 elements, two neighbours one block; a warp 512 neighbours
+// of a row at a time, kCastUnroll of those with all loads in flight before
+// the first is used. blockIdx.y: the span of columns; rows are shared out
+// over blockIdx.x and the block's warps. Rows up to the next multiple of 128
+// and blocks up to the next multiple of 4 are visited too: their scales are
+// set to zero. kBytes: the widest load that every row's alignment allows.
+constexpr int kCastThreads = 256, kCastWarps = kCastThreads / 32, kCastUnroll = 4, kCastStep = 512,
+              kCastSpan = kCastStep * kCastUnroll;
 
-template <typename T, bool kAligned>
+template <typename T, int kBytes>
 __global__ void __launch_bounds__(kCastThreads) mx4_quantise_kernel(const MxCastArgs a) {
     const MxShape s = a.shape;
     const int lane = threadIdx.x & 31;
-    const long long spans = (s.scale_tiles() * 128 + kCastSpan - 1) / kCastSpan;
-    const long long items = s.row_tiles() * 128 * spans;
-    const long long warps = (long long)gridDim.x * (kCastThreads / 32);
-    for (long long it = (long long)blockIdx.x * (kCastThreads / 32) + (threadIdx.x >> 5); it < items; it += warps) {
-        const long long row = it / spans, c0 = (it - row * spans) * kCastSpan + lane * 8;
+    const long long c0 = (long long)blockIdx.y * kCastSpan + lane * 16;
+    const long long rows = s.row_tiles() * 128, blocks = s.blocks(), tiles = s.scale_tiles();
+    for (long long row = (long long)blockIdx.x * kCastWarps + (threadIdx.x >> 5); row < rows; row += (long long)gridDim.x * kCastWarps) {
         const T* src = static_cast<const T*>(a.plain) + size_t(row) * size_t(a.ld);
-        float v[kCastUnroll][8];
+        const long long cols = row < s.rows ? s.cols : 0;
+        Run<T, 16> v[kCastUnroll];
+#pragma unroll
+        for (int u = 0; u < kCastUnroll; ++u) v[u].template load<kBytes>(src, c0 + u * kCastStep, cols);
+        uint8_t* codes = a.codes + size_t(row) * size_t(s.pitch());
+        uint8_t* scales = a.scales + scale_offset(s, row, 0);
 #pragma unroll
         for (int u = 0; u < kCastUnroll; ++u) {
-            const long long c = c0 + u * 256;
-            if (kAligned && row < s.rows && c + 8 <= s.cols) load8<T, true>(src, c, s.cols, v[u]);
-            else load8<T, false>(src, c, row < s.rows ? s.cols : 0, v[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < kCastUnroll; ++u) {
-            const long long c = c0 + u * 256, block = c >> 5;
-            uint32_t top = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[u][i]) & 0x7FFFFFFFu);
-            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-            const uint32_t field = top >> 23;
-            const bool bad = field == 255;
-            const uint32_t code = bad ? 255u : (field > 2 ? field - 2 : 0u);
-            const float inv = __uint_as_float((bad ? 127u : 254u - code) << 23);   // 1 / X
-            float y[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = bad ? 0.0f : v[u][i] * inv;
-            const uint32_t codes = pack_e2m1(y);
-            if (row < s.rows && block < s.blocks())
-                reinterpret_cast<uint32_t*>(a.codes + size_t(row) * size_t(s.pitch()))[c >> 3] = codes;
+            const long long c = c0 + u * kCastStep, block = c >> 5;
+            uint32_t field = v[u].top_field();
+            field = max(field, __shfl_xor_sync(0xFFFFFFFFu, field, 1));
+            const uint32_t code = scale_code(field);
+            if (row < s.rows && block < blocks)
+                *reinterpret_cast<uint2*>(codes + (c >> 1)) = make_uint2(v[u].codes(0, code), v[u].codes(1, code));
             // Four blocks' scales are one 4-byte word.
-            uint32_t word = code;
-            word |= __shfl_down_sync(0xFFFFFFFFu, code, 4) << 8;
-            word |= __shfl_down_sync(0xFFFFFFFFu, code, 8) << 16;
-            word |= __shfl_down_sync(0xFFFFFFFFu, code, 12) << 24;
-            if ((lane & 15) == 0 && (block >> 2) < s.scale_tiles())
-                *reinterpret_cast<uint32_t*>(a.scales + scale_offset(s, row, block)) = word;
+            uint32_t word = code | __shfl_down_sync(0xFFFFFFFFu, code, 2) << 8;
+            word |= __shfl_down_sync(0xFFFFFFFFu, word, 4) << 16;
+            if ((lane & 7) == 0 && (block >> 2) < tiles) *reinterpret_cast<uint32_t*>(scales + (block >> 2) * 512) = word;
         }
     }
     grid_launch_dependents();
 }
 
-template <typename T, bool kAligned>
+// The inverse, with the same split. A value is a code's magnitude times a
+// power of two: exact in either type (the smallest, 2^-128, is a subnormal
+// that both hold).
+template <typename T, int kBytes>
 __global__ void __launch_bounds__(kCastThreads) mx4_values_kernel(const MxCastArgs a) {
     const MxShape s = a.shape;
     const int lane = threadIdx.x & 31;
-    const long long spans = (s.cols + kCastSpan - 1) / kCastSpan;
-    const long long items = s.rows * spans;
-    const long long warps = (long long)gridDim.x * (kCastThreads / 32);
-    for (long long it = (long long)blockIdx.x * (kCastThreads / 32) + (threadIdx.x >> 5); it < items; it += warps) {
-        const long long row = it / spans, c0 = (it - row * spans) * kCastSpan + lane * 8;
-        uint32_t codes[kCastUnroll], scale[kCastUnroll];
+    const long long c0 = (long long)blockIdx.y * kCastSpan + lane * 16;
+    for (long long row = (long long)blockIdx.x * kCastWarps + (threadIdx.x >> 5); row < s.rows; row += (long long)gridDim.x * kCastWarps) {
+        const uint8_t* codes = a.codes + size_t(row) * size_t(s.pitch());
+        const uint8_t* scales = a.scales + scale_offset(s, row, 0);
+        uint2 q[kCastUnroll];
+        uint32_t scale[kCastUnroll];
 #pragma unroll
         for (int u = 0; u < kCastUnroll; ++u) {
-            const long long c = c0 + u * 256;
+            const long long c = c0 + u * kCastStep, block = c >> 5;
             const bool in = c < s.cols;
-            codes[u] = in ? __ldg(reinterpret_cast<const uint32_t*>(a.codes + size_t(row) * size_t(s.pitch())) + (c >> 3)) : 0u;
-            scale[u] = in ? __ldg(a.scales + scale_offset(s, row, c >> 5)) : 0u;
+            q[u] = in ? __ldg(reinterpret_cast<const uint2*>(codes + (c >> 1))) : make_uint2(0, 0);
+            scale[u] = in ? __ldg(scales + (block >> 2) * 512 + (block & 3)) : 0u;
         }
         T* dst = static_cast<T*>(a.plain) + size_t(row) * size_t(a.ld);
 #pragma unroll
         for (int u = 0; u < kCastUnroll; ++u) {
-            const long long c = c0 + u * 256;
+            const long long c = c0 + u * kCastStep;
             if (c >= s.cols) continue;
-            float v[8];
-            unpack_e2m1(codes[u], v);
             // 2^(code - 127): code 0 is the subnormal 2^-127, code 255 NaN.
-            const float x = scale[u] == 255 ? __uint_as_float(0x7FC00000u)
-                                            : __uint_as_float(scale[u] ? scale[u] << 23 : 0x00400000u);
+            const float x = __uint_as_float(scale[u] == 255 ? 0x7FC00000u : scale[u] ? scale[u] << 23 : 0x00400000u);
+            float v[16];
+            unpack_e2m1(q[u].x, v);
+            unpack_e2m1(q[u].y, v + 8);
+            constexpr int kWords = 16 * int(sizeof(T)) / 4;
+            uint32_t w[kWords];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] *= x;
-            if (kAligned && c + 8 <= s.cols) store8<T, true>(dst, c, s.cols, v);
-            else store8<T, false>(dst, c, s.cols, v);
+            for (int i = 0; i < kWords; ++i) {
+                if constexpr (sizeof(T) == 4) {
+                    w[i] = __float_as_uint(v[i] * x);
+                } else {
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i] * x, v[2 * i + 1] * x);
+                    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+                }
+            }
+            uint8_t* to = reinterpret_cast<uint8_t*>(dst + c);
+            if (kBytes >= 4 && c + 16 <= s.cols) {
+#pragma unroll
+                for (int i = 0; i < kWords; i += kBytes / 4) {
+                    if constexpr (kBytes == 16) *reinterpret_cast<uint4*>(to + 4 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+                    else if constexpr (kBytes == 8) *reinterpret_cast<uint2*>(to + 4 * i) = make_uint2(w[i], w[i + 1]);
+                    else *reinterpret_cast<uint32_t*>(to + 4 * i) = w[i];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    if (c + i >= s.cols) break;
+                    if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(to)[i] = w[i];
+                    else reinterpret_cast<uint16_t*>(to)[i] = uint16_t(w[i >> 1] >> (i & 1 ? 16 : 0));
+                }
+            }
         }
     }
 }
 
-int cast_grid(long long items, int sms) {
-    const long long ctas = (items + kCastThreads / 32 - 1) / (kCastThreads / 32);
-    return int(std::min<long long>(ctas, (long long)sms * 8));
+// The widest load or store (16, 8, 4 bytes, or one 2-byte element) that the
+// alignment of every row allows.
+int row_bytes(const void* p, long long rows, long long ld, int type) {
+    const uintptr_t low = reinterpret_cast<uintptr_t>(p) | (rows > 1 ? uintptr_t(ld) * elem_size(type) : 0);
+    return low % 16 == 0 ? 16 : low % 8 == 0 ? 8 : low % 4 == 0 ? 4 : 2;
 }
 
-bool rows_aligned(const MxCastArgs& a) {
-    return reinterpret_cast<uintptr_t>(a.plain) % 16 == 0 && (a.shape.rows == 1 || size_t(a.ld) * elem_size(a.type) % 16 == 0);
+dim3 cast_grid(long long rows, long long cols, int sms) {
+    const long long spans = (cols + kCastSpan - 1) / kCastSpan;
+    const long long most = std::max<long long>(1, (long long)sms * 8 / spans);   // eight blocks an SM in all
+    return dim3(unsigned(std::min((rows + kCastWarps - 1) / kCastWarps, most)), unsigned(spans));
 }
 
 // --------------------------------------------------------------- product
@@ -230,7 +282,7 @@ struct ProductTile {
     int early_w;           // w and its scales may be read before the previous launch ends
 };
 
-constexpr int kPTile = 128, kPChunkBytes = 128, kPThreads = 192, kPMaxStages = 8;
+constexpr int kPTile = 128, kPChunkBytes = 128, kPThreads = 192, kPMaxStages = 8, kPMaxSplits = 8;
 constexpr uint32_t kPWBytes = kPTile * kPChunkBytes;
 
 __host__ __device__ constexpr int scale_groups(int tn) { return (tn + 127) / 128; }
@@ -239,13 +291,17 @@ __host__ __device__ constexpr uint32_t stage_bytes(int tn) {
 }
 __host__ __device__ constexpr uint32_t stage_scale_cols(int tn) { return 8u + 8u * uint32_t(scale_groups(tn)); }
 
-// 128 scale words (512 bytes at saddr) into 4 TMEM columns, in all four lane
-// quarters.
-__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint32_t saddr) {
+// The descriptor of 128 scale words (512 bytes at saddr) for tmem_copy_scales.
+__device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
     uint64_t d = static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
     d |= static_cast<uint64_t>(128 >> 4) << 32;   // stride between groups of 8 rows of 16 bytes
     d |= 1ull << 46;                              // fixed 0b001; no swizzle
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+    return d;
+}
+
+// 128 scale words into 4 TMEM columns, in all four lane quarters.
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
 // kind::mxf4: E2M1 operands, one E8M0 scale per 32 elements of K (two per
@@ -271,6 +327,16 @@ __device__ __forceinline__ uint32_t mx4_idesc(int n, uint32_t sf_id) {
            | (sf_id << 29);                        // A's scales
 }
 
+// One thread of the (whole, converged) warp. A branch on this tells the
+// compiler that a single thread issues: the tensor core's and TMA's operands
+// are uniform registers, which under `lane == 0` it filled through a loop
+// over the lanes (8192^3: 561 us under `lane == 0`, 389 us so).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 template <typename T>
 __device__ __forceinline__ void store_out(const ProductTile& p, int row, int col, float v, float bias) {
     v += bias;
@@ -278,7 +344,8 @@ __device__ __forceinline__ void store_out(const ProductTile& p, int row, int col
     static_cast<T*>(p.out)[size_t(row) * size_t(p.ld) + size_t(col)] = T(v);
 }
 
-template <typename T>
+// kGroups: scale tiles of 128 rows of x (tn <= 128: 1, else 2).
+template <typename T, int kGroups>
 __global__ void __launch_bounds__(kPThreads, 1)
     mx4_product_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap mx, const ProductTile p) {
     extern __shared__ uint8_t smem_raw[];
@@ -286,13 +353,12 @@ __global__ void __launch_bounds__(kPThreads, 1)
     __shared__ __align__(8) uint64_t full[kPMaxStages], empty[kPMaxStages], done;
     __shared__ uint32_t tmem_slot;
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xFFFFFFFFu, int(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
     const int split = int(blockIdx.x) % p.splits;
     const int n0 = int(blockIdx.x) / p.splits * kPTile, x0 = int(blockIdx.y) * p.tn;
     // This CTA's chunks of K: an even share, in order.
     const int c_begin = int((long long)p.chunks * split / p.splits);
     const int c_end = int((long long)p.chunks * (split + 1) / p.splits);
-    const int groups = scale_groups(p.tn);
     const uint32_t stage = stage_bytes(p.tn), x_bytes = uint32_t(p.tn) * kPChunkBytes;
     const int x_tile = x0 >> 7, x_tiles = (p.m + 127) >> 7;
     const uint32_t scale_col0 = uint32_t(max(p.tn, 32));
@@ -313,9 +379,9 @@ __global__ void __launch_bounds__(kPThreads, 1)
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
 
-    if (warp == 0 && lane == 0) {
+    if (warp == 0 && elect_one()) {
         auto scale_bytes = [&](int c) { return min(2, p.scale_tiles - 2 * c) * 512; };
-        auto x_groups = [&] { return min(groups, x_tiles - x_tile); };
+        auto x_groups = [&] { return min(kGroups, x_tiles - x_tile); };
         auto load_w = [&](int c, int s) {   // arms the barrier for the whole stage
             uint8_t* b = base + size_t(s) * stage;
             const uint32_t sb = uint32_t(scale_bytes(c));
@@ -348,30 +414,39 @@ __global__ void __launch_bounds__(kPThreads, 1)
         // (the MMA warp has waited for them unless a wait ran out).
         for (int i = max(0, loaded - p.stages); i < loaded; ++i)
             mbar_wait(&full[i % p.stages], uint32_t(i / p.stages) & 1u, &g_mx4_error, kErrWaitDrain);
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1 && elect_one()) {
         Ring r;
-        bool first = true;
+        uint32_t more = 0;   // the tile's first MMA overwrites
+        const uint32_t idesc[2] = {mx4_idesc(p.tn, 0), mx4_idesc(p.tn, 2)};
+        const uint32_t x_off = uint32_t(x0 & 127) >> 5;
+        // One scale tile (128 elements of K): its scales to TMEM, then its two
+        // MMAs (the tile's second half may be past K: then one).
+        auto tile = [&](uint32_t b, uint32_t tw, int t, bool both) {
+            const uint32_t tx = tw + 8;
+            const uint64_t sw = scale_desc(b + kPWBytes + x_bytes) + uint64_t(t * 32), sx = sw + 64;
+            tmem_copy_scales(tw + uint32_t(t) * 4, sw);
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) tmem_copy_scales(tx + uint32_t(t * kGroups + g) * 4, sx + uint64_t(g * 64));
+            const uint64_t da = sw128_desc(b) + uint64_t(4 * t), db = sw128_desc(b + kPWBytes) + uint64_t(4 * t);
+            const uint32_t fx = tx + uint32_t(t * kGroups) * 4 + x_off;
+            umma_mx4(tmem, da, db, idesc[0], tw + uint32_t(t) * 4, fx, more);
+            more = 1;
+            if (both) umma_mx4(tmem, da + 2, db + 2, idesc[1], tw + uint32_t(t) * 4, fx, 1);
+        };
         for (int c = c_begin; c < c_end; ++c) {
             if (!mbar_wait(&full[r.idx], r.phase, &g_mx4_error, kErrWaitMma)) break;
             tc_fence_after();
             const uint32_t b = smem_u32(base) + r.idx * stage;
-            const uint32_t sw = b + kPWBytes + x_bytes, sx = sw + 1024;
-            const uint32_t tw = tmem + scale_col0 + r.idx * stage_scale_cols(p.tn), tx = tw + 8;
-            const int tiles = min(2, p.scale_tiles - 2 * c);
             // Each stage has its own scale columns: they are overwritten only
             // once the MMAs that read them have freed the stage.
-            for (int t = 0; t < tiles; ++t) {
-                tmem_copy_scales(tw + uint32_t(t) * 4, sw + uint32_t(t) * 512);
-                for (int g = 0; g < groups; ++g)
-                    tmem_copy_scales(tx + uint32_t(t * groups + g) * 4, sx + uint32_t(g) * 1024 + uint32_t(t) * 512);
-            }
-            const uint64_t da = sw128_desc(b), db = sw128_desc(b + kPWBytes);
-            const int steps = min(4, p.steps - 4 * c);
-            for (int k = 0; k < steps; ++k) {
-                const uint32_t t = uint32_t(k) >> 1;
-                umma_mx4(tmem, da + uint64_t(2 * k), db + uint64_t(2 * k), mx4_idesc(p.tn, (uint32_t(k) & 1u) * 2u),
-                         tw + t * 4, tx + t * uint32_t(groups) * 4 + (uint32_t(x0 & 127) >> 5), first ? 0u : 1u);
-                first = false;
+            const uint32_t tw = tmem + scale_col0 + r.idx * stage_scale_cols(p.tn);
+            const int steps = p.steps - 4 * c;
+            if (steps >= 4) {
+                tile(b, tw, 0, true);
+                tile(b, tw, 1, true);
+            } else {
+                tile(b, tw, 0, steps > 1);
+                if (steps > 2) tile(b, tw, 1, false);
             }
             umma_commit(&empty[r.idx]);
             r.next(uint32_t(p.stages));
@@ -422,26 +497,322 @@ __global__ void __launch_bounds__(kPThreads, 1)
         // `split` finishes rows split, split + splits, ... of the tile.
         cluster_sync();
         if (warp >= 2) {
-            for (int i = split; i < live; i += p.splits) {
-                float sum = 0.0f;
-                for (int r = 0; r < p.splits; ++r) {
-                    const uint32_t a = mapa(smem_u32(part + i * kPTile + quarter * 32 + lane), uint32_t(r));
-                    float v;
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-                    sum += v;
+            constexpr int kAhead = 4;   // rows whose parts are all asked for before the first sum
+            for (int i0 = split; i0 < live; i0 += p.splits * kAhead) {
+                float v[kAhead][kPMaxSplits];
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    const int i = min(i0 + u * p.splits, live - 1);
+#pragma unroll
+                    for (int r = 0; r < kPMaxSplits; ++r)
+                        if (r < p.splits) {
+                            const uint32_t a = mapa(smem_u32(part + i * kPTile + quarter * 32 + lane), uint32_t(r));
+                            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[u][r]) : "r"(a) : "memory");
+                        }
                 }
-                if (j < p.n) store_out<T>(p, x0 + i, j, sum, bias);
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    const int i = i0 + u * p.splits;
+                    float sum = v[u][0];
+#pragma unroll
+                    for (int r = 1; r < kPMaxSplits; ++r)
+                        if (r < p.splits) sum += v[u][r];
+                    if (i < live && j < p.n) store_out<T>(p, x0 + i, j, sum, bias);
+                }
             }
         }
         cluster_sync();
     }
 }
 
-template <typename T>
+// ------------------------------------------------- product by CTA pairs
+
+// Large products: the two CTAs of a cluster compute 256 x 256 tiles together
+// (cta_group::2, M = 256). Each stages 128 rows of either operand, so that a
+// tile's operands cross from L2 to 2/3 of the bytes that 128 x 256 tiles take
+// (those were bound by L2: 8192^3 at 12 TB/s of it). Persistent: a pair takes
+// every (number of pairs)-th tile, and its copies run ahead into the next
+// tile while the epilogue drains. The epilogue's eight warps read their whole
+// share of the accumulator into registers and free it before converting and
+// storing.
+//
+// kRowsOnLanes: TMEM's lanes are rows of x, so a thread holds neighbouring
+// outputs of one row and stores 16 bytes at a time (p.vec: `out` is aligned
+// for that); otherwise they are rows of w and a warp stores 32 neighbouring
+// outputs at a time, whatever the alignment.
+struct PairTile {
+    int lanes, cols;                 // rows of the operand on the lanes and of the other
+    int lane_tiles, tiles;           // tiles along the lanes, and in all
+    int chunks, steps, scale_tiles;  // as in ProductTile
+    const float* bias;
+    int relu;
+    void* out;
+    long long ld;
+};
+
+constexpr int kPairFromTiles = 32;
+constexpr int kPairThreads = 320, kPairEpiWarps = 8, kPairStages = 6;
+constexpr uint32_t kPairScaleCols = 24, kPairTmemCols = 512;   // per stage: 2 x 4 of the lanes' scales, 2 x 8 of the columns'
+constexpr uint32_t kPairStageBytes = 2 * kPWBytes + 1024 + 2048;
+
+__device__ __forceinline__ void tmem_copy_scales_pair(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+__device__ __forceinline__ void umma_mx4_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa,
+                                              uint32_t sfb, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+
+template <typename T, bool kRowsOnLanes>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    mx4_pair_kernel(const __grid_constant__ CUtensorMap ml, const __grid_constant__ CUtensorMap mc,
+                    const __grid_constant__ CUtensorMap sl, const __grid_constant__ CUtensorMap sc, const PairTile p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    __shared__ __align__(8) uint64_t full[kPairStages], empty[kPairStages], acc_full, acc_empty, done;
+    __shared__ uint32_t tmem_slot;
+    const int warp = __shfl_sync(0xFFFFFFFFu, int(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const int pairs = int(gridDim.x) >> 1;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kPairStages; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        mbar_init(&acc_full, 1);
+        mbar_init(&acc_empty, 2 * kPairEpiWarps);   // every epilogue warp of both CTAs
+        mbar_init(&done, 1);
+        fence_barrier_init();
+        tma_prefetch_map(&ml);
+        tma_prefetch_map(&mc);
+        tma_prefetch_map(&sl);
+        tma_prefetch_map(&sc);
+    }
+    if (warp == 1) tmem_alloc_pair(&tmem_slot, kPairTmemCols);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();   // both CTAs' barriers exist before either addresses the other's
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    grid_dependency_wait();
+
+    if (warp == 0) {
+        if (elect_one()) {
+            Ring r;
+            uint32_t issued = 0;
+            const uint32_t full0 = mapa(smem_u32(full), 0);   // both CTAs' copies complete on the leader's barriers
+            bool ok = true;
+            for (int tile = int(blockIdx.x) >> 1; tile < p.tiles && ok; tile += pairs) {
+                const int tl = tile % p.lane_tiles, tc = tile / p.lane_tiles;
+                const int yl = tl * 256 + int(rank) * 128, yc = tc * 256 + int(rank) * 128;
+                const int zl = (yl >> 7) * p.scale_tiles, zc = 2 * tc * p.scale_tiles;
+                for (int c = 0; c < p.chunks; ++c) {
+                    if (!(ok = mbar_wait(&empty[r.idx], r.phase ^ 1u, &g_mx4_error, kErrWaitProducer))) break;
+                    if (rank == 0) mbar_arrive_expect_tx(&full[r.idx], 2 * kPairStageBytes);
+                    uint8_t* b = base + r.idx * kPairStageBytes;
+                    const uint32_t bar = full0 + r.idx * 8u;
+                    tma_load_2d_pair(&ml, b, bar, c * kPChunkBytes, yl);
+                    tma_load_2d_pair(&mc, b + kPWBytes, bar, c * kPChunkBytes, yc);
+                    // Two scale tiles of 512 bytes at a time. Past an odd last one
+                    // this reads another row tile's (or zeros), which no MMA uses.
+                    tma_load_2d_pair(&sl, b + 2 * kPWBytes, bar, 0, zl + 2 * c);
+                    tma_load_2d_pair(&sc, b + 2 * kPWBytes + 1024, bar, 0, zc + 2 * c);
+                    tma_load_2d_pair(&sc, b + 2 * kPWBytes + 2048, bar, 0, zc + p.scale_tiles + 2 * c);
+                    r.next(kPairStages);
+                    ++issued;
+                }
+            }
+            // The leader's full barriers count both CTAs' copies: once each
+            // stage's last phase has completed, every copy of the pair has landed.
+            if (rank == 0)
+                for (uint32_t i = issued > kPairStages ? issued - kPairStages : 0; i < issued; ++i)
+                    mbar_wait(&full[i % kPairStages], (i / kPairStages) & 1u, &g_mx4_error, kErrWaitDrain);
+        }
+    } else if (warp == 1) {
+        if (rank == 0 && elect_one()) {
+            Ring r;
+            uint32_t j = 0;
+            bool ok = true;
+            const uint32_t empty0 = mapa(smem_u32(empty), 0), empty1 = mapa(smem_u32(empty), 1);
+            const uint32_t full_a = mapa(smem_u32(&acc_full), 0), full_b = mapa(smem_u32(&acc_full), 1);
+            constexpr uint32_t kIdesc = (1u << 7) | (1u << 10) | (uint32_t(256 >> 3) << 17) | (1u << 23) | (uint32_t(256 >> 4) << 24);
+            constexpr uint32_t kSecond = (2u << 4) | (2u << 29);   // the scale words' upper two bytes
+            for (int tile = int(blockIdx.x) >> 1; tile < p.tiles && ok; tile += pairs, ++j) {
+                if (!(ok = mbar_wait_cluster(&acc_empty, (j & 1u) ^ 1u, &g_mx4_error, kErrWaitMma))) break;
+                tc_fence_after();
+                uint32_t more = 0;
+                for (int c = 0; c < p.chunks; ++c) {
+                    if (!(ok = mbar_wait(&full[r.idx], r.phase, &g_mx4_error, kErrWaitMma))) break;
+                    tc_fence_after();
+                    const uint32_t b = smem_u32(base) + r.idx * kPairStageBytes;
+                    const uint32_t tw = tmem + 256u + r.idx * kPairScaleCols;
+                    auto tile_of = [&](int t, bool both) {
+                        const uint64_t z = scale_desc(b + 2 * kPWBytes) + uint64_t(t * 32);
+                        const uint32_t fl = tw + uint32_t(t) * 4, fc = tw + 8 + uint32_t(t) * 8;
+                        tmem_copy_scales_pair(fl, z);
+                        tmem_copy_scales_pair(fc, z + 64);
+                        tmem_copy_scales_pair(fc + 4, z + 128);
+                        const uint64_t da = sw128_desc(b) + uint64_t(4 * t), db = sw128_desc(b + kPWBytes) + uint64_t(4 * t);
+                        umma_mx4_pair(tmem, da, db, kIdesc, fl, fc, more);
+                        more = 1;
+                        if (both) umma_mx4_pair(tmem, da + 2, db + 2, kIdesc | kSecond, fl, fc, 1);
+                    };
+                    const int steps = p.steps - 4 * c;
+                    if (steps >= 4) {
+                        tile_of(0, true);
+                        tile_of(1, true);
+                    } else {
+                        tile_of(0, steps > 1);
+                        if (steps > 2) tile_of(1, false);
+                    }
+                    umma_commit_pair(empty0 + r.idx * 8u);
+                    umma_commit_pair(empty1 + r.idx * 8u);
+                    r.next(kPairStages);
+                }
+                if (!ok) break;
+                umma_commit_pair(full_a);
+                umma_commit_pair(full_b);
+            }
+            umma_commit_pair(mapa(smem_u32(&done), 0));
+            mbar_wait(&done, 0, &g_mx4_error, kErrWaitDrain);
+        }
+    } else {
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        const uint32_t taddr = tmem + (uint32_t(quarter) << 21) + uint32_t(half) * 128;
+        const uint32_t to_leader = mapa(smem_u32(&acc_empty), 0);
+        T* const out = static_cast<T*>(p.out);
+        uint32_t j = 0;
+        for (int tile = int(blockIdx.x) >> 1; tile < p.tiles; tile += pairs, ++j) {
+            if (!mbar_wait(&acc_full, j & 1u, &g_mx4_error, kErrWaitEpilogue)) break;
+            tc_fence_after();
+            uint32_t v[4][32];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) tmem_ld32(taddr + uint32_t(q) * 32, v[q]);
+            tmem_wait_ld();
+#pragma unroll
+            for (int q = 0; q < 4; ++q) tmem_hold(v[q]);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(to_leader);
+            const int l = (tile % p.lane_tiles) * 256 + int(rank) * 128 + quarter * 32 + lane;
+            const int c0 = tile / p.lane_tiles * 256 + half * 128;
+            const auto act = [&](uint32_t bits, float bias) {
+                const float y = __uint_as_float(bits) + bias;
+                return p.relu && y < 0.0f ? 0.0f : y;   // keeps a NaN
+            };
+            if constexpr (kRowsOnLanes) {
+                if (l >= p.lanes) continue;
+                T* const dst = out + size_t(l) * size_t(p.ld) + c0;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    constexpr int kW = 16 / int(sizeof(T));
+#pragma unroll
+                    for (int i = 0; i < 32; i += kW) {
+                        const int c = c0 + q * 32 + i;
+                        float y[kW];
+#pragma unroll
+                        for (int e = 0; e < kW; ++e) y[e] = act(v[q][i + e], p.bias && c + e < p.cols ? __ldg(p.bias + c + e) : 0.0f);
+                        if (c + kW <= p.cols) {
+                            uint4 w;
+                            if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                                for (int e = 0; e < kW; e += 2)
+                                    reinterpret_cast<__nv_bfloat162*>(&w)[e >> 1] = __floats2bfloat162_rn(y[e], y[e + 1]);
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < kW; ++e) reinterpret_cast<float*>(&w)[e] = y[e];
+                            }
+                            *reinterpret_cast<uint4*>(dst + q * 32 + i) = w;
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < kW; ++e)
+                                if (c + e < p.cols) dst[q * 32 + i + e] = T(y[e]);
+                        }
+                    }
+                }
+            } else {
+                if (l >= p.lanes) continue;
+                const float bias = p.bias ? __ldg(p.bias + l) : 0.0f;
+                T* dst = out + size_t(c0) * size_t(p.ld) + l;
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        if (c0 + q * 32 + i < p.cols) *dst = T(act(v[q][i], bias));
+                        dst += p.ld;
+                    }
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();   // no remote arrival or pair MMA is still in flight
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem, kPairTmemCols);
+    }
+}
+
+template <typename T, bool kRowsOnLanes>
+cudaError_t launch_pair(const MxProductArgs& a, int sms, cudaStream_t s) {
+    const MxShape xs{a.m, a.k}, ws{a.n, a.k};
+    const MxShape& ls = kRowsOnLanes ? xs : ws;
+    const MxShape& cs = kRowsOnLanes ? ws : xs;
+    const uint8_t* lc = kRowsOnLanes ? a.x_codes : a.w_codes;
+    const uint8_t* cc = kRowsOnLanes ? a.w_codes : a.x_codes;
+    const uint8_t* lsc = kRowsOnLanes ? a.x_scales : a.w_scales;
+    const uint8_t* csc = kRowsOnLanes ? a.w_scales : a.x_scales;
+    PairTile p{};
+    p.lanes = int(ls.rows);
+    p.cols = int(cs.rows);
+    p.lane_tiles = int((ls.rows + 255) / 256);
+    p.tiles = p.lane_tiles * int((cs.rows + 255) / 256);
+    p.chunks = int((a.k + 255) / 256);
+    p.steps = int((a.k + 63) / 64);
+    p.scale_tiles = int(ls.scale_tiles());
+    p.bias = a.bias;
+    p.relu = a.relu;
+    p.out = a.out;
+    p.ld = a.ld;
+    const CUtensorMap ml = make_byte_map(lc, uint64_t(ls.pitch()), uint64_t(ls.rows), 128);
+    const CUtensorMap mc = make_byte_map(cc, uint64_t(cs.pitch()), uint64_t(cs.rows), 128);
+    const CUtensorMap sl = make_scale_map(lsc, uint64_t(ls.row_tiles()) * uint64_t(ls.scale_tiles()));
+    const CUtensorMap sc = make_scale_map(csc, uint64_t(cs.row_tiles()) * uint64_t(cs.scale_tiles()));
+    const size_t smem = 1024 + size_t(kPairStages) * kPairStageBytes;
+    if (const cudaError_t e = open_smem<mx4_pair_kernel<T, kRowsOnLanes>>(smem); e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(2 * std::min(p.tiles, sms / 2)));
+    cfg.blockDim = dim3(kPairThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {2, 1, 1};
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = a.after_quantise ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, mx4_pair_kernel<T, kRowsOnLanes>, ml, mc, sl, sc, p);
+}
+
+// Whether rows of `out` can be stored 16 bytes at a time.
+bool out_aligned(const MxProductArgs& a) {
+    return reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && size_t(a.ld) * elem_size(a.type) % 16 == 0;
+}
+
+template <typename T, int kGroups>
 cudaError_t launch_product_t(const CUtensorMap& mw, const CUtensorMap& mx, const ProductTile& p, dim3 grid, bool pdl,
                              cudaStream_t s) {
     const size_t smem = 1024 + size_t(p.stages) * stage_bytes(p.tn);
-    if (const cudaError_t e = open_smem<mx4_product_kernel<T>>(smem); e != cudaSuccess) return e;
+    if (const cudaError_t e = open_smem<mx4_product_kernel<T, kGroups>>(smem); e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(kPThreads);
@@ -461,40 +832,48 @@ cudaError_t launch_product_t(const CUtensorMap& mw, const CUtensorMap& mx, const
     }
     cfg.attrs = attr;
     cfg.numAttrs = unsigned(na);
-    return cudaLaunchKernelEx(&cfg, mx4_product_kernel<T>, mw, mx, p);
+    return cudaLaunchKernelEx(&cfg, mx4_product_kernel<T, kGroups>, mw, mx, p);
 }
 
 }  // namespace
 
 cudaError_t launch_mx4_quantise(const MxCastArgs& a, int sms, cudaStream_t s) {
-    const MxShape& sh = a.shape;
-    const int grid = cast_grid(sh.row_tiles() * 128 * ((sh.scale_tiles() * 128 + kCastSpan - 1) / kCastSpan), sms);
-    const bool v = rows_aligned(a);
+    const dim3 grid = cast_grid(a.shape.row_tiles() * 128, a.shape.scale_tiles() * 128, sms);
+    const int bytes = row_bytes(a.plain, a.shape.rows, a.ld, a.type);
     if (a.type == kElemBF16) {
-        if (v) mx4_quantise_kernel<__nv_bfloat16, true><<<grid, kCastThreads, 0, s>>>(a);
-        else mx4_quantise_kernel<__nv_bfloat16, false><<<grid, kCastThreads, 0, s>>>(a);
+        if (bytes == 16) mx4_quantise_kernel<__nv_bfloat16, 16><<<grid, kCastThreads, 0, s>>>(a);
+        else if (bytes == 8) mx4_quantise_kernel<__nv_bfloat16, 8><<<grid, kCastThreads, 0, s>>>(a);
+        else if (bytes == 4) mx4_quantise_kernel<__nv_bfloat16, 4><<<grid, kCastThreads, 0, s>>>(a);
+        else mx4_quantise_kernel<__nv_bfloat16, 2><<<grid, kCastThreads, 0, s>>>(a);
     } else {
-        if (v) mx4_quantise_kernel<float, true><<<grid, kCastThreads, 0, s>>>(a);
-        else mx4_quantise_kernel<float, false><<<grid, kCastThreads, 0, s>>>(a);
+        if (bytes == 16) mx4_quantise_kernel<float, 16><<<grid, kCastThreads, 0, s>>>(a);
+        else if (bytes == 8) mx4_quantise_kernel<float, 8><<<grid, kCastThreads, 0, s>>>(a);
+        else mx4_quantise_kernel<float, 4><<<grid, kCastThreads, 0, s>>>(a);
     }
     return cudaGetLastError();
 }
 
 cudaError_t launch_mx4_values(const MxCastArgs& a, int sms, cudaStream_t s) {
-    const MxShape& sh = a.shape;
-    const int grid = cast_grid(sh.rows * ((sh.cols + kCastSpan - 1) / kCastSpan), sms);
-    const bool v = rows_aligned(a);
+    const dim3 grid = cast_grid(a.shape.rows, a.shape.cols, sms);
+    const int bytes = row_bytes(a.plain, a.shape.rows, a.ld, a.type);
     if (a.type == kElemBF16) {
-        if (v) mx4_values_kernel<__nv_bfloat16, true><<<grid, kCastThreads, 0, s>>>(a);
-        else mx4_values_kernel<__nv_bfloat16, false><<<grid, kCastThreads, 0, s>>>(a);
+        if (bytes == 16) mx4_values_kernel<__nv_bfloat16, 16><<<grid, kCastThreads, 0, s>>>(a);
+        else if (bytes == 8) mx4_values_kernel<__nv_bfloat16, 8><<<grid, kCastThreads, 0, s>>>(a);
+        else if (bytes == 4) mx4_values_kernel<__nv_bfloat16, 4><<<grid, kCastThreads, 0, s>>>(a);
+        else mx4_values_kernel<__nv_bfloat16, 2><<<grid, kCastThreads, 0, s>>>(a);
     } else {
-        if (v) mx4_values_kernel<float, true><<<grid, kCastThreads, 0, s>>>(a);
-        else mx4_values_kernel<float, false><<<grid, kCastThreads, 0, s>>>(a);
+        if (bytes == 16) mx4_values_kernel<float, 16><<<grid, kCastThreads, 0, s>>>(a);
+        else if (bytes == 8) mx4_values_kernel<float, 8><<<grid, kCastThreads, 0, s>>>(a);
+        else mx4_values_kernel<float, 4><<<grid, kCastThreads, 0, s>>>(a);
     }
     return cudaGetLastError();
 }
 
 cudaError_t launch_mx4_product(const MxProductArgs& a, int sms, cudaStream_t s) {
+    if (a.m > 128 && a.n > 128 && (a.m + 255) / 256 * ((a.n + 255) / 256) >= kPairFromTiles) {
+        if (a.type == kElemBF16) return out_aligned(a) ? launch_pair<__nv_bfloat16, true>(a, sms, s) : launch_pair<__nv_bfloat16, false>(a, sms, s);
+        return out_aligned(a) ? launch_pair<float, true>(a, sms, s) : launch_pair<float, false>(a, sms, s);
+    }
     const MxShape xs{a.m, a.k}, ws{a.n, a.k};
     ProductTile p{};
     p.m = int(a.m);
@@ -511,10 +890,9 @@ cudaError_t launch_mx4_product(const MxProductArgs& a, int sms, cudaStream_t s) 
         if (a.m > 128 && (a.m + tn - 1) / tn * n_tiles >= sms) p.tn = tn;
     const int x_tiles = int((a.m + p.tn - 1) / p.tn);
     // K is shared by a cluster of CTAs while the tiles leave SMs idle and
-    // every CTA keeps a chunk or more (the parts fit a stage's memory up to
-    // 64 columns).
+    // every CTA keeps a chunk or more.
     p.splits = 1;
-    while (p.tn <= 64 && p.splits < 8 && (long long)n_tiles * x_tiles * p.splits * 2 <= sms && p.splits * 2 <= p.chunks)
+    while (p.splits < kPMaxSplits && (long long)n_tiles * x_tiles * p.splits * 2 <= sms && p.splits * 2 <= p.chunks)
         p.splits *= 2;
     const int per_cta = (p.chunks + p.splits - 1) / p.splits;
     p.stages = int(std::min<size_t>(kPMaxStages, (size_t(220) << 10) / stage_bytes(p.tn)));
@@ -534,8 +912,9 @@ cudaError_t launch_mx4_product(const MxProductArgs& a, int sms, cudaStream_t s) 
     const CUtensorMap mw = make_byte_map(a.w_codes, uint64_t(ws.pitch()), uint64_t(a.n), kPTile);
     const CUtensorMap mx = make_byte_map(a.x_codes, uint64_t(xs.pitch()), uint64_t(a.m), uint32_t(p.tn));
     const dim3 grid(unsigned(n_tiles * p.splits), unsigned(x_tiles));
-    return a.type == kElemBF16 ? launch_product_t<__nv_bfloat16>(mw, mx, p, grid, a.after_quantise, s)
-                               : launch_product_t<float>(mw, mx, p, grid, a.after_quantise, s);
+    const auto go = a.type == kElemBF16 ? (p.tn > 128 ? launch_product_t<__nv_bfloat16, 2> : launch_product_t<__nv_bfloat16, 1>)
+                                        : (p.tn > 128 ? launch_product_t<float, 2> : launch_product_t<float, 1>);
+    return go(mw, mx, p, grid, a.after_quantise, s);
 }
 
 cudaError_t mx4_take_error(int* code) {

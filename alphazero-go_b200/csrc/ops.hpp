@@ -90,4 +90,7 @@ cudaError_t launch_sample_moves(const SampleArgs& a, int sms, cudaStream_t s);
 // 128 bytes x box_rows rows, 128-byte swizzle.
 CUtensorMap make_byte_map(const void* base, uint64_t pitch, uint64_t rows, uint32_t box_rows);
 
+// A map of `tiles` scale tiles of 512 bytes, in boxes of two.
+CUtensorMap make_scale_map(const void* base, uint64_t tiles);
+
 }  // namespace azb
