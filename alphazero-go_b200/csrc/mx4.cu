@@ -60,9 +60,9 @@ __device__ __forceinline__ void unpack_e2m1(uint32_t codes, float* v) {
 // kBytes (2 to 16) from global memory into the words at dst.
 template <int kBytes>
 __device__ __forceinline__ void load_piece(uint32_t* dst, const void* src) {
-    if constexpr (kBytes == 16) *reinterpret_cast<uint4*>(dst) = __ldg(static_cast<const uint4*>(src));
-    else if constexpr (kBytes == 8) *reinterpret_cast<uint2*>(dst) = __ldg(static_cast<const uint2*>(src));
-    else if constexpr (kBytes == 4) *dst = __ldg(static_cast<const uint32_t*>(src));
+    if constexpr (kBytes == 16) *reinterpret_cast<uint4*>(dst) = __ldcs(static_cast<const uint4*>(src));
+    else if constexpr (kBytes == 8) *reinterpret_cast<uint2*>(dst) = __ldcs(static_cast<const uint2*>(src));
+    else if constexpr (kBytes == 4) *dst = __ldcs(static_cast<const uint32_t*>(src));
 }
 
 // kN neighbouring elements of a row as they lie in memory (kN T in words).
@@ -149,11 +149,11 @@ __device__ __forceinline__ size_t scale_offset(const MxShape& s, long long row, 
 // over blockIdx.x and the block's warps. Rows up to the next multiple of 128
 // and blocks up to the next multiple of 4 are visited too: their scales are
 // set to zero. kBytes: the widest load that every row's alignment allows.
-constexpr int kCastThreads = 256, kCastWarps = kCastThreads / 32, kCastUnroll = 4, kCastStep = 512,
+constexpr int kCastThreads = 256, kCastWarps = kCastThreads / 32, kCastUnroll = 2, kCastStep = 512,
               kCastSpan = kCastStep * kCastUnroll;
 
 template <typename T, int kBytes>
-__global__ void __launch_bounds__(kCastThreads) mx4_quantise_kernel(const MxCastArgs a) {
+__global__ void __launch_bounds__(kCastThreads, 4) mx4_quantise_kernel(const MxCastArgs a) {
     const MxShape s = a.shape;
     const int lane = threadIdx.x & 31;
     const long long c0 = (long long)blockIdx.y * kCastSpan + lane * 16;
@@ -183,37 +183,38 @@ __global__ void __launch_bounds__(kCastThreads) mx4_quantise_kernel(const MxCast
     grid_launch_dependents();
 }
 
-// The inverse, with the same split. A value is a code's magnitude times a
+// The inverse; a thread takes 8 elements, so that a warp's 16-byte stores of
+// bfloat16 are neighbours. A value is a code's magnitude times a
 // power of two: exact in either type (the smallest, 2^-128, is a subnormal
 // that both hold).
+constexpr int kValuesUnroll = 4, kValuesStep = 256, kValuesSpan = kValuesStep * kValuesUnroll;
+
 template <typename T, int kBytes>
-__global__ void __launch_bounds__(kCastThreads) mx4_values_kernel(const MxCastArgs a) {
+__global__ void __launch_bounds__(kCastThreads, 5) mx4_values_kernel(const MxCastArgs a) {
     const MxShape s = a.shape;
     const int lane = threadIdx.x & 31;
-    const long long c0 = (long long)blockIdx.y * kCastSpan + lane * 16;
+    const long long c0 = (long long)blockIdx.y * kValuesSpan + lane * 8;
     for (long long row = (long long)blockIdx.x * kCastWarps + (threadIdx.x >> 5); row < s.rows; row += (long long)gridDim.x * kCastWarps) {
         const uint8_t* codes = a.codes + size_t(row) * size_t(s.pitch());
         const uint8_t* scales = a.scales + scale_offset(s, row, 0);
-        uint2 q[kCastUnroll];
-        uint32_t scale[kCastUnroll];
+        uint32_t q[kValuesUnroll], scale[kValuesUnroll];
 #pragma unroll
-        for (int u = 0; u < kCastUnroll; ++u) {
-            const long long c = c0 + u * kCastStep, block = c >> 5;
+        for (int u = 0; u < kValuesUnroll; ++u) {
+            const long long c = c0 + u * kValuesStep, block = c >> 5;
             const bool in = c < s.cols;
-            q[u] = in ? __ldg(reinterpret_cast<const uint2*>(codes + (c >> 1))) : make_uint2(0, 0);
+            q[u] = in ? __ldg(reinterpret_cast<const uint32_t*>(codes + (c >> 1))) : 0u;
             scale[u] = in ? __ldg(scales + (block >> 2) * 512 + (block & 3)) : 0u;
         }
         T* dst = static_cast<T*>(a.plain) + size_t(row) * size_t(a.ld);
 #pragma unroll
-        for (int u = 0; u < kCastUnroll; ++u) {
-            const long long c = c0 + u * kCastStep;
+        for (int u = 0; u < kValuesUnroll; ++u) {
+            const long long c = c0 + u * kValuesStep;
             if (c >= s.cols) continue;
             // 2^(code - 127): code 0 is the subnormal 2^-127, code 255 NaN.
             const float x = __uint_as_float(scale[u] == 255 ? 0x7FC00000u : scale[u] ? scale[u] << 23 : 0x00400000u);
-            float v[16];
-            unpack_e2m1(q[u].x, v);
-            unpack_e2m1(q[u].y, v + 8);
-            constexpr int kWords = 16 * int(sizeof(T)) / 4;
+            float v[8];
+            unpack_e2m1(q[u], v);
+            constexpr int kWords = 8 * int(sizeof(T)) / 4;
             uint32_t w[kWords];
 #pragma unroll
             for (int i = 0; i < kWords; ++i) {
@@ -225,16 +226,16 @@ __global__ void __launch_bounds__(kCastThreads) mx4_values_kernel(const MxCastAr
                 }
             }
             uint8_t* to = reinterpret_cast<uint8_t*>(dst + c);
-            if (kBytes >= 4 && c + 16 <= s.cols) {
+            if (kBytes >= 4 && c + 8 <= s.cols) {
 #pragma unroll
                 for (int i = 0; i < kWords; i += kBytes / 4) {
-                    if constexpr (kBytes == 16) *reinterpret_cast<uint4*>(to + 4 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
-                    else if constexpr (kBytes == 8) *reinterpret_cast<uint2*>(to + 4 * i) = make_uint2(w[i], w[i + 1]);
-                    else *reinterpret_cast<uint32_t*>(to + 4 * i) = w[i];
+                    if constexpr (kBytes == 16) __stcs(reinterpret_cast<uint4*>(to + 4 * i), make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]));
+                    else if constexpr (kBytes == 8) __stcs(reinterpret_cast<uint2*>(to + 4 * i), make_uint2(w[i], w[i + 1]));
+                    else __stcs(reinterpret_cast<uint32_t*>(to + 4 * i), w[i]);
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
+                for (int i = 0; i < 8; ++i) {
                     if (c + i >= s.cols) break;
                     if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(to)[i] = w[i];
                     else reinterpret_cast<uint16_t*>(to)[i] = uint16_t(w[i >> 1] >> (i & 1 ? 16 : 0));
@@ -251,9 +252,9 @@ int row_bytes(const void* p, long long rows, long long ld, int type) {
     return low % 16 == 0 ? 16 : low % 8 == 0 ? 8 : low % 4 == 0 ? 4 : 2;
 }
 
-dim3 cast_grid(long long rows, long long cols, int sms) {
-    const long long spans = (cols + kCastSpan - 1) / kCastSpan;
-    const long long most = std::max<long long>(1, (long long)sms * 8 / spans);   // eight blocks an SM in all
+dim3 cast_grid(long long rows, long long cols, int span, int sms) {
+    const long long spans = (cols + span - 1) / span;
+    const long long most = std::max<long long>(1, (long long)sms * 16 / spans);   // sixteen blocks an SM in all
     return dim3(unsigned(std::min((rows + kCastWarps - 1) / kCastWarps, most)), unsigned(spans));
 }
 
@@ -838,7 +839,7 @@ cudaError_t launch_product_t(const CUtensorMap& mw, const CUtensorMap& mx, const
 }  // namespace
 
 cudaError_t launch_mx4_quantise(const MxCastArgs& a, int sms, cudaStream_t s) {
-    const dim3 grid = cast_grid(a.shape.row_tiles() * 128, a.shape.scale_tiles() * 128, sms);
+    const dim3 grid = cast_grid(a.shape.row_tiles() * 128, a.shape.scale_tiles() * 128, kCastSpan, sms);
     const int bytes = row_bytes(a.plain, a.shape.rows, a.ld, a.type);
     if (a.type == kElemBF16) {
         if (bytes == 16) mx4_quantise_kernel<__nv_bfloat16, 16><<<grid, kCastThreads, 0, s>>>(a);
@@ -854,7 +855,7 @@ cudaError_t launch_mx4_quantise(const MxCastArgs& a, int sms, cudaStream_t s) {
 }
 
 cudaError_t launch_mx4_values(const MxCastArgs& a, int sms, cudaStream_t s) {
-    const dim3 grid = cast_grid(a.shape.rows, a.shape.cols, sms);
+    const dim3 grid = cast_grid(a.shape.rows, a.shape.cols, kValuesSpan, sms);
     const int bytes = row_bytes(a.plain, a.shape.rows, a.ld, a.type);
     if (a.type == kElemBF16) {
         if (bytes == 16) mx4_values_kernel<__nv_bfloat16, 16><<<grid, kCastThreads, 0, s>>>(a);
