@@ -285,7 +285,7 @@ struct Part {   // what one CTA knows of its slice
 
 struct RowShared {
     uint32_t hist_n[kBins], hist_w[kBins];   // this CTA's; then the lists
-    uint32_t all_n[kBins], all_w[kBins];     // the cluster's
+    uint32_t all_n[kBins], all_w[kBins];     // the cluster's; then the kept columns
     Part part[kMaxCluster];
     float f[2][kMaxCluster];
     int n[2][kMaxCluster];
@@ -293,11 +293,12 @@ struct RowShared {
     float best_x[kMaxCluster];
     float wf[kRowWarps], wg[kRowWarps], wh[kRowWarps];
     int wn[kRowWarps], wm[kRowWarps], wk[kRowWarps];
-    unsigned list_n;
+    unsigned list_n, kept_n;
     int first, last;
     float kept;
     uint64_t cut;
 };
+constexpr int kKept = 2 * kBins;   // columns that all_n and all_w hold
 static_assert(kList * 2 * 8 <= int(sizeof(uint32_t)) * kBins * 2, "a CTA's list and the merged one take the histogram's place");
 
 // The address of *p in CTA `rank` of the cluster.
@@ -380,6 +381,10 @@ struct Slice {
         if (l != l || (legal && !legal[i])) l = neg_inf();
         if (infinite) l = l == __uint_as_float(0x7F800000u) ? 0.0f : neg_inf();
         return l;
+    }
+    __device__ __forceinline__ float at(int i) const {
+        if constexpr (kResident) return float(reinterpret_cast<const T*>(mem)[shift + i]);
+        else return direct(i);
     }
     __device__ __forceinline__ int packs() const { return (shift + n + W - 1) / W; }
 
@@ -815,52 +820,91 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const Sample
             }
         }
         if (!raced) {
-            const uint32_t cut_key = uint32_t(cut >> 32);
+            const float cut_l = logit_of_key(uint32_t(cut >> 32));
             float low = kNoChance * kLog2e;
             if (rp.min_p > 0.0f) low = fmaxf(low, fminf(__log2f(rp.min_p) - 1e-3f, 0.0f));
             const auto stays = [&](float l, int i) {
                 const float y = (l - m) * c;
-                if (!(y >= low)) return false;
-                const uint32_t key = key_of(l);
-                if (key < cut_key || place_of(key, i0 + i) < cut) return false;
-                return l == m || !(rp.min_p > 0.0f) || ex2(y) >= rp.min_p;
+                return y >= low && place_of(key_of(l), i0 + i) >= cut &&
+                       (l == m || !(rp.min_p > 0.0f) || ex2(y) >= rp.min_p);
             };
-            if constexpr (kResident) {
-                // Every kept logit's number is asked for before the first is used.
-                using P = Pack<T>;
-                constexpr int kAhead = 16 / P::kWidth;
-                const int np = sl.packs();
-                for (int v0 = t; v0 < np; v0 += kRowThreads * kAhead) {
-                    float u[kAhead * P::kWidth];
-                    uint32_t in = 0;
+            // Where a filter has left few columns they are listed first and
+            // raced from the list, all their numbers in flight at once.
+            bool listed = by_k || by_p || rp.min_p > 0.0f;
+            if (listed) {
+                __syncthreads();
+                if (t == 0) sh.kept_n = 0;
+                __syncthreads();
+                uint32_t* kept_at = sh.all_n;
+                sl.each([&](float l, int i) {
+                    if (l >= cut_l && stays(l, i)) {
+                        const unsigned at = atomicAdd(&sh.kept_n, 1u);
+                        if (at < unsigned(kKept)) kept_at[at] = uint32_t(i);
+                    }
+                });
+                __syncthreads();
+                const int n = int(sh.kept_n);
+                if (n <= kKept) {
+                    for (int j = t; j < n; j += kRowThreads) {
+                        const int i = int(kept_at[j]);
+                        run_race(sl.at(i), i0 + i, noise[i]);
+                    }
+                } else {
+                    listed = false;
+                }
+            }
+            if (!listed) {
+                // -log u >= 1 - u, so that log2(w) - log2(1 - u) bounds a
+                // column's key from above: the two logarithms (accurate, where
+                // the bound's are approximate: the margin) are taken only
+                // where the bound reaches the warp's best so far.
+                float lead = neg_inf();   // the warp's best key, in log2
+                const auto bound = [&](float l, float u) { return (l - m) * c - __log2f(fmaxf(1.0f - u, 5.9604645e-8f)) + 1e-3f; };
+                const auto consider = [&](float l, int i, float u) {
+                    if (bound(l, u) >= lead && stays(l, i)) run_race(l, i0 + i, u);
+                };
+                const auto follow = [&] {   // (a warp's lanes together)
+                    const uint32_t k = __reduce_max_sync(__activemask(), uint32_t(best >> 32));
+                    if (k) lead = logit_of_key(k) * kLog2e;
+                };
+                if constexpr (kResident) {
+                    using P = Pack<T>;
+                    constexpr int W = P::kWidth, kAhead = 16 / W;
+                    const int np = sl.packs();
+                    const bool wide = (reinterpret_cast<uintptr_t>(noise) - 4u * unsigned(sl.shift)) % 16 == 0;
+                    for (int v0 = t; v0 < np; v0 += kRowThreads * kAhead) {
+                        float u[kAhead * W];
 #pragma unroll
-                    for (int g = 0; g < kAhead; ++g) {
-                        const int v = v0 + g * kRowThreads;
-                        if (v < np) {
-                            const P p = sl.mem[v];
+                        for (int g = 0; g < kAhead; ++g) {
+                            const int v = v0 + g * kRowThreads, i = v * W - sl.shift;
+                            if (v < np && i >= 0 && i + W <= sl.n && wide) {
 #pragma unroll
-                            for (int e = 0; e < P::kWidth; ++e) {
-                                const int i = v * P::kWidth - sl.shift + e;
-                                if (stays(p.get(e), i)) {
-                                    in |= 1u << (g * P::kWidth + e);
-                                    u[g * P::kWidth + e] = __ldg(noise + i);
+                                for (int e = 0; e < W; e += 4) {
+                                    const float4 f = __ldg(reinterpret_cast<const float4*>(noise + i + e));
+                                    u[g * W + e] = f.x, u[g * W + e + 1] = f.y, u[g * W + e + 2] = f.z, u[g * W + e + 3] = f.w;
                                 }
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < W; ++e)
+                                    u[g * W + e] = v < np && i + e >= 0 && i + e < sl.n ? __ldg(noise + i + e) : 0.0f;
                             }
                         }
-                    }
 #pragma unroll
-                    for (int g = 0; g < kAhead; ++g) {
-                        const int v = v0 + g * kRowThreads;
+                        for (int g = 0; g < kAhead; ++g) {
+                            const int v = v0 + g * kRowThreads;
+                            if (v >= np) break;
+                            const P p = sl.mem[v];
 #pragma unroll
-                        for (int e = 0; e < P::kWidth; ++e)
-                            if (in >> (g * P::kWidth + e) & 1u)
-                                run_race(sl.mem[v].get(e), i0 + v * P::kWidth - sl.shift + e, u[g * P::kWidth + e]);
+                            for (int e = 0; e < W; ++e) consider(p.get(e), v * W - sl.shift + e, u[g * W + e]);
+                            follow();
+                        }
                     }
+                } else {
+                    sl.each([&](float l, int i) {
+                        consider(l, i, __ldg(noise + i));
+                        follow();
+                    });
                 }
-            } else {
-                sl.each([&](float l, int i) {
-                    if (stays(l, i)) run_race(l, i0 + i, noise[i]);
-                });
             }
         }
     }
