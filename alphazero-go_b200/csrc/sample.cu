@@ -286,6 +286,7 @@ struct Part {   // what one CTA knows of its slice
 struct RowShared {
     uint32_t hist_n[kBins], hist_w[kBins];   // this CTA's; then the lists
     uint32_t all_n[kBins], all_w[kBins];     // the cluster's; then the kept columns
+    uint32_t upto_n[kBins];                  // inclusive sums of all_n
     Part part[kMaxCluster];
     float f[2][kMaxCluster];
     int n[2][kMaxCluster];
@@ -442,6 +443,38 @@ struct Slice {
             for (int i = int(threadIdx.x); i < n; i += kRowThreads) f(direct(i), i);
         }
     }
+    // f(l, i) for this thread's logits of at least l_min, a few of many: they
+    // are marked 32 at a time, so that a warp runs f as often as its busiest
+    // lane has marks, and not for every place where any lane has one.
+    template <class F>
+    __device__ __forceinline__ void each_above(float l_min, F f) const {
+        if constexpr (kResident) {
+            constexpr int kPacks = 32 / P::kWidth;
+            const int np = packs();
+            for (int v0 = int(threadIdx.x); v0 < np; v0 += kRowThreads * kPacks) {
+                uint32_t marks = 0;
+#pragma unroll
+                for (int g = 0; g < kPacks; ++g) {
+                    const int v = v0 + g * kRowThreads;
+                    if (v >= np) break;
+                    const P p = mem[v];
+#pragma unroll
+                    for (int e = 0; e < P::kWidth; ++e) marks |= p.get(e) >= l_min ? 1u << (g * P::kWidth + e) : 0u;
+                }
+                while (marks) {
+                    const int b = __ffs(int(marks)) - 1;
+                    marks &= marks - 1;
+                    const int i = (v0 + b / P::kWidth * kRowThreads) * P::kWidth - shift + b % P::kWidth;
+                    f(at(i), i);
+                }
+            }
+        } else {
+            for (int i = int(threadIdx.x); i < n; i += kRowThreads) {
+                const float l = direct(i);
+                if (l >= l_min) f(l, i);
+            }
+        }
+    }
     // The row's maximum is +inf (every CTA of the cluster learns it at once).
     __device__ void only_infinite() {
         infinite = true;
@@ -478,11 +511,9 @@ __device__ __forceinline__ Weighed cluster_add(Weighed v, RowShared& sh, int ran
     }
     __syncthreads();
     if (warp == 0) {
-        Weighed s{0, 0.0f};
-        for (int w = 0; w < kRowWarps; ++w) {
-            s.count += sh.wn[w];
-            s.mass += sh.wf[w];
-        }
+        Weighed s{lane < kRowWarps ? sh.wn[lane] : 0, lane < kRowWarps ? sh.wf[lane] : 0.0f};
+        s.count = int(__reduce_add_sync(0xFFFFFFFFu, unsigned(s.count)));
+        s.mass = warp_sum(s.mass);
         if (lane < ranks) {
             put_f(at_rank(&sh.f[turn][rank], lane), s.mass);
             put_u(at_rank(&sh.n[turn][rank], lane), uint32_t(s.count));
@@ -490,10 +521,12 @@ __device__ __forceinline__ Weighed cluster_add(Weighed v, RowShared& sh, int ran
     }
     cluster_barrier();
     Weighed s{0, 0.0f};
-    for (int r = 0; r < ranks; ++r) {
-        s.count += sh.n[turn][r];
-        s.mass += sh.f[turn][r];
-    }
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r)
+        if (r < ranks) {
+            s.count += sh.n[turn][r];
+            s.mass += sh.f[turn][r];
+        }
     turn ^= 1;
     return s;
 }
@@ -515,6 +548,7 @@ __device__ __forceinline__ Inclusive scan_bins(RowShared& sh) {
     if (lane == 31) sh.wn[warp] = int(s.n), sh.wm[warp] = int(s.w);
     __syncthreads();
     for (int w = 0; w < warp; ++w) s.n += uint32_t(sh.wn[w]), s.w += uint32_t(sh.wm[w]);
+    sh.upto_n[threadIdx.x] = s.n;
     return s;
 }
 
@@ -569,33 +603,35 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const Sample
     }
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // every CTA runs
     __syncthreads();
-    if (warp == 0 && lane < ranks) {
-        Part p{m, 0.0f, inf, inf, 0, 0, 0};
-        for (int w = 0; w < kRowWarps; ++w) {
-            p.z += sh.wh[w];
-            p.valid += sh.wk[w];
-            p.threads += sh.wn[w];
-            if (sh.wf[w] > neg_inf()) {
-                ++p.warps;
-                p.warp_low = fminf(p.warp_low, sh.wf[w]);
-                p.thread_low = fminf(p.thread_low, -sh.wg[w]);
-            }
+    if (warp == 0) {
+        const bool has = lane < kRowWarps && sh.wf[lane] > neg_inf();
+        Part p;
+        p.top = m;
+        p.z = warp_sum(lane < kRowWarps ? sh.wh[lane] : 0.0f);
+        p.warp_low = -warp_max(has ? -sh.wf[lane] : neg_inf());
+        p.thread_low = -warp_max(has ? sh.wg[lane] : neg_inf());
+        p.valid = int(__reduce_add_sync(0xFFFFFFFFu, lane < kRowWarps ? unsigned(sh.wk[lane]) : 0u));
+        p.warps = __popc(__ballot_sync(0xFFFFFFFFu, has));
+        p.threads = int(__reduce_add_sync(0xFFFFFFFFu, lane < kRowWarps ? unsigned(sh.wn[lane]) : 0u));
+        if (lane < ranks) {
+            const uint32_t to = at_rank(&sh.part[rank], lane);
+            const uint32_t* words = reinterpret_cast<const uint32_t*>(&p);
+#pragma unroll
+            for (int i = 0; i < int(sizeof(Part) / 4); ++i) put_u(to + uint32_t(i) * 4, words[i]);
         }
-        const uint32_t to = at_rank(&sh.part[rank], lane);
-        const uint32_t* words = reinterpret_cast<const uint32_t*>(&p);
-        for (int i = 0; i < int(sizeof(Part) / 4); ++i) put_u(to + uint32_t(i) * 4, words[i]);
     }
     cluster_barrier();
-    Part all{neg_inf(), 0.0f, inf, inf, 0, 0, 0};
-    for (int r = 0; r < ranks; ++r) all.top = fmaxf(all.top, sh.part[r].top);
-    for (int r = 0; r < ranks; ++r) {
-        const Part& p = sh.part[r];
-        all.z += p.top == all.top ? p.z : p.z * ex2((p.top - all.top) * c);
-        all.valid += p.valid;
-        all.warps += p.warps;
-        all.threads += p.threads;
-        all.warp_low = fminf(all.warp_low, p.warp_low);
-        all.thread_low = fminf(all.thread_low, p.thread_low);
+    Part all;
+    {   // lane r has CTA r's part; the sums' order is fixed
+        Part p{neg_inf(), 0.0f, inf, inf, 0, 0, 0};
+        if (lane < ranks) p = sh.part[lane];
+        all.top = warp_max(p.top);
+        all.z = warp_sum(p.top == all.top ? p.z : p.z * ex2((p.top - all.top) * c));
+        all.warp_low = -warp_max(-p.warp_low);
+        all.thread_low = -warp_max(-p.thread_low);
+        all.valid = int(__reduce_add_sync(0xFFFFFFFFu, unsigned(p.valid)));
+        all.warps = int(__reduce_add_sync(0xFFFFFFFFu, unsigned(p.warps)));
+        all.threads = int(__reduce_add_sync(0xFFFFFFFFu, unsigned(p.threads)));
     }
     m = all.top;
     int turn = 0;
@@ -636,56 +672,66 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const Sample
                 });
                 return cluster_add(s, sh, rank, ranks, turn);
             };
-            // What the histogram covers: log2 w from `low` to 0.
-            float low;
+            // What the histogram covers: log2 w from `low` to 0. Any range that
+            // holds the cut will do. The bound for top-p takes every logit below
+            // to weigh as much as it may, so an eighth of the weight is tried
+            // first; should the cut lie below, the bound itself is taken.
+            float low, sure;
             if (by_k) {
                 const float l = k <= all.warps ? all.warp_low : k <= all.threads ? all.thread_low : neg_inf();
-                low = fmaxf((l - m) * c, -40.0f);
+                sure = low = fmaxf((l - m) * c, -40.0f);
             } else {
-                low = fmaxf(__log2f((1.0f - rp.top_p) * 0.99f * all.z / float(a.cols)), -40.0f);
+                sure = fmaxf(__log2f((1.0f - rp.top_p) * 0.99f * all.z / float(a.cols)), -40.0f);
+                low = sure < -6.0f ? sure + 3.0f : sure;
             }
-            low = fminf(low, -1e-3f);
-            const float steps = float(kBins - 1) / -low;   // bins per unit of log2 w; the last bin holds `low`
-            const float fixed = 2147483648.0f / all.z;     // all masses together stay below 2^31 + cols / 2
+            const float fixed = 2147483648.0f / all.z;   // all masses together stay below 2^31 + cols / 2
+            float steps;                                 // bins per unit of log2 w; the last bin holds `low`
             const auto bin_of = [&](float y) { return int(-y * steps); };
-            sh.hist_n[t] = 0;
-            sh.hist_w[t] = 0;
-            __syncthreads();
-            sl.each([&](float l, int) {
-                const float y = (l - m) * c;
-                if (y >= low) {
-                    const int b = bin_of(y);
-                    atomicAdd(&sh.hist_n[b], 1u);
-                    atomicAdd(&sh.hist_w[b], __float2uint_rn(ex2(y) * fixed));
-                }
-            });
-            cluster_barrier();
-            {   // this CTA adds its share of the bins over the cluster, for everyone
+            // A little below the logit of log2 w = y.
+            const auto logit_below = [&](float y) { return m + y / c * 1.00001f - fabsf(m) * 1e-6f; };
+            Inclusive upto;
+            const auto count_bins = [&] {
+                low = fminf(low, -1e-3f);
+                steps = float(kBins - 1) / -low;
+                sh.hist_n[t] = 0;
+                sh.hist_w[t] = 0;
+                if (t == 0) sh.first = sh.last = kBins, sh.list_n = 0;
+                __syncthreads();
+                sl.each_above(logit_below(low), [&](float l, int) {
+                    const float y = (l - m) * c;
+                    if (y >= low) {
+                        const int b = bin_of(y);
+                        atomicAdd(&sh.hist_n[b], 1u);
+                        atomicAdd(&sh.hist_w[b], __float2uint_rn(ex2(y) * fixed));
+                    }
+                });
+                cluster_barrier();
+                // This CTA adds its share of the bins over the cluster, for everyone.
                 const int share = kBins / ranks;
                 if (t < share) {
                     const int b = rank * share + t;
-                    uint32_t n = 0, w = 0;
-                    for (int r = 0; r < ranks; ++r) {
-                        n += get_u(at_rank(&sh.hist_n[b], r));
-                        w += get_u(at_rank(&sh.hist_w[b], r));
-                    }
-                    for (int r = 0; r < ranks; ++r) {
-                        put_u(at_rank(&sh.all_n[b], r), n);
-                        put_u(at_rank(&sh.all_w[b], r), w);
-                    }
+                    uint32_t n[kMaxCluster], w[kMaxCluster];
+#pragma unroll
+                    for (int r = 0; r < kMaxCluster; ++r)
+                        if (r < ranks) n[r] = get_u(at_rank(&sh.hist_n[b], r)), w[r] = get_u(at_rank(&sh.hist_w[b], r));
+#pragma unroll
+                    for (int r = 1; r < kMaxCluster; ++r)
+                        if (r < ranks) n[0] += n[r], w[0] += w[r];
+#pragma unroll
+                    for (int r = 0; r < kMaxCluster; ++r)
+                        if (r < ranks) put_u(at_rank(&sh.all_n[b], r), n[0]), put_u(at_rank(&sh.all_w[b], r), w[0]);
                 }
-            }
-            cluster_barrier();
-            const Inclusive upto = scan_bins(sh);
+                cluster_barrier();
+                upto = scan_bins(sh);
+            };
+            count_bins();
             uint64_t* list = reinterpret_cast<uint64_t*>(sh.hist_n);
             uint64_t* merged = list + kList;
             // The cut of one filter: the first `count` logits, or the shortest
             // prefix of mass `target`. False: the histogram does not settle it.
             // kept: the mass of what the cut is taken from.
+            // (sh.first, sh.last and sh.list_n are at their starts before it.)
             const auto settle = [&](int count, double target, float* kept) -> bool {
-                __syncthreads();
-                if (t == 0) sh.first = sh.last = kBins, sh.list_n = 0;
-                __syncthreads();
                 if (count > 0) {
                     if (upto.n >= uint32_t(count) && upto.n - sh.all_n[t] < uint32_t(count)) sh.first = sh.last = t;
                 } else {
@@ -699,20 +745,13 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const Sample
                 int first = sh.first;
                 const int last = sh.last;
                 if (last >= kBins) return false;
-                __syncthreads();
                 // Few enough down to the cut: all of them are listed, and raced there.
-                if (t == last) sh.list_n = upto.n;
-                if (t == first) sh.wk[0] = int(upto.n - sh.all_n[t]);
-                __syncthreads();
-                const uint32_t down = sh.list_n, above = uint32_t(sh.wk[0]);
+                const uint32_t down = sh.upto_n[last], above = first > 0 ? sh.upto_n[first - 1] : 0u;
                 const bool whole = down <= uint32_t(kList);
                 if (!whole && down - above > uint32_t(kList)) return false;
                 if (whole) first = 0;
-                __syncthreads();
-                if (t == 0) sh.list_n = 0;
-                __syncthreads();
                 Weighed s{0, 0.0f};
-                sl.each([&](float l, int i) {
+                sl.each_above(logit_below(fmaxf(low, -float(last + 2) / steps)), [&](float l, int i) {
                     const float y = (l - m) * c;
                     if (y >= low) {
                         const int b = bin_of(y);
@@ -728,11 +767,16 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const Sample
                 // All lists here, then in order.
                 int n = 0;
                 uint64_t mineplace = 0;
-                for (int r = 0; r < ranks; ++r) {
-                    const int rn = int(get_u(at_rank(&sh.list_n, r)));
-                    if (t >= n && t < n + rn) mineplace = get_l(at_rank(&list[t - n], r));
-                    n += rn;
-                }
+                int of_rank[kMaxCluster];
+#pragma unroll
+                for (int r = 0; r < kMaxCluster; ++r)
+                    if (r < ranks) of_rank[r] = int(get_u(at_rank(&sh.list_n, r)));
+#pragma unroll
+                for (int r = 0; r < kMaxCluster; ++r)
+                    if (r < ranks) {
+                        if (t >= n && t < n + of_rank[r]) mineplace = get_l(at_rank(&list[t - n], r));
+                        n += of_rank[r];
+                    }
                 if (t < n) merged[t] = mineplace;
                 __syncthreads();
                 int before = 0;
@@ -798,8 +842,18 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const Sample
             bool settled = true;
             if (by_k) settled = settle(k, 0.0, &kept);
             if (settled && by_p && !raced) {
-                if (by_k) cluster_barrier();   // the first cut's lists have been read
+                if (by_k) {   // again from the start, once the first cut's lists have been read
+                    cluster_barrier();
+                    if (t == 0) sh.first = sh.last = kBins, sh.list_n = 0;
+                    __syncthreads();
+                }
                 settled = settle(0, double(rp.top_p) * double(kept), &kept);
+                if (!settled && low > sure && sh.last >= kBins) {
+                    low = sure;
+                    cluster_barrier();
+                    count_bins();
+                    settled = settle(0, double(rp.top_p) * double(kept), &kept);
+                }
             }
             if (!settled) {
                 const Weighed every = at(kKeyLow);
@@ -836,8 +890,8 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const Sample
                 if (t == 0) sh.kept_n = 0;
                 __syncthreads();
                 uint32_t* kept_at = sh.all_n;
-                sl.each([&](float l, int i) {
-                    if (l >= cut_l && stays(l, i)) {
+                sl.each_above(cut_l, [&](float l, int i) {
+                    if (stays(l, i)) {
                         const unsigned at = atomicAdd(&sh.kept_n, 1u);
                         if (at < unsigned(kKept)) kept_at[at] = uint32_t(i);
                     }
