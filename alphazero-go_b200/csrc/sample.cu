@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(128) sample_warp_kernel(const SampleArgs a) {
 // of their maxima; and logits with w < (1 - p) Z / cols have together less
 // than (1 - p) Z, so the prefix that top-p keeps ends above them.
 
-constexpr int kRowThreads = 512, kRowWarps = kRowThreads / 32, kMaxCluster = 8;
+constexpr int kMaxCluster = 8, kMaxRowWarps = 8;
 constexpr int kBins = 512, kList = 256;
 // Gumbel noise -log(-log u) lies in [-2.86, 16.64]: a logit with x < -19.6
 // loses to the maximum whatever their numbers, which need not be read.
@@ -292,8 +292,8 @@ struct RowShared {
     int n[2][kMaxCluster];
     unsigned long long best[kMaxCluster];
     float best_x[kMaxCluster];
-    float wf[kRowWarps], wg[kRowWarps], wh[kRowWarps];
-    int wn[kRowWarps], wm[kRowWarps], wk[kRowWarps];
+    float wf[kMaxRowWarps], wg[kMaxRowWarps], wh[kMaxRowWarps];
+    int wn[kMaxRowWarps], wm[kMaxRowWarps], wk[kMaxRowWarps];
     unsigned list_n, kept_n;
     int first, last;
     float kept;
@@ -302,9 +302,26 @@ struct RowShared {
 constexpr int kKept = 2 * kBins;   // columns that all_n and all_w hold
 static_assert(kList * 2 * 8 <= int(sizeof(uint32_t)) * kBins * 2, "a CTA's list and the merged one take the histogram's place");
 
-// The address of *p in CTA `rank` of the cluster.
-template <typename P>
-__device__ __forceinline__ uint32_t at_rank(P* p, int rank) { return mapa(smem_u32(p), uint32_t(rank)); }
+// The CTAs that share a row: kThreads each, one of them (kSolo) or a cluster.
+template <int kThreads_, bool kSolo_>
+struct Team {
+    static constexpr int kThreads = kThreads_, kWarps = kThreads / 32;
+    static constexpr bool kSolo = kSolo_;
+    int rank, ranks;
+    // The address of *p in CTA r.
+    template <typename P>
+    __device__ __forceinline__ uint32_t at(P* p, int r) const {
+        return kSolo ? smem_u32(p) : mapa(smem_u32(p), uint32_t(r));
+    }
+    __device__ __forceinline__ void barrier() const {
+        if constexpr (kSolo) {
+            __syncthreads();
+        } else {
+            __syncwarp();
+            cluster_sync();
+        }
+    }
+};
 __device__ __forceinline__ void put_f(uint32_t a, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory"); }
 __device__ __forceinline__ void put_u(uint32_t a, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
 __device__ __forceinline__ uint32_t get_u(uint32_t a) {
@@ -366,7 +383,7 @@ struct Pack {
     }
 };
 
-template <typename T, bool kResident>
+template <typename T, bool kResident, int kThreads>
 struct Slice {
     using P = Pack<T>;
     enum : int { W = P::kWidth };
@@ -396,16 +413,16 @@ struct Slice {
             const uint4* base = reinterpret_cast<const uint4*>(src - shift);
             const int np = packs();
             constexpr int kAhead = 4;
-            for (int v0 = int(threadIdx.x); v0 < np; v0 += kRowThreads * kAhead) {
+            for (int v0 = int(threadIdx.x); v0 < np; v0 += kThreads * kAhead) {
                 P p[kAhead];
 #pragma unroll
                 for (int u = 0; u < kAhead; ++u) {
-                    const int v = v0 + u * kRowThreads, i = v * W - shift;
+                    const int v = v0 + u * kThreads, i = v * W - shift;
                     if (v < np && i >= 0 && i + W <= n) p[u].q = __ldg(base + v);
                 }
 #pragma unroll
                 for (int u = 0; u < kAhead; ++u) {
-                    const int v = v0 + u * kRowThreads, i = v * W - shift;
+                    const int v = v0 + u * kThreads, i = v * W - shift;
                     if (v >= np) continue;
                     if (i < 0 || i + W > n) {
 #pragma unroll
@@ -426,7 +443,7 @@ struct Slice {
                 }
             }
         } else {
-            for (int i = int(threadIdx.x); i < n; i += kRowThreads) f(direct(i));
+            for (int i = int(threadIdx.x); i < n; i += kThreads) f(direct(i));
         }
     }
     // f(l, i) for this thread's logits (and some of -inf around the slice).
@@ -434,13 +451,13 @@ struct Slice {
     __device__ __forceinline__ void each(F f) const {
         if constexpr (kResident) {
             const int np = packs();
-            for (int v = int(threadIdx.x); v < np; v += kRowThreads) {
+            for (int v = int(threadIdx.x); v < np; v += kThreads) {
                 const P p = mem[v];
 #pragma unroll
                 for (int e = 0; e < W; ++e) f(p.get(e), v * W - shift + e);
             }
         } else {
-            for (int i = int(threadIdx.x); i < n; i += kRowThreads) f(direct(i), i);
+            for (int i = int(threadIdx.x); i < n; i += kThreads) f(direct(i), i);
         }
     }
     // f(l, i) for this thread's logits of at least l_min, a few of many: they
@@ -451,11 +468,11 @@ struct Slice {
         if constexpr (kResident) {
             constexpr int kPacks = 32 / P::kWidth;
             const int np = packs();
-            for (int v0 = int(threadIdx.x); v0 < np; v0 += kRowThreads * kPacks) {
+            for (int v0 = int(threadIdx.x); v0 < np; v0 += kThreads * kPacks) {
                 uint32_t marks = 0;
 #pragma unroll
                 for (int g = 0; g < kPacks; ++g) {
-                    const int v = v0 + g * kRowThreads;
+                    const int v = v0 + g * kThreads;
                     if (v >= np) break;
                     const P p = mem[v];
 #pragma unroll
@@ -464,12 +481,12 @@ struct Slice {
                 while (marks) {
                     const int b = __ffs(int(marks)) - 1;
                     marks &= marks - 1;
-                    const int i = (v0 + b / P::kWidth * kRowThreads) * P::kWidth - shift + b % P::kWidth;
+                    const int i = (v0 + b / P::kWidth * kThreads) * P::kWidth - shift + b % P::kWidth;
                     f(at(i), i);
                 }
             }
         } else {
-            for (int i = int(threadIdx.x); i < n; i += kRowThreads) {
+            for (int i = int(threadIdx.x); i < n; i += kThreads) {
                 const float l = direct(i);
                 if (l >= l_min) f(l, i);
             }
@@ -479,7 +496,7 @@ struct Slice {
     __device__ void only_infinite() {
         infinite = true;
         if constexpr (kResident) {
-            for (int v = int(threadIdx.x); v < packs(); v += kRowThreads) {
+            for (int v = int(threadIdx.x); v < packs(); v += kThreads) {
                 P p = mem[v];
 #pragma unroll
                 for (int e = 0; e < W; ++e) {
@@ -492,15 +509,13 @@ struct Slice {
     }
 };
 
-__device__ __forceinline__ void cluster_barrier() {
-    __syncwarp();
-    cluster_sync();
-}
-
-// Count and mass over the cluster, in a fixed order; the same everywhere.
+// Count and mass over the team, in a fixed order; the same everywhere.
 // `turn` alternates between two sets of slots: a CTA writes a set again only
 // after a barrier that every CTA reaches past its reads of it.
-__device__ __forceinline__ Weighed cluster_add(Weighed v, RowShared& sh, int rank, int ranks, int& turn) {
+template <class Team>
+__device__ __forceinline__ Weighed team_add(const Team& team, Weighed v, RowShared& sh, int& turn) {
+    constexpr int kWarps = Team::kWarps;
+    const int rank = team.rank, ranks = team.ranks;
     const int warp = int(threadIdx.x) >> 5, lane = int(threadIdx.x) & 31;
     v.count = int(__reduce_add_sync(0xFFFFFFFFu, unsigned(v.count)));
     v.mass = warp_sum(v.mass);
@@ -511,15 +526,15 @@ __device__ __forceinline__ Weighed cluster_add(Weighed v, RowShared& sh, int ran
     }
     __syncthreads();
     if (warp == 0) {
-        Weighed s{lane < kRowWarps ? sh.wn[lane] : 0, lane < kRowWarps ? sh.wf[lane] : 0.0f};
+        Weighed s{lane < kWarps ? sh.wn[lane] : 0, lane < kWarps ? sh.wf[lane] : 0.0f};
         s.count = int(__reduce_add_sync(0xFFFFFFFFu, unsigned(s.count)));
         s.mass = warp_sum(s.mass);
         if (lane < ranks) {
-            put_f(at_rank(&sh.f[turn][rank], lane), s.mass);
-            put_u(at_rank(&sh.n[turn][rank], lane), uint32_t(s.count));
+            put_f(team.at(&sh.f[turn][rank], lane), s.mass);
+            put_u(team.at(&sh.n[turn][rank], lane), uint32_t(s.count));
         }
     }
-    cluster_barrier();
+    team.barrier();
     Weighed s{0, 0.0f};
 #pragma unroll
     for (int r = 0; r < kMaxCluster; ++r)
@@ -534,33 +549,52 @@ __device__ __forceinline__ Weighed cluster_add(Weighed v, RowShared& sh, int ran
 struct Inclusive {
     uint32_t n, w;
 };
-// The histogram's inclusive sums up to bin threadIdx.x (kBins == kRowThreads).
-static_assert(kBins == kRowThreads, "a thread per bin");
-__device__ __forceinline__ Inclusive scan_bins(RowShared& sh) {
-    const int warp = int(threadIdx.x) >> 5, lane = int(threadIdx.x) & 31;
-    Inclusive s{sh.all_n[threadIdx.x], sh.all_w[threadIdx.x]};
+// The histogram's inclusive sums up to this thread's bins, kPer neighbours.
+template <int kThreads>
+struct Sums {
+    static constexpr int kPer = kBins / kThreads;
+    uint32_t n[kPer], w[kPer];
+    __device__ __forceinline__ void scan(RowShared& sh) {
+        const int warp = int(threadIdx.x) >> 5, lane = int(threadIdx.x) & 31, b0 = int(threadIdx.x) * kPer;
+        uint32_t sn = 0, sw = 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t n = __shfl_up_sync(0xFFFFFFFFu, s.n, o), w = __shfl_up_sync(0xFFFFFFFFu, s.w, o);
-        if (lane >= o) s.n += n, s.w += w;
+        for (int j = 0; j < kPer; ++j) {
+            n[j] = sn += sh.all_n[b0 + j];
+            w[j] = sw += sh.all_w[b0 + j];
+        }
+        const uint32_t own_n = sn, own_w = sw;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t un = __shfl_up_sync(0xFFFFFFFFu, sn, o), uw = __shfl_up_sync(0xFFFFFFFFu, sw, o);
+            if (lane >= o) sn += un, sw += uw;
+        }
+        if (lane == 31) sh.wn[warp] = int(sn), sh.wm[warp] = int(sw);
+        __syncthreads();
+        sn -= own_n;
+        sw -= own_w;
+        for (int v = 0; v < warp; ++v) sn += uint32_t(sh.wn[v]), sw += uint32_t(sh.wm[v]);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            n[j] += sn;
+            w[j] += sw;
+            sh.upto_n[b0 + j] = n[j];
+        }
     }
-    __syncthreads();
-    if (lane == 31) sh.wn[warp] = int(s.n), sh.wm[warp] = int(s.w);
-    __syncthreads();
-    for (int w = 0; w < warp; ++w) s.n += uint32_t(sh.wn[w]), s.w += uint32_t(sh.wm[w]);
-    sh.upto_n[threadIdx.x] = s.n;
-    return s;
-}
+};
 
-template <typename T, bool kResident>
-__global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const SampleArgs a, const int ranks, const int per) {
+template <typename T, bool kResident, int kThreads, bool kSolo>
+__global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
+    sample_row_kernel(const SampleArgs a, const int ranks, const int per) {
+    using Crew = Team<kThreads, kSolo>;
+    constexpr int kWarps = Crew::kWarps;
     extern __shared__ __align__(16) uint8_t smem_raw[];
     __shared__ RowShared sh;
-    const int rank = int(blockIdx.x) % ranks, t = int(threadIdx.x), warp = t >> 5, lane = t & 31;
-    const long long row = blockIdx.x / unsigned(ranks);
-    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // this CTA runs: its memory may be written
+    const int rank = kSolo ? 0 : int(blockIdx.x) % ranks, t = int(threadIdx.x), warp = t >> 5, lane = t & 31;
+    const long long row = kSolo ? blockIdx.x : blockIdx.x / unsigned(ranks);
+    const Crew crew{rank, ranks};
+    if constexpr (!kSolo) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // this CTA runs: its memory may be written
     const RowParams rp(a, row);
-    Slice<T, kResident> sl;
+    Slice<T, kResident, kThreads> sl;
     const int i0 = min(rank * per, a.cols);
     sl.src = static_cast<const T*>(a.logits) + size_t(row) * size_t(a.ld) + i0;
     sl.legal = a.legal ? a.legal + size_t(row) * size_t(a.legal_ld) + i0 : nullptr;
@@ -582,7 +616,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const Sample
     }
     __syncthreads();
     float m = neg_inf();
-    for (int w = 0; w < kRowWarps; ++w) m = fmaxf(m, sh.wf[w]);
+    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sh.wf[w]);
     const bool greedy = rp.greedy();
     // w = 2^((l - m) c). The bounds keep 0 * c and -inf * c what they should be.
     const float c = greedy ? 1.0f : fminf(fmaxf(kLog2e / rp.temperature, 1e-38f), 3e38f);
@@ -601,26 +635,26 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const Sample
         s.count = int(__reduce_add_sync(0xFFFFFFFFu, unsigned(s.count)));
         if (lane == 0) sh.wh[warp] = s.mass, sh.wk[warp] = s.count;
     }
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // every CTA runs
+    if constexpr (!kSolo) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // every CTA runs
     __syncthreads();
     if (warp == 0) {
-        const bool has = lane < kRowWarps && sh.wf[lane] > neg_inf();
+        const bool has = lane < kWarps && sh.wf[lane] > neg_inf();
         Part p;
         p.top = m;
-        p.z = warp_sum(lane < kRowWarps ? sh.wh[lane] : 0.0f);
+        p.z = warp_sum(lane < kWarps ? sh.wh[lane] : 0.0f);
         p.warp_low = -warp_max(has ? -sh.wf[lane] : neg_inf());
         p.thread_low = -warp_max(has ? sh.wg[lane] : neg_inf());
-        p.valid = int(__reduce_add_sync(0xFFFFFFFFu, lane < kRowWarps ? unsigned(sh.wk[lane]) : 0u));
+        p.valid = int(__reduce_add_sync(0xFFFFFFFFu, lane < kWarps ? unsigned(sh.wk[lane]) : 0u));
         p.warps = __popc(__ballot_sync(0xFFFFFFFFu, has));
-        p.threads = int(__reduce_add_sync(0xFFFFFFFFu, lane < kRowWarps ? unsigned(sh.wn[lane]) : 0u));
+        p.threads = int(__reduce_add_sync(0xFFFFFFFFu, lane < kWarps ? unsigned(sh.wn[lane]) : 0u));
         if (lane < ranks) {
-            const uint32_t to = at_rank(&sh.part[rank], lane);
+            const uint32_t to = crew.at(&sh.part[rank], lane);
             const uint32_t* words = reinterpret_cast<const uint32_t*>(&p);
 #pragma unroll
             for (int i = 0; i < int(sizeof(Part) / 4); ++i) put_u(to + uint32_t(i) * 4, words[i]);
         }
     }
-    cluster_barrier();
+    crew.barrier();
     Part all;
     {   // lane r has CTA r's part; the sums' order is fixed
         Part p{neg_inf(), 0.0f, inf, inf, 0, 0, 0};
@@ -661,6 +695,28 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const Sample
         const bool by_k = k > 0 && k < all.valid, by_p = rp.filters_p() && rp.top_p > 0.0f && k != 1;
         uint64_t cut = place_of(kKeyLow, 0x7FFFFFFF);   // the last place kept
         bool raced = false;
+        const auto passes_min_p = [&](float l) { return l == m || !(rp.min_p > 0.0f) || ex2((l - m) * c) >= rp.min_p; };
+        // The race among n listed columns of the slice, their numbers asked for
+        // some at a time.
+        const auto race_kept = [&](const uint32_t* at, int n) {
+            constexpr int kAhead = 4;
+            for (int j0 = t; j0 < n; j0 += kThreads * kAhead) {
+                int i[kAhead];
+                float u[kAhead];
+#pragma unroll
+                for (int g = 0; g < kAhead; ++g)
+                    if (j0 + g * kThreads < n) {
+                        i[g] = int(at[j0 + g * kThreads]);
+                        u[g] = __ldg(noise + i[g]);
+                    }
+#pragma unroll
+                for (int g = 0; g < kAhead; ++g)
+                    if (j0 + g * kThreads < n) {
+                        const float l = sl.at(i[g]);
+                        if (passes_min_p(l)) run_race(l, i0 + i[g], u[g]);
+                    }
+            }
+        };
         if (by_k || by_p) {
             const auto at = [&](uint32_t key) {
                 Weighed s{0, 0.0f};
@@ -670,7 +726,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const Sample
                         s.mass += ex2((l - m) * c);
                     }
                 });
-                return cluster_add(s, sh, rank, ranks, turn);
+                return team_add(crew, s, sh, turn);
             };
             // What the histogram covers: log2 w from `low` to 0. Any range that
             // holds the cut will do. The bound for top-p takes every logit below
@@ -689,13 +745,12 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const Sample
             const auto bin_of = [&](float y) { return int(-y * steps); };
             // A little below the logit of log2 w = y.
             const auto logit_below = [&](float y) { return m + y / c * 1.00001f - fabsf(m) * 1e-6f; };
-            Inclusive upto;
+            Sums<kThreads> upto;
             const auto count_bins = [&] {
                 low = fminf(low, -1e-3f);
                 steps = float(kBins - 1) / -low;
-                sh.hist_n[t] = 0;
-                sh.hist_w[t] = 0;
-                if (t == 0) sh.first = sh.last = kBins, sh.list_n = 0;
+                for (int b = t; b < kBins; b += kThreads) sh.hist_n[b] = sh.hist_w[b] = 0;
+                if (t == 0) sh.first = sh.last = kBins, sh.list_n = sh.kept_n = 0;
                 __syncthreads();
                 sl.each_above(logit_below(low), [&](float l, int) {
                     const float y = (l - m) * c;
@@ -705,41 +760,44 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const Sample
                         atomicAdd(&sh.hist_w[b], __float2uint_rn(ex2(y) * fixed));
                     }
                 });
-                cluster_barrier();
+                crew.barrier();
                 // This CTA adds its share of the bins over the cluster, for everyone.
                 const int share = kBins / ranks;
-                if (t < share) {
-                    const int b = rank * share + t;
+                for (int b = rank * share + t; b < (rank + 1) * share; b += kThreads) {
                     uint32_t n[kMaxCluster], w[kMaxCluster];
 #pragma unroll
                     for (int r = 0; r < kMaxCluster; ++r)
-                        if (r < ranks) n[r] = get_u(at_rank(&sh.hist_n[b], r)), w[r] = get_u(at_rank(&sh.hist_w[b], r));
+                        if (r < ranks) n[r] = get_u(crew.at(&sh.hist_n[b], r)), w[r] = get_u(crew.at(&sh.hist_w[b], r));
 #pragma unroll
                     for (int r = 1; r < kMaxCluster; ++r)
                         if (r < ranks) n[0] += n[r], w[0] += w[r];
 #pragma unroll
                     for (int r = 0; r < kMaxCluster; ++r)
-                        if (r < ranks) put_u(at_rank(&sh.all_n[b], r), n[0]), put_u(at_rank(&sh.all_w[b], r), w[0]);
+                        if (r < ranks) put_u(crew.at(&sh.all_n[b], r), n[0]), put_u(crew.at(&sh.all_w[b], r), w[0]);
                 }
-                cluster_barrier();
-                upto = scan_bins(sh);
+                crew.barrier();
+                upto.scan(sh);
             };
-            count_bins();
             uint64_t* list = reinterpret_cast<uint64_t*>(sh.hist_n);
             uint64_t* merged = list + kList;
-            // The cut of one filter: the first `count` logits, or the shortest
-            // prefix of mass `target`. False: the histogram does not settle it.
-            // kept: the mass of what the cut is taken from.
-            // (sh.first, sh.last and sh.list_n are at their starts before it.)
-            const auto settle = [&](int count, double target, float* kept) -> bool {
-                if (count > 0) {
-                    if (upto.n >= uint32_t(count) && upto.n - sh.all_n[t] < uint32_t(count)) sh.first = sh.last = t;
-                } else {
-                    // A fixed-point sum is off by half a unit a logit, and by the
-                    // masses' own rounding, a few 2^-22 of it.
-                    const double goal = target * double(fixed), slack = 0.5 * double(upto.n) + 4096.0;
-                    if (double(upto.w) + slack >= goal) atomicMin(&sh.first, t);
-                    if (double(upto.w) - slack >= goal) atomicMin(&sh.last, t);
+            // One filter's cut: the first `count` logits, or the shortest prefix
+            // of mass `target`. False: the histogram does not settle it. kept:
+            // the mass that the cut is taken from. `final`: the last filter, so
+            // that what lies above its cut is raced on the way. (sh.first,
+            // sh.last, sh.list_n and sh.kept_n are at their starts before it.)
+            const auto settle = [&](int count, double target, bool final, float* kept) -> bool {
+#pragma unroll
+                for (int j = 0; j < Sums<kThreads>::kPer; ++j) {
+                    const int b = t * Sums<kThreads>::kPer + j;
+                    if (count > 0) {
+                        if (upto.n[j] >= uint32_t(count) && upto.n[j] - sh.all_n[b] < uint32_t(count)) sh.first = sh.last = b;
+                    } else {
+                        // A fixed-point sum is off by half a unit a logit, and by
+                        // the masses' own rounding, a few 2^-22 of it.
+                        const double goal = target * double(fixed), slack = 0.5 * double(upto.n[j]) + 4096.0;
+                        if (double(upto.w[j]) + slack >= goal) atomicMin(&sh.first, b);
+                        if (double(upto.w[j]) - slack >= goal) atomicMin(&sh.last, b);
+                    }
                 }
                 __syncthreads();
                 int first = sh.first;
@@ -750,6 +808,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const Sample
                 const bool whole = down <= uint32_t(kList);
                 if (!whole && down - above > uint32_t(kList)) return false;
                 if (whole) first = 0;
+                uint32_t* const kept_at = sh.all_n;
                 Weighed s{0, 0.0f};
                 sl.each_above(logit_below(fmaxf(low, -float(last + 2) / steps)), [&](float l, int i) {
                     const float y = (l - m) * c;
@@ -758,102 +817,124 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const Sample
                         if (b < first) {
                             ++s.count;
                             s.mass += ex2(y);
+                            if (final) {
+                                const unsigned at = atomicAdd(&sh.kept_n, 1u);
+                                if (at < unsigned(kKept)) kept_at[at] = uint32_t(i);
+                            }
                         } else if (b <= last) {
                             list[atomicAdd(&sh.list_n, 1u)] = place_of(key_of(l), i0 + i);
                         }
                     }
                 });
-                s = cluster_add(s, sh, rank, ranks, turn);   // (also: every list is written)
+                __syncthreads();
+                const bool race_now = final && !whole && sh.kept_n <= unsigned(kKept);
+                if (race_now) race_kept(kept_at, int(sh.kept_n));
+                s = team_add(crew, s, sh, turn);   // (also: every list is written)
                 // All lists here, then in order.
+                constexpr int kSlots = kList / kThreads;
                 int n = 0;
-                uint64_t mineplace = 0;
+                uint64_t place[kSlots] = {};
                 int of_rank[kMaxCluster];
 #pragma unroll
                 for (int r = 0; r < kMaxCluster; ++r)
-                    if (r < ranks) of_rank[r] = int(get_u(at_rank(&sh.list_n, r)));
+                    if (r < ranks) of_rank[r] = int(get_u(crew.at(&sh.list_n, r)));
 #pragma unroll
                 for (int r = 0; r < kMaxCluster; ++r)
                     if (r < ranks) {
-                        if (t >= n && t < n + of_rank[r]) mineplace = get_l(at_rank(&list[t - n], r));
+#pragma unroll
+                        for (int j = 0; j < kSlots; ++j) {
+                            const int at = t + j * kThreads - n;
+                            if (at >= 0 && at < of_rank[r]) place[j] = get_l(crew.at(&list[at], r));
+                        }
                         n += of_rank[r];
                     }
-                if (t < n) merged[t] = mineplace;
+#pragma unroll
+                for (int j = 0; j < kSlots; ++j)
+                    if (t + j * kThreads < n) merged[t + j * kThreads] = place[j];
                 __syncthreads();
-                int before = 0;
+                int before[kSlots] = {};
                 if (t < n)
-                    for (int j = 0; j < n; ++j) before += merged[j] > mineplace;
+                    for (int q = 0; q < n; ++q) {
+                        const uint64_t other = merged[q];
+#pragma unroll
+                        for (int j = 0; j < kSlots; ++j) before[j] += other > place[j];
+                    }
                 __syncthreads();
-                if (t < n) merged[before] = mineplace;
+#pragma unroll
+                for (int j = 0; j < kSlots; ++j)
+                    if (t + j * kThreads < n) merged[before[j]] = place[j];
                 __syncthreads();
                 // The sums run down the sorted list: the same for every CTA and
                 // run. A lane takes kList / 32 neighbours.
                 if (warp == 0) {
                     constexpr int kEach = kList / 32;
-                    double w[kEach], sum = 0.0;
+                    const int live = count > 0 ? min(n, count - s.count) : n;   // of the list, what top-k keeps
+                    float w[kEach], sum = 0.0f;
 #pragma unroll
                     for (int j = 0; j < kEach; ++j) {
-                        const int at_ = lane * kEach + j;
-                        w[j] = at_ < n ? double(ex2((logit_of_key(uint32_t(merged[at_] >> 32)) - m) * c)) : 0.0;
+                        const int q = lane * kEach + j;
+                        w[j] = q < live ? ex2((logit_of_key(uint32_t(merged[q] >> 32)) - m) * c) : 0.0f;
+                        sum += w[j];
                     }
-                    const int live = count > 0 ? min(n, count - s.count) : n;   // of the list, what top-k keeps
-#pragma unroll
-                    for (int j = 0; j < kEach; ++j) sum += lane * kEach + j < live ? w[j] : 0.0;
-                    double ahead = sum;   // up to and with this lane's
+                    float ahead = sum;   // up to and with this lane's
 #pragma unroll
                     for (int o = 1; o < 32; o <<= 1) {
-                        const double d = __shfl_up_sync(0xFFFFFFFFu, ahead, o);
+                        const float d = __shfl_up_sync(0xFFFFFFFFu, ahead, o);
                         if (lane >= o) ahead += d;
                     }
-                    const double total = double(s.mass) + __shfl_sync(0xFFFFFFFFu, ahead, 31);
-                    double before_me = double(s.mass) + __shfl_up_sync(0xFFFFFFFFu, ahead, 1);
-                    if (lane == 0) before_me = double(s.mass);
+                    const float total = s.mass + __shfl_sync(0xFFFFFFFFu, ahead, 31);
+                    float ahead_of_me = __shfl_up_sync(0xFFFFFFFFu, ahead, 1);
+                    ahead_of_me = s.mass + (lane ? ahead_of_me : 0.0f);
                     int stay = live;
                     if (count == 0 || (whole && by_p)) {
-                        if (count > 0) target = double(rp.top_p) * total;
+                        if (count > 0) target = double(rp.top_p) * double(total);
                         int here = 0;
 #pragma unroll
                         for (int j = 0; j < kEach; ++j) {
-                            here += lane * kEach + j < live && before_me < target;
-                            before_me += w[j];
+                            here += lane * kEach + j < live && double(ahead_of_me) < target;
+                            ahead_of_me += w[j];
                         }
                         stay = int(__reduce_add_sync(0xFFFFFFFFu, unsigned(here)));
                     }
                     if (lane == 0) {
                         sh.cut = stay > 0 ? merged[stay - 1] : merged[0] + 1;
-                        sh.kept = float(total);
+                        sh.kept = total;
                     }
                 }
                 __syncthreads();
                 *kept = sh.kept;
                 if (sh.cut > cut) cut = sh.cut;
-                if (whole) {
-                    raced = true;
-                    if (rank == 0 && t < n) {
-                        const uint64_t place = merged[t];   // (rank 0: i0 is 0)
-                        const float l = logit_of_key(uint32_t(place >> 32));
-                        const int i = int(~uint32_t(place));
-                        if (place >= cut && (l == m || !(rp.min_p > 0.0f) || ex2((l - m) * c) >= rp.min_p))
-                            run_race(l, i, noise[i]);
+                // Whole: rank 0 has them all in order. Else every CTA has its own.
+                if (whole ? rank == 0 : race_now) {
+                    const uint64_t* from = whole ? merged : list;
+                    const int count_of = whole ? n : int(sh.list_n);
+                    for (int j = t; j < count_of; j += kThreads) {
+                        const uint64_t at = from[j];
+                        const float l = logit_of_key(uint32_t(at >> 32));
+                        const int i = int(~uint32_t(at)) - i0;
+                        if (at >= cut && passes_min_p(l)) run_race(l, i0 + i, __ldg(noise + i));
                     }
                 }
+                raced = whole || race_now;
                 return true;
             };
             float kept = all.z;
-            bool settled = true;
-            if (by_k) settled = settle(k, 0.0, &kept);
-            if (settled && by_p && !raced) {
-                if (by_k) {   // again from the start, once the first cut's lists have been read
-                    cluster_barrier();
-                    if (t == 0) sh.first = sh.last = kBins, sh.list_n = 0;
-                    __syncthreads();
+            bool settled = false, count_now = true, k_stage = by_k;
+            for (;;) {
+                if (count_now) count_bins();
+                count_now = false;
+                settled = settle(k_stage ? k : 0, double(rp.top_p) * double(kept), !k_stage || !by_p, &kept);
+                if (!settled) {
+                    if (k_stage || !(low > sure) || sh.last < kBins) break;
+                    low = sure;   // the cut lies lower than was tried
+                    count_now = true;
+                } else {
+                    if (!k_stage || !by_p || raced) break;
+                    k_stage = false;
                 }
-                settled = settle(0, double(rp.top_p) * double(kept), &kept);
-                if (!settled && low > sure && sh.last >= kBins) {
-                    low = sure;
-                    cluster_barrier();
-                    count_bins();
-                    settled = settle(0, double(rp.top_p) * double(kept), &kept);
-                }
+                crew.barrier();   // every CTA is past its reads of this one's lists
+                if (t == 0) sh.first = sh.last = kBins, sh.list_n = sh.kept_n = 0;
+                __syncthreads();
             }
             if (!settled) {
                 const Weighed every = at(kKeyLow);
@@ -866,7 +947,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const Sample
                         const int mid = lo + (end - lo) / 2;
                         Weighed s{0, 0.0f};
                         sl.each([&](float l, int i) { s.count += i0 + i < mid && key_of(l) == th.key; });
-                        if (cluster_add(s, sh, rank, ranks, turn).count >= th.ties) end = mid;
+                        if (team_add(crew, s, sh, turn).count >= th.ties) end = mid;
                         else lo = mid;
                     }
                 }
@@ -879,8 +960,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const Sample
             if (rp.min_p > 0.0f) low = fmaxf(low, fminf(__log2f(rp.min_p) - 1e-3f, 0.0f));
             const auto stays = [&](float l, int i) {
                 const float y = (l - m) * c;
-                return y >= low && place_of(key_of(l), i0 + i) >= cut &&
-                       (l == m || !(rp.min_p > 0.0f) || ex2(y) >= rp.min_p);
+                return y >= low && place_of(key_of(l), i0 + i) >= cut && passes_min_p(l);
             };
             // Where a filter has left few columns they are listed first and
             // raced from the list, all their numbers in flight at once.
@@ -899,10 +979,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const Sample
                 __syncthreads();
                 const int n = int(sh.kept_n);
                 if (n <= kKept) {
-                    for (int j = t; j < n; j += kRowThreads) {
-                        const int i = int(kept_at[j]);
-                        run_race(sl.at(i), i0 + i, noise[i]);
-                    }
+                    race_kept(kept_at, n);
                 } else {
                     listed = false;
                 }
@@ -926,11 +1003,11 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const Sample
                     constexpr int W = P::kWidth, kAhead = 16 / W;
                     const int np = sl.packs();
                     const bool wide = (reinterpret_cast<uintptr_t>(noise) - 4u * unsigned(sl.shift)) % 16 == 0;
-                    for (int v0 = t; v0 < np; v0 += kRowThreads * kAhead) {
+                    for (int v0 = t; v0 < np; v0 += kThreads * kAhead) {
                         float u[kAhead * W];
 #pragma unroll
                         for (int g = 0; g < kAhead; ++g) {
-                            const int v = v0 + g * kRowThreads, i = v * W - sl.shift;
+                            const int v = v0 + g * kThreads, i = v * W - sl.shift;
                             if (v < np && i >= 0 && i + W <= sl.n && wide) {
 #pragma unroll
                                 for (int e = 0; e < W; e += 4) {
@@ -945,7 +1022,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const Sample
                         }
 #pragma unroll
                         for (int g = 0; g < kAhead; ++g) {
-                            const int v = v0 + g * kRowThreads;
+                            const int v = v0 + g * kThreads;
                             if (v >= np) break;
                             const P p = sl.mem[v];
 #pragma unroll
@@ -970,16 +1047,16 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const Sample
         const float x = __shfl_xor_sync(0xFFFFFFFFu, best_x, o);
         if (b > best) best = b, best_x = x;
     }
-    __shared__ uint64_t warp_best[kRowWarps];
+    __shared__ uint64_t warp_best[kWarps];
     if (lane == 0) warp_best[warp] = best, sh.wg[warp] = best_x;
     __syncthreads();
     if (t == 0) {
-        for (int w = 0; w < kRowWarps; ++w)
+        for (int w = 0; w < kWarps; ++w)
             if (warp_best[w] > best) best = warp_best[w], best_x = sh.wg[w];
-        put_l(at_rank(&sh.best[rank], 0), best);
-        put_f(at_rank(&sh.best_x[rank], 0), best_x);
+        put_l(crew.at(&sh.best[rank], 0), best);
+        put_f(crew.at(&sh.best_x[rank], 0), best_x);
     }
-    cluster_barrier();
+    crew.barrier();
     if (rank == 0 && t == 0) {
         for (int r = 0; r < ranks; ++r)
             if (sh.best[r] > best) best = sh.best[r], best_x = sh.best_x[r];
@@ -988,20 +1065,21 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const Sample
     }
 }
 
-template <typename T, bool kResident>
+template <typename T, bool kResident, int kThreads, bool kSolo>
 cudaError_t launch_rows(const SampleArgs& a, int ranks, int per, size_t smem, cudaStream_t s) {
-    if (const cudaError_t e = open_smem<sample_row_kernel<T, kResident>>(smem); e != cudaSuccess) return e;
+    constexpr auto kernel = sample_row_kernel<T, kResident, kThreads, kSolo>;
+    if (const cudaError_t e = open_smem<kernel>(smem); e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(a.rows * ranks));
-    cfg.blockDim = dim3(kRowThreads);
+    cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim = {unsigned(ranks), 1, 1};
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, sample_row_kernel<T, kResident>, a, ranks, per);
+    cfg.numAttrs = kSolo ? 0 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, a, ranks, per);
 }
 
 template <typename T>
@@ -1013,10 +1091,16 @@ cudaError_t launch_sample_t(const SampleArgs& a, cudaStream_t s) {
         else sample_warp_kernel<T, 32><<<grid, 128, 0, s>>>(a);
         return cudaGetLastError();
     }
-    const int ranks = a.cols <= 4096 ? 1 : a.cols <= 8192 ? 2 : a.cols <= 16384 ? 4 : kMaxCluster;
+    // Slices of at most 16384 columns (64 KB of float32: three CTAs an SM)
+    // while eight CTAs can hold the row; small rows in small CTAs, of which
+    // more run at once.
+    const int ranks = a.cols <= 16384 ? 1 : a.cols <= 32768 ? 2 : a.cols <= 65536 ? 4 : kMaxCluster;
     const int per = (a.cols + ranks - 1) / ranks;
     const size_t smem = size_t(per) * sizeof(T) + 32;   // up to 16 bytes of alignment at either end
-    return smem <= (size_t(200) << 10) ? launch_rows<T, true>(a, ranks, per, smem, s) : launch_rows<T, false>(a, ranks, per, 0, s);
+    if (a.cols <= 8192) return launch_rows<T, true, 128, true>(a, 1, per, smem, s);
+    if (ranks == 1) return launch_rows<T, true, 256, true>(a, 1, per, smem, s);
+    return smem <= (size_t(200) << 10) ? launch_rows<T, true, 256, false>(a, ranks, per, smem, s)
+                                       : launch_rows<T, false, 256, false>(a, ranks, per, 0, s);
 }
 
 }  // namespace
