@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(128) sample_warp_kernel(const SampleArgs a) {
 // than (1 - p) Z, so the prefix that top-p keeps ends above them.
 
 constexpr int kMaxCluster = 8, kMaxRowWarps = 8;
-constexpr int kBins = 512, kList = 256;
+constexpr int kBins = 512, kList = 256, kUpper = 2048;
 // Gumbel noise -log(-log u) lies in [-2.86, 16.64]: a logit with x < -19.6
 // loses to the maximum whatever their numbers, which need not be read.
 constexpr float kNoChance = -19.6f;
@@ -284,9 +284,9 @@ struct Part {   // what one CTA knows of its slice
 };
 
 struct RowShared {
-    uint32_t hist_n[kBins], hist_w[kBins];   // this CTA's; then the lists
-    uint32_t all_n[kBins], all_w[kBins];     // the cluster's; then the kept columns
-    uint32_t upto_n[kBins];                  // inclusive sums of all_n
+    uint32_t hist_n[kBins], hist_w[kBins];            // this CTA's; then the lists
+    uint32_t share_n[kBins / 2], share_w[kBins / 2];  // a cluster's CTA: its share of the bins, added over the cluster
+    uint16_t upper[kUpper];                           // the slice's upper columns, a part for each warp
     Part part[kMaxCluster];
     float f[2][kMaxCluster];
     int n[2][kMaxCluster];
@@ -294,12 +294,12 @@ struct RowShared {
     float best_x[kMaxCluster];
     float wf[kMaxRowWarps], wg[kMaxRowWarps], wh[kMaxRowWarps];
     int wn[kMaxRowWarps], wm[kMaxRowWarps], wk[kMaxRowWarps];
-    unsigned list_n, kept_n;
+    unsigned list_n;
     int first, last;
+    uint32_t down, above;
     float kept;
     uint64_t cut;
 };
-constexpr int kKept = 2 * kBins;   // columns that all_n and all_w hold
 static_assert(kList * 2 * 8 <= int(sizeof(uint32_t)) * kBins * 2, "a CTA's list and the merged one take the histogram's place");
 
 // The CTAs that share a row: kThreads each, one of them (kSolo) or a cluster.
@@ -412,7 +412,7 @@ struct Slice {
         if constexpr (kResident) {
             const uint4* base = reinterpret_cast<const uint4*>(src - shift);
             const int np = packs();
-            constexpr int kAhead = 4;
+            constexpr int kAhead = 8;
             for (int v0 = int(threadIdx.x); v0 < np; v0 += kThreads * kAhead) {
                 P p[kAhead];
 #pragma unroll
@@ -492,6 +492,56 @@ struct Slice {
             }
         }
     }
+    // The columns of each_above, in its order, into this warp's part of
+    // `upper`; returns their number, or -1 where they do not fit.
+    __device__ __forceinline__ int list_above(float l_min, uint16_t* part) const {
+        constexpr int kPart = kUpper / (kThreads / 32);
+        const int lane = int(threadIdx.x) & 31, first = int(threadIdx.x) & ~31;
+        int filled = 0;
+        if (n > 65536) return -1;
+        const auto put = [&](uint32_t marks, auto column) {   // a warp together
+            const int mine = __popc(marks);
+            int upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int d = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+                if (lane >= o) upto += d;
+            }
+            const int total = __shfl_sync(0xFFFFFFFFu, upto, 31);
+            if (filled + total <= kPart) {
+                for (int to = filled + upto - mine; marks; marks &= marks - 1) part[to++] = uint16_t(column(__ffs(int(marks)) - 1));
+            }
+            filled += total;
+        };
+        if constexpr (kResident) {
+            constexpr int kPacks = 32 / P::kWidth;
+            const int np = packs();
+            for (int w0 = first; w0 < np && filled <= kPart; w0 += kThreads * kPacks) {
+                const int v0 = w0 + lane;
+                uint32_t marks = 0;
+#pragma unroll
+                for (int g = 0; g < kPacks; ++g) {
+                    const int v = v0 + g * kThreads;
+                    if (v >= np) break;
+                    const P p = mem[v];
+#pragma unroll
+                    for (int e = 0; e < P::kWidth; ++e) marks |= p.get(e) >= l_min ? 1u << (g * P::kWidth + e) : 0u;
+                }
+                put(marks, [&](int b) { return (v0 + b / P::kWidth * kThreads) * P::kWidth - shift + b % P::kWidth; });
+            }
+        } else {
+            for (int w0 = first; w0 < n && filled <= kPart; w0 += kThreads * 32) {
+                uint32_t marks = 0;
+                for (int g = 0; g < 32; ++g) {
+                    const int i = w0 + lane + g * kThreads;
+                    if (i < n && direct(i) >= l_min) marks |= 1u << g;
+                }
+                put(marks, [&](int b) { return w0 + lane + b * kThreads; });
+            }
+        }
+        __syncwarp();
+        return filled <= kPart ? filled : -1;
+    }
     // The row's maximum is +inf (every CTA of the cluster learns it at once).
     __device__ void only_infinite() {
         infinite = true;
@@ -549,35 +599,46 @@ __device__ __forceinline__ Weighed team_add(const Team& team, Weighed v, RowShar
 struct Inclusive {
     uint32_t n, w;
 };
-// The histogram's inclusive sums up to this thread's bins, kPer neighbours.
-template <int kThreads>
+// The team's histogram at this thread's bins, kPer neighbours: a bin's sums
+// (in a cluster, from the CTA that added them up) and those up to it.
+template <class Team>
 struct Sums {
-    static constexpr int kPer = kBins / kThreads;
-    uint32_t n[kPer], w[kPer];
-    __device__ __forceinline__ void scan(RowShared& sh) {
+    static constexpr int kPer = kBins / Team::kThreads;
+    uint32_t own_n[kPer], n[kPer], w[kPer];
+    __device__ __forceinline__ void scan(const Team& team, RowShared& sh) {
         const int warp = int(threadIdx.x) >> 5, lane = int(threadIdx.x) & 31, b0 = int(threadIdx.x) * kPer;
         uint32_t sn = 0, sw = 0;
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
-            n[j] = sn += sh.all_n[b0 + j];
-            w[j] = sw += sh.all_w[b0 + j];
+            if constexpr (Team::kSolo) {
+                own_n[j] = sh.hist_n[b0 + j];
+                w[j] = sh.hist_w[b0 + j];
+            } else {
+                const int share = kBins / team.ranks, r = (b0 + j) / share, q = (b0 + j) % share;
+                own_n[j] = get_u(team.at(&sh.share_n[q], r));
+                w[j] = get_u(team.at(&sh.share_w[q], r));
+            }
         }
-        const uint32_t own_n = sn, own_w = sw;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            n[j] = sn += own_n[j];
+            w[j] = sw += w[j];
+        }
+        const uint32_t mine_n = sn, mine_w = sw;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t un = __shfl_up_sync(0xFFFFFFFFu, sn, o), uw = __shfl_up_sync(0xFFFFFFFFu, sw, o);
             if (lane >= o) sn += un, sw += uw;
         }
         if (lane == 31) sh.wn[warp] = int(sn), sh.wm[warp] = int(sw);
-        __syncthreads();
-        sn -= own_n;
-        sw -= own_w;
+        __syncthreads();   // (the lists may take the histogram's place after this)
+        sn -= mine_n;
+        sw -= mine_w;
         for (int v = 0; v < warp; ++v) sn += uint32_t(sh.wn[v]), sw += uint32_t(sh.wm[v]);
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
             n[j] += sn;
             w[j] += sw;
-            sh.upto_n[b0 + j] = n[j];
         }
     }
 };
@@ -696,25 +757,21 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
         uint64_t cut = place_of(kKeyLow, 0x7FFFFFFF);   // the last place kept
         bool raced = false;
         const auto passes_min_p = [&](float l) { return l == m || !(rp.min_p > 0.0f) || ex2((l - m) * c) >= rp.min_p; };
-        // The race among n listed columns of the slice, their numbers asked for
-        // some at a time.
-        const auto race_kept = [&](const uint32_t* at, int n) {
-            constexpr int kAhead = 4;
-            for (int j0 = t; j0 < n; j0 += kThreads * kAhead) {
-                int i[kAhead];
-                float u[kAhead];
-#pragma unroll
-                for (int g = 0; g < kAhead; ++g)
-                    if (j0 + g * kThreads < n) {
-                        i[g] = int(at[j0 + g * kThreads]);
-                        u[g] = __ldg(noise + i[g]);
-                    }
-#pragma unroll
-                for (int g = 0; g < kAhead; ++g)
-                    if (j0 + g * kThreads < n) {
-                        const float l = sl.at(i[g]);
-                        if (passes_min_p(l)) run_race(l, i0 + i[g], u[g]);
-                    }
+        // A little below the logit of log2 w = y (and never -inf, which stands
+        // around the slice).
+        const auto logit_below = [&](float y) { return fmaxf(m + y / c * 1.00001f - fabsf(m) * 1e-6f, -3.40282347e38f); };
+        // This warp's upper columns, while they fit (upper_n is not negative).
+        uint16_t* const part = sh.upper + warp * (kUpper / kWarps);
+        int upper_n = -1;
+        // f(l, i) for this thread's share of the logits of at least l_min.
+        const auto each_upper = [&](float l_min, auto f) {
+            if (upper_n < 0) {
+                sl.each_above(l_min, f);
+            } else {
+                for (int j = lane; j < upper_n; j += 32) {
+                    const int i = part[j];
+                    f(sl.at(i), i);
+                }
             }
         };
         if (by_k || by_p) {
@@ -743,16 +800,15 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
             const float fixed = 2147483648.0f / all.z;   // all masses together stay below 2^31 + cols / 2
             float steps;                                 // bins per unit of log2 w; the last bin holds `low`
             const auto bin_of = [&](float y) { return int(-y * steps); };
-            // A little below the logit of log2 w = y.
-            const auto logit_below = [&](float y) { return m + y / c * 1.00001f - fabsf(m) * 1e-6f; };
-            Sums<kThreads> upto;
+            Sums<Crew> upto;
             const auto count_bins = [&] {
                 low = fminf(low, -1e-3f);
                 steps = float(kBins - 1) / -low;
                 for (int b = t; b < kBins; b += kThreads) sh.hist_n[b] = sh.hist_w[b] = 0;
-                if (t == 0) sh.first = sh.last = kBins, sh.list_n = sh.kept_n = 0;
+                if (t == 0) sh.first = sh.last = kBins, sh.list_n = 0;
+                upper_n = sl.list_above(logit_below(low), part);
                 __syncthreads();
-                sl.each_above(logit_below(low), [&](float l, int) {
+                each_upper(logit_below(low), [&](float l, int) {
                     const float y = (l - m) * c;
                     if (y >= low) {
                         const int b = bin_of(y);
@@ -761,22 +817,25 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
                     }
                 });
                 crew.barrier();
-                // This CTA adds its share of the bins over the cluster, for everyone.
-                const int share = kBins / ranks;
-                for (int b = rank * share + t; b < (rank + 1) * share; b += kThreads) {
-                    uint32_t n[kMaxCluster], w[kMaxCluster];
+                if constexpr (!kSolo) {   // this CTA adds its share of the bins over the cluster
+                    const int share = kBins / ranks;
+                    for (int q = t; q < share; q += kThreads) {
+                        uint32_t n[kMaxCluster], w[kMaxCluster];
 #pragma unroll
-                    for (int r = 0; r < kMaxCluster; ++r)
-                        if (r < ranks) n[r] = get_u(crew.at(&sh.hist_n[b], r)), w[r] = get_u(crew.at(&sh.hist_w[b], r));
+                        for (int r = 0; r < kMaxCluster; ++r)
+                            if (r < ranks) {
+                                n[r] = get_u(crew.at(&sh.hist_n[rank * share + q], r));
+                                w[r] = get_u(crew.at(&sh.hist_w[rank * share + q], r));
+                            }
 #pragma unroll
-                    for (int r = 1; r < kMaxCluster; ++r)
-                        if (r < ranks) n[0] += n[r], w[0] += w[r];
-#pragma unroll
-                    for (int r = 0; r < kMaxCluster; ++r)
-                        if (r < ranks) put_u(crew.at(&sh.all_n[b], r), n[0]), put_u(crew.at(&sh.all_w[b], r), w[0]);
+                        for (int r = 1; r < kMaxCluster; ++r)
+                            if (r < ranks) n[0] += n[r], w[0] += w[r];
+                        sh.share_n[q] = n[0];
+                        sh.share_w[q] = w[0];
+                    }
+                    crew.barrier();
                 }
-                crew.barrier();
-                upto.scan(sh);
+                upto.scan(crew, sh);
             };
             uint64_t* list = reinterpret_cast<uint64_t*>(sh.hist_n);
             uint64_t* merged = list + kList;
@@ -784,13 +843,13 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
             // of mass `target`. False: the histogram does not settle it. kept:
             // the mass that the cut is taken from. `final`: the last filter, so
             // that what lies above its cut is raced on the way. (sh.first,
-            // sh.last, sh.list_n and sh.kept_n are at their starts before it.)
+            // sh.last and sh.list_n are at their starts before it.)
             const auto settle = [&](int count, double target, bool final, float* kept) -> bool {
 #pragma unroll
-                for (int j = 0; j < Sums<kThreads>::kPer; ++j) {
-                    const int b = t * Sums<kThreads>::kPer + j;
+                for (int j = 0; j < Sums<Crew>::kPer; ++j) {
+                    const int b = t * Sums<Crew>::kPer + j;
                     if (count > 0) {
-                        if (upto.n[j] >= uint32_t(count) && upto.n[j] - sh.all_n[b] < uint32_t(count)) sh.first = sh.last = b;
+                        if (upto.n[j] >= uint32_t(count) && upto.n[j] - upto.own_n[j] < uint32_t(count)) sh.first = sh.last = b;
                     } else {
                         // A fixed-point sum is off by half a unit a logit, and by
                         // the masses' own rounding, a few 2^-22 of it.
@@ -803,32 +862,31 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
                 int first = sh.first;
                 const int last = sh.last;
                 if (last >= kBins) return false;
+#pragma unroll
+                for (int j = 0; j < Sums<Crew>::kPer; ++j) {
+                    const int b = t * Sums<Crew>::kPer + j;
+                    if (b == last) sh.down = upto.n[j];
+                    if (b == first) sh.above = upto.n[j] - upto.own_n[j];
+                }
+                __syncthreads();
                 // Few enough down to the cut: all of them are listed, and raced there.
-                const uint32_t down = sh.upto_n[last], above = first > 0 ? sh.upto_n[first - 1] : 0u;
-                const bool whole = down <= uint32_t(kList);
-                if (!whole && down - above > uint32_t(kList)) return false;
+                const bool whole = sh.down <= uint32_t(kList);
+                if (!whole && sh.down - sh.above > uint32_t(kList)) return false;
                 if (whole) first = 0;
-                uint32_t* const kept_at = sh.all_n;
                 Weighed s{0, 0.0f};
-                sl.each_above(logit_below(fmaxf(low, -float(last + 2) / steps)), [&](float l, int i) {
+                each_upper(logit_below(fmaxf(low, -float(last + 2) / steps)), [&](float l, int i) {
                     const float y = (l - m) * c;
                     if (y >= low) {
                         const int b = bin_of(y);
                         if (b < first) {
                             ++s.count;
                             s.mass += ex2(y);
-                            if (final) {
-                                const unsigned at = atomicAdd(&sh.kept_n, 1u);
-                                if (at < unsigned(kKept)) kept_at[at] = uint32_t(i);
-                            }
+                            if (final && passes_min_p(l)) run_race(l, i0 + i, __ldg(noise + i));
                         } else if (b <= last) {
                             list[atomicAdd(&sh.list_n, 1u)] = place_of(key_of(l), i0 + i);
                         }
                     }
                 });
-                __syncthreads();
-                const bool race_now = final && !whole && sh.kept_n <= unsigned(kKept);
-                if (race_now) race_kept(kept_at, int(sh.kept_n));
                 s = team_add(crew, s, sh, turn);   // (also: every list is written)
                 // All lists here, then in order.
                 constexpr int kSlots = kList / kThreads;
@@ -854,6 +912,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
                 __syncthreads();
                 int before[kSlots] = {};
                 if (t < n)
+#pragma unroll 8
                     for (int q = 0; q < n; ++q) {
                         const uint64_t other = merged[q];
 #pragma unroll
@@ -865,15 +924,16 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
                     if (t + j * kThreads < n) merged[before[j]] = place[j];
                 __syncthreads();
                 // The sums run down the sorted list: the same for every CTA and
-                // run. A lane takes kList / 32 neighbours.
+                // run. A lane takes `each` neighbours.
                 if (warp == 0) {
                     constexpr int kEach = kList / 32;
+                    const int each = (n + 31) / 32;
                     const int live = count > 0 ? min(n, count - s.count) : n;   // of the list, what top-k keeps
                     float w[kEach], sum = 0.0f;
 #pragma unroll
                     for (int j = 0; j < kEach; ++j) {
-                        const int q = lane * kEach + j;
-                        w[j] = q < live ? ex2((logit_of_key(uint32_t(merged[q] >> 32)) - m) * c) : 0.0f;
+                        const int q = lane * each + j;
+                        w[j] = j < each && q < live ? ex2((logit_of_key(uint32_t(merged[q] >> 32)) - m) * c) : 0.0f;
                         sum += w[j];
                     }
                     float ahead = sum;   // up to and with this lane's
@@ -891,7 +951,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
                         int here = 0;
 #pragma unroll
                         for (int j = 0; j < kEach; ++j) {
-                            here += lane * kEach + j < live && double(ahead_of_me) < target;
+                            here += j < each && lane * each + j < live && double(ahead_of_me) < target;
                             ahead_of_me += w[j];
                         }
                         stay = int(__reduce_add_sync(0xFFFFFFFFu, unsigned(here)));
@@ -905,17 +965,17 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
                 *kept = sh.kept;
                 if (sh.cut > cut) cut = sh.cut;
                 // Whole: rank 0 has them all in order. Else every CTA has its own.
-                if (whole ? rank == 0 : race_now) {
+                if (whole ? rank == 0 : final) {
                     const uint64_t* from = whole ? merged : list;
-                    const int count_of = whole ? n : int(sh.list_n);
-                    for (int j = t; j < count_of; j += kThreads) {
+                    const int those = whole ? n : int(sh.list_n);
+                    for (int j = t; j < those; j += kThreads) {
                         const uint64_t at = from[j];
                         const float l = logit_of_key(uint32_t(at >> 32));
                         const int i = int(~uint32_t(at)) - i0;
                         if (at >= cut && passes_min_p(l)) run_race(l, i0 + i, __ldg(noise + i));
                     }
                 }
-                raced = whole || race_now;
+                raced = whole || final;
                 return true;
             };
             float kept = all.z;
@@ -933,7 +993,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
                     k_stage = false;
                 }
                 crew.barrier();   // every CTA is past its reads of this one's lists
-                if (t == 0) sh.first = sh.last = kBins, sh.list_n = sh.kept_n = 0;
+                if (t == 0) sh.first = sh.last = kBins, sh.list_n = 0;
                 __syncthreads();
             }
             if (!settled) {
@@ -962,29 +1022,17 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
                 const float y = (l - m) * c;
                 return y >= low && place_of(key_of(l), i0 + i) >= cut && passes_min_p(l);
             };
-            // Where a filter has left few columns they are listed first and
-            // raced from the list, all their numbers in flight at once.
-            bool listed = by_k || by_p || rp.min_p > 0.0f;
-            if (listed) {
-                __syncthreads();
-                if (t == 0) sh.kept_n = 0;
-                __syncthreads();
-                uint32_t* kept_at = sh.all_n;
-                sl.each_above(cut_l, [&](float l, int i) {
-                    if (stays(l, i)) {
-                        const unsigned at = atomicAdd(&sh.kept_n, 1u);
-                        if (at < unsigned(kKept)) kept_at[at] = uint32_t(i);
-                    }
-                });
-                __syncthreads();
-                const int n = int(sh.kept_n);
-                if (n <= kKept) {
-                    race_kept(kept_at, n);
-                } else {
-                    listed = false;
-                }
+            // Where a filter leaves few columns they are listed first and raced
+            // from the list.
+            if (by_k || by_p || rp.min_p > 0.0f) {
+                const float l_min = fmaxf(cut_l, logit_below(low));
+                upper_n = sl.list_above(l_min, part);
+                if (upper_n >= 0)
+                    each_upper(l_min, [&](float l, int i) {
+                        if (stays(l, i)) run_race(l, i0 + i, __ldg(noise + i));
+                    });
             }
-            if (!listed) {
+            if (upper_n < 0) {
                 // -log u >= 1 - u, so that log2(w) - log2(1 - u) bounds a
                 // column's key from above: the two logarithms (accurate, where
                 // the bound's are approximate: the margin) are taken only
