@@ -40,21 +40,38 @@ __device__ __forceinline__ uint32_t key_of(float l) {
     return b ^ (b >> 31 ? 0xFFFFFFFFu : 0x80000000u);
 }
 
-template <typename T>
-__device__ __forceinline__ float logit_at(const SampleArgs& a, const T* row, const uint8_t* legal, int i) {
-    float l = float(row[i]);
-    if ((legal && !legal[i]) || l != l) l = neg_inf();
-    return l;
+// Noise as the race takes it; a NaN is read as the lowest number.
+__device__ __forceinline__ float clamped(float u) { return fminf(fmaxf(u, kULow), kUHigh); }
+
+__device__ __forceinline__ float race(float x, float u) { return x - logf(-logf(clamped(u))); }
+
+constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
+
+__device__ __forceinline__ float ex2(float y) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
+    return r;
 }
 
-__device__ __forceinline__ float scaled(float l, float m, float inv_t) {
-    const float x = (l - m) * inv_t;
-    return l == m ? 0.0f : x == x ? x : neg_inf();   // (an infinite m over an infinite T)
+__device__ __forceinline__ float lg2(float x) {   // x >= 2^-25
+    float r;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
 }
 
-__device__ __forceinline__ float race(float x, float u) {
-    // fmaxf reads a NaN as the lowest number.
-    return x - logf(-logf(fminf(fmaxf(u, kULow), kUHigh)));
+// w = 2^((l - m) c). The bounds keep 0 * c and -inf * c what they should be
+// whatever the temperature.
+__device__ __forceinline__ float log2_scale(float temperature) { return fminf(fmaxf(kLog2e / temperature, 1e-38f), 3e38f); }
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+    return v;
 }
 
 // A row's numbers.
@@ -84,45 +101,69 @@ struct Weighed {
     float mass;
 };
 
+__device__ __forceinline__ float logit_of_key(uint32_t key) {
+    return __uint_as_float(key >> 31 ? key ^ 0x80000000u : ~key);
+}
+
+// A key inside (lo, hi), hi - lo > 1: the middle logit's for the first steps,
+// which about halves the logits between where they lie evenly; then the
+// middle key, which ends after 32 steps whatever their distribution.
+__device__ __forceinline__ uint32_t between(uint32_t lo, uint32_t hi, int step) {
+    if (step < 16) {
+        const uint32_t mid = key_of(0.5f * logit_of_key(lo) + 0.5f * logit_of_key(hi));
+        if (mid > lo && mid < hi) return mid;
+    }
+    return lo + (hi - lo) / 2;
+}
+
 // The threshold of a row's filters. at(k): count and mass of the logits
-// with key >= k, the same on every calling thread. top: the largest key.
-template <class At>
-__device__ Threshold find_threshold(const RowParams& rp, uint32_t top, int valid, float mass, At at) {
+// with key >= k, the same on every calling thread; count_at(k): the count
+// alone. top: the largest key; low_k, low_p: keys at or below which top-k's
+// and top-p's cuts should lie (a hint: the lowest key is tried otherwise).
+template <class At, class CountAt>
+__device__ Threshold find_threshold(const RowParams& rp, uint32_t top, uint32_t low_k, uint32_t low_p, int valid, float mass,
+                                    At at, CountAt count_at) {
     Threshold th{kKeyLow, kAllTies};
     const int k = rp.first_k();
     float kept = mass;   // mass of what is kept so far
     if (k > 0 && k < valid) {
-        uint32_t lo = kKeyLow, hi = top + 1;   // count(lo) >= k > count(hi)
-        Weighed wlo{valid, mass}, whi{0, 0.0f};
-        while (hi - lo > 1 && wlo.count != k) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            const Weighed w = at(mid);
-            if (w.count >= k) lo = mid, wlo = w;
-            else hi = mid, whi = w;
+        uint32_t lo = max(low_k, kKeyLow), hi = top + 1;   // count(lo) >= k > count(hi)
+        int clo = lo > kKeyLow ? count_at(lo) : valid, chi = 0;
+        if (clo < k) hi = lo, chi = clo, lo = kKeyLow, clo = valid;
+        for (int step = 0; hi - lo > 1 && clo != k; ++step) {
+            const uint32_t mid = between(lo, hi, step);
+            const int n = count_at(mid);
+            if (n >= k) lo = mid, clo = n;
+            else hi = mid, chi = n;
         }
         th.key = lo;
-        kept = wlo.mass;
-        if (wlo.count != k) {   // ties at lo: the first k - count(hi) of them
-            th.ties = k - whi.count;
-            kept = whi.mass + (wlo.mass - whi.mass) * (float(th.ties) / float(wlo.count - whi.count));
+        if (clo != k) th.ties = k - chi;   // ties at lo: the first k - count(hi) of them
+        if (k == 1 || !rp.filters_p()) return th;
+        kept = at(lo).mass;
+        if (clo != k) {
+            const float above = at(hi).mass;
+            kept = above + (kept - above) * (float(th.ties) / float(clo - chi));
         }
-        if (k == 1) return th;
     }
     if (rp.filters_p()) {
-        const double target = double(rp.top_p) * double(kept);
-        uint32_t lo = th.key, hi = top + 1;   // mass(lo) >= target > mass(hi)
+        const float target = rp.top_p * kept;
+        uint32_t lo = max(low_p, th.key), hi = top + 1;   // mass(lo) >= target > mass(hi)
         Weighed wlo = at(lo), whi{0, 0.0f};
-        while (hi - lo > 1 && wlo.count - whi.count > 1) {
-            const uint32_t mid = lo + (hi - lo) / 2;
+        if (wlo.mass < target && lo > th.key) {
+            hi = lo, whi = wlo;
+            lo = th.key, wlo = at(lo);
+        }
+        for (int step = 0; hi - lo > 1 && wlo.count - whi.count > 1; ++step) {
+            const uint32_t mid = between(lo, hi, step);
             const Weighed w = at(mid);
-            if (double(w.mass) >= target) lo = mid, wlo = w;
+            if (w.mass >= target) lo = mid, wlo = w;
             else hi = mid, whi = w;
         }
         const int group = wlo.count - whi.count;   // equal logits unless there is only one
         int ties = kAllTies;
         if (group > 1) {
             const double each = (double(wlo.mass) - double(whi.mass)) / group;
-            const double need = each > 0.0 ? ceil((target - double(whi.mass)) / each) : double(group);
+            const double need = each > 0.0 ? ceil((double(rp.top_p) * double(kept) - double(whi.mass)) / each) : double(group);
             ties = need < 1.0 ? 1 : need >= double(group) ? kAllTies : int(need);
         }
         if (lo > th.key) th = Threshold{lo, ties};
@@ -134,6 +175,10 @@ __device__ Threshold find_threshold(const RowParams& rp, uint32_t top, int valid
 // -------------------------------------------------------- a warp per row
 //
 // Up to 32 * kPer columns: lane l holds columns l, l + 32, ... in registers.
+// One warp has no other to hide its latency behind, so everything is asked
+// for at once, the reductions are single instructions where the type allows,
+// and the race's two accurate logarithms are taken only for the columns that
+// cheap bounds of their keys leave in it.
 template <typename T, int kPer>
 __global__ void __launch_bounds__(128) sample_warp_kernel(const SampleArgs a) {
     const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
@@ -143,16 +188,27 @@ __global__ void __launch_bounds__(128) sample_warp_kernel(const SampleArgs a) {
     const RowParams rp(a, row);
     const T* logits = static_cast<const T*>(a.logits) + size_t(row) * size_t(a.ld);
     const uint8_t* legal = a.legal ? a.legal + size_t(row) * size_t(a.legal_ld) : nullptr;
-    float l[kPer];
-    float m = neg_inf();
+    const float* noise = a.noise ? a.noise + size_t(row) * size_t(a.noise_ld) : nullptr;
+    float l[kPer], u[kPer];   // the numbers are few: asked for before it shows which are needed
+    {
+        T raw[kPer];
+        uint8_t open[kPer];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-        const int i = j * 32 + lane;
-        l[j] = i < a.cols ? logit_at(a, logits, legal, i) : neg_inf();
-        m = fmaxf(m, l[j]);
+        for (int j = 0; j < kPer; ++j) {
+            const int i = j * 32 + lane;
+            const bool in = i < a.cols;
+            raw[j] = in ? logits[i] : T(0.0f);
+            open[j] = in ? (legal ? legal[i] : uint8_t(1)) : uint8_t(0);
+            u[j] = in && noise ? __ldg(noise + i) : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) l[j] = open[j] ? fmaxf(float(raw[j]), neg_inf()) : neg_inf();   // (a NaN: -inf)
     }
+    float lane_top = neg_inf();
 #pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
+    for (int j = 0; j < kPer; ++j) lane_top = fmaxf(lane_top, l[j]);
+    uint32_t top = __reduce_max_sync(kFull, key_of(lane_top));
+    float m = logit_of_key(top);
     if (m == neg_inf()) {   // nothing to choose from
         if (lane == 0) {
             a.moves[row] = -1;
@@ -172,62 +228,98 @@ __global__ void __launch_bounds__(128) sample_warp_kernel(const SampleArgs a) {
         }
         return;
     }
-    const float inv_t = 1.0f / rp.temperature;
-    uint32_t key[kPer];
-    float x[kPer], w[kPer];
-    float z = 0.0f;
-    int valid = 0;
+    if (m == __uint_as_float(0x7F800000u)) {   // the infinite logits share everything
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) l[j] = l[j] == m ? 0.0f : neg_inf();
+        lane_top = lane_top == m ? 0.0f : neg_inf();
+        m = 0.0f;
+        top = key_of(m);
+    }
+    const float c = log2_scale(rp.temperature);
+    float w[kPer], z = 0.0f;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-        key[j] = key_of(l[j]);
-        x[j] = scaled(l[j], m, inv_t);
-        w[j] = key[j] >= kKeyLow ? expf(x[j]) : 0.0f;
+        w[j] = ex2((l[j] - m) * c);
         z += w[j];
-        valid += key[j] >= kKeyLow;
     }
+    z = warp_sum(z);
+    uint32_t in = 0;   // this lane's kept columns, bit j for column j * 32 + lane
+    Threshold th{kKeyLow, kAllTies};
+    if (rp.first_k() > 0 || rp.filters_p()) {
+        const auto count_at = [&](uint32_t at) {
+            unsigned n = 0;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(kFull, z, o);
-    valid = int(__reduce_add_sync(kFull, unsigned(valid)));
-    const Threshold th = find_threshold(rp, key_of(m), valid, z, [&](uint32_t at) {
-        Weighed s{0, 0.0f};
+            for (int j = 0; j < kPer; ++j) n += key_of(l[j]) >= at;
+            return int(__reduce_add_sync(kFull, n));
+        };
+        const auto at = [&](uint32_t key) {
+            Weighed s{0, 0.0f};
 #pragma unroll
-        for (int j = 0; j < kPer; ++j)
-            if (key[j] >= at) {
-                ++s.count;
-                s.mass += w[j];
-            }
-        s.count = int(__reduce_add_sync(kFull, unsigned(s.count)));
+            for (int j = 0; j < kPer; ++j)
+                if (key_of(l[j]) >= key) {
+                    ++s.count;
+                    s.mass += w[j];
+                }
+            s.count = int(__reduce_add_sync(kFull, unsigned(s.count)));
+            s.mass = warp_sum(s.mass);
+            return s;
+        };
+        // Up to 32, the k-th largest is at least the least of the lanes'
+        // largest; beyond, at least the least of all.
+        float least = lane_top;
+        if (rp.first_k() > 32) {
 #pragma unroll
-        for (int o = 16; o; o >>= 1) s.mass += __shfl_xor_sync(kFull, s.mass, o);
-        return s;
-    });
-    const float* noise = a.noise + size_t(row) * size_t(a.noise_ld);
-    float best = neg_inf(), best_x = 0.0f;
-    uint32_t best_i = 0xFFFFFFFFu;
+            for (int j = 0; j < kPer; ++j) least = fminf(least, l[j] > neg_inf() ? l[j] : least);
+        }
+        const uint32_t low_k = __reduce_min_sync(kFull, least > neg_inf() ? key_of(least) : 0xFFFFFFFFu);
+        const uint32_t low_p = key_of(m + __log2f((1.0f - rp.top_p) * 0.99f * z / float(a.cols)) / c);
+        th = find_threshold(rp, top, low_k, low_p, rp.first_k() > 0 ? count_at(kKeyLow) : 0, z, at, count_at);
+    }
     int seen = 0;   // logits equal to the threshold, in columns before
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-        const int i = j * 32 + lane;
-        bool keep = key[j] >= th.key && (w[j] >= rp.min_p || l[j] == m || !(rp.min_p > 0.0f));
+        const uint32_t key = key_of(l[j]);
+        bool keep = key >= th.key && (l[j] == m || !(rp.min_p > 0.0f) || w[j] >= rp.min_p);
         if (th.ties != kAllTies) {
-            const uint32_t tied = __ballot_sync(kFull, key[j] == th.key);
-            if (key[j] == th.key && seen + __popc(tied & ((1u << lane) - 1u)) >= th.ties) keep = false;
+            const uint32_t tied = __ballot_sync(kFull, key == th.key);
+            if (key == th.key && seen + __popc(tied & ((1u << lane) - 1u)) >= th.ties) keep = false;
             seen += __popc(tied);
         }
-        if (keep) {
-            const float r = race(x[j], noise[i]);
-            if (r > best) best = r, best_i = uint32_t(i), best_x = x[j];
-        }
+        in |= keep ? 1u << j : 0u;
     }
+    // With d = 1 - u: d <= -log u <= d / u, so a column's key x - log(-log u)
+    // lies, in log2, between y - lg2(d) + lg2(u) and y - lg2(d). Only those
+    // whose upper bound reaches the largest lower one (less the logarithms'
+    // error) can win.
+    float need = neg_inf();
+    const auto upper = [&](int j) { return (l[j] - m) * c - lg2(1.0f - u[j]); };
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const float r = __shfl_xor_sync(kFull, best, o);
-        const uint32_t i = __shfl_xor_sync(kFull, best_i, o);
-        const float bx = __shfl_xor_sync(kFull, best_x, o);
-        if (r > best || (r == best && i < best_i)) best = r, best_i = i, best_x = bx;
+    for (int j = 0; j < kPer; ++j) {
+        u[j] = clamped(u[j]);
+        if (in >> j & 1u) need = fmaxf(need, upper(j) + lg2(u[j]));
     }
-    if (lane == 0) {
-        a.moves[row] = (long long)best_i;
+    need = logit_of_key(__reduce_max_sync(kFull, key_of(need))) - 2e-3f;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+        if (!(upper(j) >= need)) in &= ~(1u << j);
+    uint32_t best = 0, best_i = 0xFFFFFFFFu;   // the largest key of the race, as an ordered integer
+    float best_x = 0.0f;
+    while (in) {
+        const int b = __ffs(int(in)) - 1, i = b * 32 + lane;
+        in &= in - 1;
+        float lb = 0.0f, ub = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+            if (j == b) lb = l[j], ub = u[j];
+        const float x = (lb - m) * c * kLn2;
+        const uint32_t key = key_of(race(x, ub));
+        if (key > best) best = key, best_i = uint32_t(i), best_x = x;   // (columns ascend)
+    }
+    __syncwarp();
+    const uint32_t winner = __reduce_max_sync(kFull, best);
+    const uint32_t column = __reduce_min_sync(kFull, best == winner ? best_i : 0xFFFFFFFFu);
+    if (best == winner && best_i == column) {
+        a.moves[row] = (long long)column;
         if (a.logprob) a.logprob[row] = best_x - logf(z);
     }
 }
@@ -260,17 +352,6 @@ constexpr int kBins = 512, kList = 256, kUpper = 2048;
 // Gumbel noise -log(-log u) lies in [-2.86, 16.64]: a logit with x < -19.6
 // loses to the maximum whatever their numbers, which need not be read.
 constexpr float kNoChance = -19.6f;
-constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
-
-__device__ __forceinline__ float ex2(float y) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
-    return r;
-}
-
-__device__ __forceinline__ float logit_of_key(uint32_t key) {
-    return __uint_as_float(key >> 31 ? key ^ 0x80000000u : ~key);
-}
 
 // Descending order of logits, ties by ascending column, as descending numbers.
 __device__ __forceinline__ uint64_t place_of(uint32_t key, int i) { return uint64_t(key) << 32 | uint32_t(~uint32_t(i)); }
@@ -333,17 +414,6 @@ __device__ __forceinline__ void put_l(uint32_t a, unsigned long long v) { asm vo
 __device__ __forceinline__ unsigned long long get_l(uint32_t a) {
     unsigned long long v;
     asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
-    return v;
-}
-
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-    return v;
-}
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
     return v;
 }
 
@@ -679,8 +749,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
     float m = neg_inf();
     for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sh.wf[w]);
     const bool greedy = rp.greedy();
-    // w = 2^((l - m) c). The bounds keep 0 * c and -inf * c what they should be.
-    const float c = greedy ? 1.0f : fminf(fmaxf(kLog2e / rp.temperature, 1e-38f), 3e38f);
+    const float c = greedy ? 1.0f : log2_scale(rp.temperature);
     {
         Weighed s{0, 0.0f};
         if (!greedy && m > neg_inf()) {
@@ -874,19 +943,44 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
                 if (!whole && sh.down - sh.above > uint32_t(kList)) return false;
                 if (whole) first = 0;
                 Weighed s{0, 0.0f};
-                each_upper(logit_below(fmaxf(low, -float(last + 2) / steps)), [&](float l, int i) {
+                // A column's bin against the cut's: above it is kept for certain
+                // (and raced if no filter follows).
+                const auto place_in = [&](float l, int i) -> bool {
                     const float y = (l - m) * c;
-                    if (y >= low) {
-                        const int b = bin_of(y);
-                        if (b < first) {
-                            ++s.count;
-                            s.mass += ex2(y);
-                            if (final && passes_min_p(l)) run_race(l, i0 + i, __ldg(noise + i));
-                        } else if (b <= last) {
-                            list[atomicAdd(&sh.list_n, 1u)] = place_of(key_of(l), i0 + i);
-                        }
+                    if (!(y >= low)) return false;
+                    const int b = bin_of(y);
+                    if (b < first) {
+                        ++s.count;
+                        s.mass += ex2(y);
+                        return final && passes_min_p(l);
                     }
-                });
+                    if (b <= last) list[atomicAdd(&sh.list_n, 1u)] = place_of(key_of(l), i0 + i);
+                    return false;
+                };
+                if (upper_n < 0) {
+                    sl.each_above(logit_below(fmaxf(low, -float(last + 2) / steps)), [&](float l, int i) {
+                        if (place_in(l, i)) run_race(l, i0 + i, __ldg(noise + i));
+                    });
+                } else {
+                    constexpr int kAhead = 4;   // numbers asked for before the first is used
+                    for (int j0 = lane; j0 < upper_n; j0 += 32 * kAhead) {
+                        int i[kAhead];
+                        float u[kAhead];
+                        uint32_t in = 0;
+#pragma unroll
+                        for (int g = 0; g < kAhead; ++g)
+                            if (j0 + 32 * g < upper_n) {
+                                i[g] = part[j0 + 32 * g];
+                                if (place_in(sl.at(i[g]), i[g])) {
+                                    in |= 1u << g;
+                                    u[g] = __ldg(noise + i[g]);
+                                }
+                            }
+#pragma unroll
+                        for (int g = 0; g < kAhead; ++g)
+                            if (in >> g & 1u) run_race(sl.at(i[g]), i0 + i[g], u[g]);
+                    }
+                }
                 s = team_add(crew, s, sh, turn);   // (also: every list is written)
                 // All lists here, then in order.
                 constexpr int kSlots = kList / kThreads;
@@ -998,8 +1092,9 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
             }
             if (!settled) {
                 const Weighed every = at(kKeyLow);
-                RowParams only = rp;
-                const Threshold th = find_threshold(only, key_of(m), every.count, every.mass, at);
+                const uint32_t hint = key_of(logit_below(sure));
+                const Threshold th = find_threshold(rp, key_of(m), hint, hint, every.count, every.mass, at,
+                                                    [&](uint32_t key) { return at(key).count; });
                 int end = a.cols;   // the column after the threshold's last tie kept
                 if (th.ties != kAllTies) {
                     int lo = 0;     // ties before lo < th.ties <= ties before end
@@ -1038,12 +1133,12 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
                 // the bound's are approximate: the margin) are taken only
                 // where the bound reaches the warp's best so far.
                 float lead = neg_inf();   // the warp's best key, in log2
-                const auto bound = [&](float l, float u) { return (l - m) * c - __log2f(fmaxf(1.0f - u, 5.9604645e-8f)) + 1e-3f; };
+                const auto bound = [&](float l, float u) { return (l - m) * c - lg2(fmaxf(1.0f - u, 5.9604645e-8f)) + 1e-3f; };
                 const auto consider = [&](float l, int i, float u) {
                     if (bound(l, u) >= lead && stays(l, i)) run_race(l, i0 + i, u);
                 };
-                const auto follow = [&] {   // (a warp's lanes together)
-                    const uint32_t k = __reduce_max_sync(__activemask(), uint32_t(best >> 32));
+                const auto follow = [&] {
+                    const uint32_t k = __reduce_max_sync(0xFFFFFFFFu, uint32_t(best >> 32));
                     if (k) lead = logit_of_key(k) * kLog2e;
                 };
                 if constexpr (kResident) {
@@ -1051,11 +1146,11 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
                     constexpr int W = P::kWidth, kAhead = 16 / W;
                     const int np = sl.packs();
                     const bool wide = (reinterpret_cast<uintptr_t>(noise) - 4u * unsigned(sl.shift)) % 16 == 0;
-                    for (int v0 = t; v0 < np; v0 += kThreads * kAhead) {
+                    for (int w0 = t & ~31; w0 < np; w0 += kThreads * kAhead) {   // a warp's lanes stay together
                         float u[kAhead * W];
 #pragma unroll
                         for (int g = 0; g < kAhead; ++g) {
-                            const int v = v0 + g * kThreads, i = v * W - sl.shift;
+                            const int v = w0 + lane + g * kThreads, i = v * W - sl.shift;
                             if (v < np && i >= 0 && i + W <= sl.n && wide) {
 #pragma unroll
                                 for (int e = 0; e < W; e += 4) {
@@ -1070,19 +1165,30 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
                         }
 #pragma unroll
                         for (int g = 0; g < kAhead; ++g) {
-                            const int v = v0 + g * kThreads;
-                            if (v >= np) break;
-                            const P p = sl.mem[v];
+                            const int v = w0 + lane + g * kThreads;
+                            P p;
+                            float most = neg_inf();
+                            if (v < np) {
+                                p = sl.mem[v];
 #pragma unroll
-                            for (int e = 0; e < W; ++e) consider(p.get(e), v * W - sl.shift + e, u[g * W + e]);
+                                for (int e = 0; e < W; ++e) most = fmaxf(most, bound(p.get(e), u[g * W + e]));
+                            }
+                            if (!__any_sync(0xFFFFFFFFu, most >= lead)) continue;
+                            if (v < np) {
+#pragma unroll
+                                for (int e = 0; e < W; ++e) consider(p.get(e), v * W - sl.shift + e, u[g * W + e]);
+                            }
+                            __syncwarp();
                             follow();
                         }
                     }
                 } else {
-                    sl.each([&](float l, int i) {
-                        consider(l, i, __ldg(noise + i));
+                    for (int w0 = t & ~31; w0 < sl.n; w0 += kThreads) {
+                        const int i = w0 + lane;
+                        if (i < sl.n) consider(sl.direct(i), i, __ldg(noise + i));
+                        __syncwarp();
                         follow();
-                    });
+                    }
                 }
             }
         }
