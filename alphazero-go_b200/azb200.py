@@ -141,7 +141,7 @@ def lib() -> C.CDLL:
             L.azb_mx4_quantise.argtypes = [i, V, i, ll, ll, ll, V, V, V] + err
             L.azb_mx4_values.argtypes = [i, V, V, ll, ll, V, i, ll, V] + err
             L.azb_mx4_product.argtypes = [i, V, V, ll, V, V, ll, ll, V, i, V, i, ll, V] + err
-            L.azb_mx4_linear_workspace.argtypes = [ll, ll]
+            L.azb_mx4_linear_workspace.argtypes = [ll, ll, ll]
             L.azb_mx4_linear_workspace.restype = s
             L.azb_mx4_linear.argtypes = [i, V, i, ll, ll, ll, V, V, ll, V, i, V, i, ll, V, s, V] + err
             L.azb_sample_moves.argtypes = [i, C.POINTER(SampleArgs), V] + err

@@ -15,7 +15,7 @@ raise ValueError, failures of the device azb200.CudaError.
 """
 from __future__ import annotations
 
-import ctypes as C
+import functools
 
 import torch
 
@@ -105,6 +105,11 @@ def _sizes(rows: int, cols: int) -> tuple[int, int]:
     return rows * blocks * 16, -(-rows // 128) * -(-blocks // 4) * 512
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace(m: int, n: int, k: int) -> int:
+    return azb200.lib().azb_mx4_linear_workspace(m, n, k)
+
+
 def mx4_quantise(x: torch.Tensor) -> Mx4:
     """The 4-bit microscaled form of a matrix."""
     code, rows, cols, ld = _matrix(x, "x")
@@ -166,11 +171,12 @@ def mx4_product(x, w: Mx4, *, bias: torch.Tensor | None = None, relu: bool = Fal
         rc = L.azb_mx4_product(device.index, *x.pointers(), m, *w.pointers(), n, k, b, relu, out.data_ptr(), code, n,
                                _stream(device.index), e, 1024)
     else:
-        nc, ns = _sizes(m, k)
-        need = -(-nc // 256) * 256 + ns   # azb_mx4_linear_workspace
-        ws = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=device)
+        need, ws = _workspace(m, n, k), None
+        if need:
+            ws = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=device)
         rc = L.azb_mx4_linear(device.index, x.data_ptr(), x_type, m, k, x_ld, *w.pointers(), n, b, relu,
-                              out.data_ptr(), code, n, ws.data_ptr(), need, _stream(device.index), e, 1024)
+                              out.data_ptr(), code, n, ws.data_ptr() if ws is not None else None, need,
+                              _stream(device.index), e, 1024)
     if rc != 0:
         _fail("azb_mx4_product", e)
     return out[0] if vector else out

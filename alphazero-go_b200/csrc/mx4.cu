@@ -12,6 +12,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "ops.hpp"
 #include "sm100.cuh"
@@ -281,6 +282,9 @@ struct ProductTile {
     void* out;
     long long ld;
     int early_w;           // w and its scales may be read before the previous launch ends
+    const void* x;         // plain x, where the kernel quantises it itself, and its rows
+    long long x_ld;
+    int k, x_bytes;        // x_bytes: the widest load that its rows' alignment allows
 };
 
 constexpr int kPTile = 128, kPChunkBytes = 128, kPThreads = 192, kPMaxStages = 8, kPMaxSplits = 8;
@@ -345,10 +349,40 @@ __device__ __forceinline__ void store_out(const ProductTile& p, int row, int col
     static_cast<T*>(p.out)[size_t(row) * size_t(p.ld) + size_t(col)] = T(v);
 }
 
-// kGroups: scale tiles of 128 rows of x (tn <= 128: 1, else 2).
-template <typename T, int kGroups>
-__global__ void __launch_bounds__(kPThreads, 1)
+// A block of 32 elements of plain x.
+template <typename X>
+struct PlainBlock {
+    Run<X, 16> a, b;
+    __device__ __forceinline__ void load(const X* row, long long c, long long cols, int bytes) {
+        if (bytes == 16) load_as<16>(row, c, cols);
+        else load_as<int(sizeof(X))>(row, c, cols);
+    }
+    template <int kBytes>
+    __device__ __forceinline__ void load_as(const X* row, long long c, long long cols) {
+        a.template load<kBytes>(row, c, cols);
+        b.template load<kBytes>(row, c + 16, cols);
+    }
+    __device__ __forceinline__ uint4 codes(uint32_t* code) const {
+        *code = scale_code(max(a.top_field(), b.top_field()));
+        return make_uint4(a.codes(0, *code), a.codes(1, *code), b.codes(0, *code), b.codes(1, *code));
+    }
+};
+
+constexpr int kPEpiThreads = kPThreads - 64;
+// Up to so many rows, and chunks of K a CTA, a plain x is quantised by the
+// product's CTAs: 1 x 4096 x 4096 6.7 us so and 8.1 us with a launch before it
+// (16 rows: 8.4 and 8.8), and the launch's host time is saved. With 32 rows
+// 9.9 and 9.0, with 64 14.0 and 10.8.
+constexpr int kPPlainRows = 16, kPPlainChunks = 8;
+
+// kGroups: scale tiles of 128 rows of x (tn <= 128: 1, else 2). X: void, or
+// the type of plain x, which the epilogue's warps then quantise into the
+// stages themselves while w is on its way (every CTA its part of K; for few
+// rows that costs less than a launch of its own).
+template <typename T, int kGroups, typename X>
+__global__ void __launch_bounds__(kPThreads)
     mx4_product_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap mx, const ProductTile p) {
+    constexpr bool kPlain = !std::is_void_v<X>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     __shared__ __align__(8) uint64_t full[kPMaxStages], empty[kPMaxStages], done;
@@ -360,19 +394,42 @@ __global__ void __launch_bounds__(kPThreads, 1)
     // This CTA's chunks of K: an even share, in order.
     const int c_begin = int((long long)p.chunks * split / p.splits);
     const int c_end = int((long long)p.chunks * (split + 1) / p.splits);
+    const int ahead = min(p.stages, c_end - c_begin);
     const uint32_t stage = stage_bytes(p.tn), x_bytes = uint32_t(p.tn) * kPChunkBytes;
     const int x_tile = x0 >> 7, x_tiles = (p.m + 127) >> 7;
     const uint32_t scale_col0 = uint32_t(max(p.tn, 32));
 
-    if (warp == 0 && lane == 0) {
-        tma_prefetch_map(&mw);
-        tma_prefetch_map(&mx);
+    const auto scale_bytes = [&](int c) { return uint32_t(min(2, p.scale_tiles - 2 * c)) * 512u; };
+    const auto x_groups = [&] { return min(kGroups, x_tiles - x_tile); };
+    const auto load_w = [&](int c, int s) {   // arms the barrier for all of the stage's copies
+        uint8_t* b = base + size_t(s) * stage;
+        const uint32_t sb = scale_bytes(c);
+        mbar_arrive_expect_tx(&full[s], kPWBytes + sb + (kPlain ? 0u : x_bytes + sb * uint32_t(x_groups())));
+        tma_load_2d(&mw, b, &full[s], c * kPChunkBytes, n0);
+        bulk_load(b + kPWBytes + x_bytes, p.w_scales + (size_t(n0 >> 7) * p.scale_tiles + 2 * c) * 512, sb, &full[s]);
+    };
+    const auto load_x = [&](int c, int s) {
+        if constexpr (!kPlain) {
+            uint8_t* b = base + size_t(s) * stage;
+            tma_load_2d(&mx, b + kPWBytes, &full[s], c * kPChunkBytes, x0);
+            for (int g = 0; g < x_groups(); ++g)
+                bulk_load(b + kPWBytes + x_bytes + 1024 + 1024 * g,
+                          p.x_scales + (size_t(x_tile + g) * p.scale_tiles + 2 * c) * 512, scale_bytes(c), &full[s]);
+        }
+    };
+
+    // The first stages' copies are under way before the block meets.
+    if (warp == 0 && elect_one()) {
         for (int i = 0; i < p.stages; ++i) {
-            mbar_init(&full[i], 1);
+            mbar_init(&full[i], kPlain ? 1 + kPEpiThreads : 1);
             mbar_init(&empty[i], 1);
         }
         mbar_init(&done, 1);
         fence_barrier_init();
+        if (!p.early_w) grid_dependency_wait();
+        for (int i = 0; i < ahead; ++i) load_w(c_begin + i, i);
+        if (p.early_w) grid_dependency_wait();
+        for (int i = 0; i < ahead; ++i) load_x(c_begin + i, i);
     }
     if (warp == 1) tmem_alloc(&tmem_slot, p.tmem_cols);
     tc_fence_before();
@@ -381,27 +438,6 @@ __global__ void __launch_bounds__(kPThreads, 1)
     const uint32_t tmem = tmem_slot;
 
     if (warp == 0 && elect_one()) {
-        auto scale_bytes = [&](int c) { return min(2, p.scale_tiles - 2 * c) * 512; };
-        auto x_groups = [&] { return min(kGroups, x_tiles - x_tile); };
-        auto load_w = [&](int c, int s) {   // arms the barrier for the whole stage
-            uint8_t* b = base + size_t(s) * stage;
-            const uint32_t sb = uint32_t(scale_bytes(c));
-            mbar_arrive_expect_tx(&full[s], kPWBytes + x_bytes + sb * (1u + uint32_t(x_groups())));
-            tma_load_2d(&mw, b, &full[s], c * kPChunkBytes, n0);
-            bulk_load(b + kPWBytes + x_bytes, p.w_scales + (size_t(n0 >> 7) * p.scale_tiles + 2 * c) * 512, sb, &full[s]);
-        };
-        auto load_x = [&](int c, int s) {
-            uint8_t* b = base + size_t(s) * stage;
-            tma_load_2d(&mx, b + kPWBytes, &full[s], c * kPChunkBytes, x0);
-            for (int g = 0; g < x_groups(); ++g)
-                bulk_load(b + kPWBytes + x_bytes + 1024 + 1024 * g,
-                          p.x_scales + (size_t(x_tile + g) * p.scale_tiles + 2 * c) * 512, uint32_t(scale_bytes(c)), &full[s]);
-        };
-        const int ahead = min(p.stages, c_end - c_begin);
-        if (!p.early_w) grid_dependency_wait();
-        for (int i = 0; i < ahead; ++i) load_w(c_begin + i, i);
-        if (p.early_w) grid_dependency_wait();
-        for (int i = 0; i < ahead; ++i) load_x(c_begin + i, i);
         Ring r;
         int loaded = ahead;
         for (int c = c_begin + ahead; c < c_end; ++c) {
@@ -461,6 +497,35 @@ __global__ void __launch_bounds__(kPThreads, 1)
     const float bias = p.bias && j < p.n ? p.bias[j] : 0.0f;
     const int live = min(p.tn, p.m - x0);         // the tile's rows of x
     float* part = reinterpret_cast<float*>(base);
+    if constexpr (kPlain) {
+        if (warp >= 2) {
+            const int t = int(threadIdx.x) - 64;
+            // Block b of row r of chunk c into stage s, as TMA and the scales'
+            // copies lay them out. (x is one tile of at most 16 rows; rows past
+            // m stay as they are: they reach no column that is stored.)
+            const auto put = [&](int c, int s, int r, int b) {
+                PlainBlock<X> v;
+                v.load(static_cast<const X*>(p.x) + size_t(r) * size_t(p.x_ld), (long long)c * 256 + b * 32, p.k, p.x_bytes);
+                uint32_t code;
+                const uint4 q = v.codes(&code);
+                uint8_t* to = base + size_t(s) * stage + kPWBytes;
+                *reinterpret_cast<uint4*>(to + r * kPChunkBytes + ((b ^ (r & 7)) << 4)) = q;
+                to[x_bytes + 1024 + (b >> 2) * 512 + r * 16 + (b & 3)] = uint8_t(code);
+            };
+            const int each = live * 8;
+            for (int i = t; i < ahead * each; i += kPEpiThreads) put(c_begin + i / each, i / each, (i % each) >> 3, i & 7);
+            fence_proxy_async_smem();
+            for (int i = 0; i < ahead; ++i) mbar_arrive(&full[i]);
+            Ring r;
+            for (int c = c_begin + ahead; c < c_end; ++c) {
+                if (!mbar_wait(&empty[r.idx], r.phase, &g_mx4_error, kErrWaitProducer)) break;
+                for (int i = t; i < each; i += kPEpiThreads) put(c, int(r.idx), i >> 3, i & 7);
+                fence_proxy_async_smem();
+                mbar_arrive(&full[r.idx]);
+                r.next(uint32_t(p.stages));
+            }
+        }
+    }
     if (warp >= 2) {
         mbar_wait(&done, 0, &g_mx4_error, kErrWaitEpilogue);
         tc_fence_after();
@@ -809,11 +874,11 @@ bool out_aligned(const MxProductArgs& a) {
     return reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && size_t(a.ld) * elem_size(a.type) % 16 == 0;
 }
 
-template <typename T, int kGroups>
+template <typename T, int kGroups, typename X>
 cudaError_t launch_product_t(const CUtensorMap& mw, const CUtensorMap& mx, const ProductTile& p, dim3 grid, bool pdl,
                              cudaStream_t s) {
     const size_t smem = 1024 + size_t(p.stages) * stage_bytes(p.tn);
-    if (const cudaError_t e = open_smem<mx4_product_kernel<T, kGroups>>(smem); e != cudaSuccess) return e;
+    if (const cudaError_t e = open_smem<mx4_product_kernel<T, kGroups, X>>(smem); e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(kPThreads);
@@ -833,7 +898,7 @@ cudaError_t launch_product_t(const CUtensorMap& mw, const CUtensorMap& mx, const
     }
     cfg.attrs = attr;
     cfg.numAttrs = unsigned(na);
-    return cudaLaunchKernelEx(&cfg, mx4_product_kernel<T, kGroups>, mw, mx, p);
+    return cudaLaunchKernelEx(&cfg, mx4_product_kernel<T, kGroups, X>, mw, mx, p);
 }
 
 }  // namespace
@@ -870,8 +935,55 @@ cudaError_t launch_mx4_values(const MxCastArgs& a, int sms, cudaStream_t s) {
     return cudaGetLastError();
 }
 
+namespace {
+
+// How a product is cut up.
+struct ProductPlan {
+    bool pairs;            // 256 x 256 tiles by CTA pairs
+    int tn, n_tiles, x_tiles, splits, per_cta, stages;
+    bool quantises;        // a plain x is quantised by the product's own CTAs
+};
+
+ProductPlan plan_of(long long m, long long n, long long k) {
+    constexpr int kSms = 148;
+    ProductPlan p{};
+    if (m > 128 && n > 128 && (m + 255) / 256 * ((n + 255) / 256) >= kPairFromTiles) {
+        p.pairs = true;
+        return p;
+    }
+    const int chunks = int((k + 255) / 256);
+    // Columns per tile: as few as hold all of x up to 128; more rows of x in
+    // tiles of 256 where those alone fill the SMs, else 128, else 64.
+    p.n_tiles = int((n + kPTile - 1) / kPTile);
+    if (m <= 128) p.tn = int((m + 15) / 16 * 16);
+    else p.tn = 64;
+    for (const int tn : {128, 256})
+        if (m > 128 && (m + tn - 1) / tn * p.n_tiles >= kSms) p.tn = tn;
+    p.x_tiles = int((m + p.tn - 1) / p.tn);
+    // Up to 64 columns two CTAs share an SM (four stages each), so that one's
+    // issue and waits fill the other's; K is shared by a cluster of CTAs while
+    // there are slots for them and every CTA keeps a chunk or more.
+    const int slots = p.tn <= 64 ? 2 * kSms : kSms;
+    p.splits = 1;
+    while (p.splits < kPMaxSplits && (long long)p.n_tiles * p.x_tiles * p.splits * 2 <= slots && p.splits * 2 <= chunks)
+        p.splits *= 2;
+    p.per_cta = (chunks + p.splits - 1) / p.splits;
+    const size_t budget = p.tn <= 64 ? size_t(108) << 10 : size_t(220) << 10;
+    p.stages = int(std::min<size_t>(kPMaxStages, budget / stage_bytes(p.tn)));
+    p.stages = std::max(1, std::min(p.stages, p.per_cta));
+    // The parts of a shared K reuse the stages' memory: 512 bytes a column.
+    while (p.splits > 1 && size_t(p.stages) * stage_bytes(p.tn) < size_t(p.tn) * kPTile * 4) ++p.stages;
+    p.quantises = m <= kPPlainRows && p.per_cta <= kPPlainChunks;
+    return p;
+}
+
+}  // namespace
+
+bool mx4_product_quantises(long long m, long long n, long long k) { return plan_of(m, n, k).quantises; }
+
 cudaError_t launch_mx4_product(const MxProductArgs& a, int sms, cudaStream_t s) {
-    if (a.m > 128 && a.n > 128 && (a.m + 255) / 256 * ((a.n + 255) / 256) >= kPairFromTiles) {
+    const ProductPlan plan = plan_of(a.m, a.n, a.k);
+    if (plan.pairs) {
         if (a.type == kElemBF16) return out_aligned(a) ? launch_pair<__nv_bfloat16, true>(a, sms, s) : launch_pair<__nv_bfloat16, false>(a, sms, s);
         return out_aligned(a) ? launch_pair<float, true>(a, sms, s) : launch_pair<float, false>(a, sms, s);
     }
@@ -882,24 +994,9 @@ cudaError_t launch_mx4_product(const MxProductArgs& a, int sms, cudaStream_t s) 
     p.chunks = int((a.k + 255) / 256);
     p.steps = int((a.k + 63) / 64);
     p.scale_tiles = int(xs.scale_tiles());
-    // Columns per tile: as few as hold all of x up to 128; more rows of x in
-    // tiles of 256 where those alone fill the SMs, else 128, else 64.
-    const int n_tiles = int((a.n + kPTile - 1) / kPTile);
-    if (a.m <= 128) p.tn = int((a.m + 15) / 16 * 16);
-    else p.tn = 64;
-    for (const int tn : {128, 256})
-        if (a.m > 128 && (a.m + tn - 1) / tn * n_tiles >= sms) p.tn = tn;
-    const int x_tiles = int((a.m + p.tn - 1) / p.tn);
-    // K is shared by a cluster of CTAs while the tiles leave SMs idle and
-    // every CTA keeps a chunk or more.
-    p.splits = 1;
-    while (p.splits < kPMaxSplits && (long long)n_tiles * x_tiles * p.splits * 2 <= sms && p.splits * 2 <= p.chunks)
-        p.splits *= 2;
-    const int per_cta = (p.chunks + p.splits - 1) / p.splits;
-    p.stages = int(std::min<size_t>(kPMaxStages, (size_t(220) << 10) / stage_bytes(p.tn)));
-    p.stages = std::max(1, std::min(p.stages, per_cta));
-    // The parts of a shared K reuse the stages' memory: 512 bytes a column.
-    while (p.splits > 1 && size_t(p.stages) * stage_bytes(p.tn) < size_t(p.tn) * kPTile * 4) ++p.stages;
+    p.tn = plan.tn;
+    p.stages = plan.stages;
+    p.splits = plan.splits;
     const uint32_t cols = uint32_t(std::max(p.tn, 32)) + uint32_t(p.stages) * stage_scale_cols(p.tn);
     p.tmem_cols = 32;
     while (p.tmem_cols < cols) p.tmem_cols *= 2;
@@ -910,12 +1007,21 @@ cudaError_t launch_mx4_product(const MxProductArgs& a, int sms, cudaStream_t s) 
     p.out = a.out;
     p.ld = a.ld;
     p.early_w = a.after_quantise ? 1 : 0;
+    p.x = a.x;
+    p.x_ld = a.x_ld;
+    p.k = int(a.k);
+    p.x_bytes = a.x ? row_bytes(a.x, a.m, a.x_ld, a.x_type) : 0;
     const CUtensorMap mw = make_byte_map(a.w_codes, uint64_t(ws.pitch()), uint64_t(a.n), kPTile);
-    const CUtensorMap mx = make_byte_map(a.x_codes, uint64_t(xs.pitch()), uint64_t(a.m), uint32_t(p.tn));
-    const dim3 grid(unsigned(n_tiles * p.splits), unsigned(x_tiles));
-    const auto go = a.type == kElemBF16 ? (p.tn > 128 ? launch_product_t<__nv_bfloat16, 2> : launch_product_t<__nv_bfloat16, 1>)
-                                        : (p.tn > 128 ? launch_product_t<float, 2> : launch_product_t<float, 1>);
-    return go(mw, mx, p, grid, a.after_quantise, s);
+    const CUtensorMap mx = a.x ? mw : make_byte_map(a.x_codes, uint64_t(xs.pitch()), uint64_t(a.m), uint32_t(p.tn));
+    const dim3 grid(unsigned(plan.n_tiles * p.splits), unsigned(plan.x_tiles));
+    const auto launch = [&](auto out) {
+        using T = decltype(out);
+        if (a.x) return a.x_type == kElemBF16 ? launch_product_t<T, 1, __nv_bfloat16>(mw, mx, p, grid, false, s)
+                                              : launch_product_t<T, 1, float>(mw, mx, p, grid, false, s);
+        return p.tn > 128 ? launch_product_t<T, 2, void>(mw, mx, p, grid, a.after_quantise, s)
+                          : launch_product_t<T, 1, void>(mw, mx, p, grid, a.after_quantise, s);
+    };
+    return a.type == kElemBF16 ? launch(__nv_bfloat16()) : launch(0.0f);
 }
 
 cudaError_t mx4_take_error(int* code) {

@@ -58,7 +58,14 @@ struct MxProductArgs {
     int type;            // ElemType of `out`
     long long ld;        // elements from one row of `out` to the next
     bool after_quantise;
+    // Plain x in place of its codes and scales (then null), where
+    // mx4_product_quantises(m, n, k).
+    const void* x = nullptr;
+    int x_type = 0;
+    long long x_ld = 0;
 };
+// Whether the product quantises a plain x itself.
+bool mx4_product_quantises(long long m, long long n, long long k);
 cudaError_t launch_mx4_product(const MxProductArgs& a, int sms, cudaStream_t s);
 // The product kernels' error word on the current device (KernelError; 0:
 // none), read and cleared after waiting for the device.

@@ -149,8 +149,8 @@ int azb_mx4_product(int device, const void* x_codes, const void* x_scales, long 
     });
 }
 
-size_t azb_mx4_linear_workspace(long long m, long long k) {
-    if (m < 0 || m > kMaxRows || k < 1 || k > kMaxCols) return 0;
+size_t azb_mx4_linear_workspace(long long m, long long n, long long k) {
+    if (m < 1 || m > kMaxRows || n < 1 || n > kMaxRows || k < 1 || k > kMaxCols || mx4_product_quantises(m, n, k)) return 0;
     const MxShape s{m, k};
     return round_256(s.code_bytes()) + s.scale_bytes();
 }
@@ -171,7 +171,14 @@ int azb_mx4_linear(int device, const void* x, int x_type, long long m, long long
         check_aligned(x, elem_size(x_type), "x", fn);
         check_aligned(out, elem_size(type), "out", fn);
         check_mx(w_codes, w_scales, "w", fn);
-        const size_t need = azb_mx4_linear_workspace(m, k);
+        if (mx4_product_quantises(m, n, k)) {
+            const OnDevice on(device);
+            const MxProductArgs a{nullptr, nullptr, static_cast<const uint8_t*>(w_codes), static_cast<const uint8_t*>(w_scales),
+                                  m, n, k, bias, relu != 0, out, type, ld, false, x, x_type, x_ld};
+            check(launch_mx4_product(a, on.sms(), stream_of(stream)), fn);
+            return;
+        }
+        const size_t need = azb_mx4_linear_workspace(m, n, k);
         require(workspace && workspace_bytes >= need,
                 std::string(fn) + ": the workspace holds " + std::to_string(workspace_bytes) + " bytes of " + std::to_string(need));
         check_aligned(workspace, 256, "the workspace", fn);

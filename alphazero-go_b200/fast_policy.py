@@ -96,7 +96,7 @@ def main() -> None:
     azb_ops.check(0)
     print(f"fast policy: {policy.nbytes() / 1024:.0f} KiB, correlation with the teacher's logits {corr:.3f} on "
           f"held-out positions, {start.elapsed_time(end) * 10:.1f} us for 1024 positions (planes to moves), "
-          f"mean logprob {logprob.mean():.2f}, all legal {bool(legal.gather(1, moves[:, None]).all())}")
+          f"mean logprob {logprob.mean():.2f}, all legal {bool(legal.gather(1, moves.clamp(min=0)[:, None]).all())}")
 
 
 if __name__ == "__main__":

@@ -296,10 +296,11 @@ int azb_mx4_values(int device, const void* codes, const void* scales, long long 
 int azb_mx4_product(int device, const void* x_codes, const void* x_scales, long long m, const void* w_codes,
                     const void* w_scales, long long n, long long k, const float* bias, int relu, void* out, int type,
                     long long ld, void* stream, char* err, size_t err_cap);
-/* The product with x given as plain elements, quantised on the way into the
- * workspace (azb_mx4_linear_workspace bytes, 256-byte aligned; 0 for sizes
- * out of range). */
-size_t azb_mx4_linear_workspace(long long m, long long k);
+/* The product with x given as plain elements, quantised on the way: by the
+ * product itself where its tiles are few, else into the workspace, of
+ * azb_mx4_linear_workspace bytes and 256-byte aligned (0 bytes, and null will
+ * do, where it needs none and for sizes out of range). */
+size_t azb_mx4_linear_workspace(long long m, long long n, long long k);
 int azb_mx4_linear(int device, const void* x, int x_type, long long m, long long k, long long x_ld, const void* w_codes,
                    const void* w_scales, long long n, const float* bias, int relu, void* out, int type, long long ld,
                    void* workspace, size_t workspace_bytes, void* stream, char* err, size_t err_cap);

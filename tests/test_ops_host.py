@@ -10,6 +10,13 @@ import azb200 as E
 P = 1 << 20   # an aligned address
 
 
+def test_workspace():
+    w = E.lib().azb_mx4_linear_workspace
+    assert w(1, 4096, 4096) == 0 and w(2000, 3000, 8) == 2000 * 16 + 16 * 512
+    assert w(8192, 8192, 8192) == 8192 * 4096 + 64 * 64 * 512
+    assert w(2000, 0, 8) == w(2000, 3000, 0) == w(2000, (1 << 22) + 1, 8) == 0
+
+
 def call(fn, *args):
     e = C.create_string_buffer(1024)
     rc = getattr(E.lib(), fn)(*args, e, 1024)
@@ -33,7 +40,7 @@ def test_sizes(rows, cols, codes, scales):
 @pytest.mark.parametrize("rows,cols", [(-1, 4), (4, 0), (4, -3), ((1 << 22) + 1, 4), (4, (1 << 26) + 1)])
 def test_sizes_refused(rows, cols):
     assert "azb_mx4_sizes: a matrix of" in sizes(rows, cols)
-    assert E.lib().azb_mx4_linear_workspace(rows, cols) == 0
+    assert E.lib().azb_mx4_linear_workspace(rows, 4, cols) == 0
 
 
 def quantise(x=P, type=0, rows=2, cols=8, ld=8, codes=P, scales=P):
@@ -44,8 +51,8 @@ def product(xc=P, xs=P, m=2, wc=P, ws=P, n=3, k=8, bias=None, out=P, type=0, ld=
     return call("azb_mx4_product", 0, xc, xs, m, wc, ws, n, k, bias, 0, out, type, ld, None)
 
 
-def linear(x=P, xt=0, m=2, k=8, xld=8, wc=P, ws=P, n=3, out=P, type=0, ld=3, work=P, bytes=None):
-    need = E.lib().azb_mx4_linear_workspace(m, k) if bytes is None else bytes
+def linear(x=P, xt=0, m=2000, k=8, xld=8, wc=P, ws=P, n=3000, out=P, type=0, ld=3000, work=P, bytes=None):
+    need = E.lib().azb_mx4_linear_workspace(m, n, k) if bytes is None else bytes
     return call("azb_mx4_linear", 0, x, xt, m, k, xld, wc, ws, n, None, 0, out, type, ld, work, need, None)
 
 
