@@ -144,7 +144,7 @@ def lib() -> C.CDLL:
             L.azb_mx4_linear_workspace.argtypes = [ll, ll, ll]
             L.azb_mx4_linear_workspace.restype = s
             L.azb_mx4_linear.argtypes = [i, V, i, ll, ll, ll, V, V, ll, V, i, V, i, ll, V, s, V] + err
-            L.azb_sample_moves.argtypes = [i, C.POINTER(SampleArgs), V] + err
+            L.azb_sample_moves.argtypes = [i, V, V] + err   # (a SampleArgs by reference, or its bytes)
             L.azb_ops_check.argtypes = [i] + err
             L.azb_workspace_bytes.argtypes = [D, C.c_int, C.c_int]
             L.azb_workspace_bytes.restype = s

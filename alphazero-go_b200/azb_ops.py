@@ -16,12 +16,15 @@ raise ValueError, failures of the device azb200.CudaError.
 from __future__ import annotations
 
 import functools
+import struct
 
 import torch
 
 import azb200
-from azb200 import CudaError, SampleArgs
+from azb200 import CudaError
 
+# azb_sample_args (azb200.SampleArgs), packed in one step.
+_SAMPLE_ARGS = struct.Struct("@PiqqqPqPqfffiPPPPPP")
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 
@@ -114,14 +117,16 @@ def mx4_quantise(x: torch.Tensor) -> Mx4:
     """The 4-bit microscaled form of a matrix."""
     code, rows, cols, ld = _matrix(x, "x")
     device = x.device
+    index, e = device.index, azb200._err()
+    blocks = -(-cols // 32)
+    nc = rows * blocks * 16
+    at = -(-nc // 256) * 256   # the scales' place
     q = object.__new__(Mx4)
-    nc, ns = _sizes(rows, cols)
-    q._split, q._scales = nc, None
-    q._data = torch.empty_strided((-(-nc // 256) * 256 + ns,), (1,), dtype=torch.uint8, device=device)
-    q.rows, q.cols, q.device = rows, cols, device
-    e = azb200._err()
-    if azb200.lib().azb_mx4_quantise(device.index, x.data_ptr(), code, rows, cols, ld, *q.pointers(),
-                                     _stream(device.index), e, 1024) != 0:
+    q.rows, q.cols, q.device, q._split, q._scales = rows, cols, device, nc, None
+    q._data = data = torch.empty_strided((at + -(-rows // 128) * -(-blocks // 4) * 512,), (1,), dtype=torch.uint8,
+                                         device=device)
+    p = data.data_ptr()
+    if azb200.lib().azb_mx4_quantise(index, x.data_ptr(), code, rows, cols, ld, p, p + at, _stream(index), e, 1024) != 0:
         _fail("azb_mx4_quantise", e)
     return q
 
@@ -185,7 +190,7 @@ def mx4_product(x, w: Mx4, *, bias: torch.Tensor | None = None, relu: bool = Fal
 def _per_row(v, name: str, rows: int, device, dtype):
     """(number, pointer) of a setting: one number, or one per row."""
     if not isinstance(v, torch.Tensor):
-        return v, None
+        return v, 0
     if v.dtype != dtype or v.shape != (rows,) or v.device != device or not v.is_contiguous():
         raise ValueError(f"{name}: a number, or {rows} adjacent {dtype} numbers on {device}")
     return 0, v.data_ptr()
@@ -202,28 +207,29 @@ def sample_moves(logits: torch.Tensor, noise: torch.Tensor | None, *, legal: tor
     nothing legal gives -1 and -inf. azb_sample_moves states the arithmetic."""
     code, rows, cols, ld = _matrix(logits, "logits")
     device = logits.device
-    a = SampleArgs()
-    a.logits, a.type, a.rows, a.cols, a.ld = logits.data_ptr(), code, rows, cols, ld
+    n_at = n_ld = l_at = l_ld = 0
     if noise is not None:
-        if noise.dtype != torch.float32 or noise.shape != logits.shape or (cols > 1 and noise.stride(1) != 1):
-            raise ValueError("noise: float32 of logits' shape, columns adjacent")
-        a.noise, a.noise_ld = noise.data_ptr(), noise.stride(0)
+        if noise.dtype != torch.float32 or noise.shape != logits.shape:
+            raise ValueError("noise: float32 of logits' shape is needed")
+        n_at, (n_ld, inner) = noise.data_ptr(), noise.stride()
+        if (inner != 1 and cols > 1) or noise.device != device:
+            raise ValueError(f"noise: adjacent columns on {device} are needed (stride {inner}; it is on {noise.device})")
     if legal is not None:
-        if legal.dtype not in (torch.bool, torch.uint8) or legal.shape != logits.shape or (cols > 1 and legal.stride(1) != 1):
-            raise ValueError("legal: bool or uint8 of logits' shape, columns adjacent")
-        a.legal, a.legal_ld = legal.data_ptr(), legal.stride(0)
-    for name, t in (("noise", noise), ("legal", legal)):
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, not on {device}")
-    a.temperature, a.temperature_rows = _per_row(temperature, "temperature", rows, device, torch.float32)
-    a.top_k, a.top_k_rows = _per_row(top_k, "top_k", rows, device, torch.int32)
-    a.top_p, a.top_p_rows = _per_row(top_p, "top_p", rows, device, torch.float32)
-    a.min_p, a.min_p_rows = _per_row(min_p, "min_p", rows, device, torch.float32)
+        if legal.dtype not in (torch.bool, torch.uint8) or legal.shape != logits.shape:
+            raise ValueError("legal: bool or uint8 of logits' shape is needed")
+        l_at, (l_ld, inner) = legal.data_ptr(), legal.stride()
+        if (inner != 1 and cols > 1) or legal.device != device:
+            raise ValueError(f"legal: adjacent columns on {device} are needed (stride {inner}; it is on {legal.device})")
+    temperature, t_at = _per_row(temperature, "temperature", rows, device, torch.float32)
+    top_k, k_at = _per_row(top_k, "top_k", rows, device, torch.int32)
+    top_p, p_at = _per_row(top_p, "top_p", rows, device, torch.float32)
+    min_p, m_at = _per_row(min_p, "min_p", rows, device, torch.float32)
     moves = torch.empty_strided((rows,), (1,), dtype=torch.int64, device=device)
     logprob = torch.empty_strided((rows,), (1,), dtype=torch.float32, device=device)
-    a.moves, a.logprob = moves.data_ptr(), logprob.data_ptr()
-    e = azb200._err()
-    if azb200.lib().azb_sample_moves(device.index, a, _stream(device.index), e, 1024) != 0:
+    args = _SAMPLE_ARGS.pack(logits.data_ptr(), code, rows, cols, ld, n_at, n_ld, l_at, l_ld, temperature, top_p, min_p,
+                             top_k, t_at, p_at, m_at, k_at, moves.data_ptr(), logprob.data_ptr())
+    index, e = device.index, azb200._err()
+    if azb200.lib().azb_sample_moves(index, args, _stream(index), e, 1024) != 0:
         _fail("azb_sample_moves", e)
     return moves, logprob
 

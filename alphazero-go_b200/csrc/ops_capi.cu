@@ -17,29 +17,25 @@ namespace {
 // `device` current for the scope.
 class OnDevice {
 public:
-    explicit OnDevice(int device) {
+    explicit OnDevice(int device) : info_(&device_info(device)) {
+        if (!info_->usable) throw std::runtime_error("cuda: " + info_->why);
         if (cudaGetDevice(&before_) != cudaSuccess) {
             cudaGetLastError();
             before_ = -1;
         }
-        try {
-            info_ = &require_device(device);
-        } catch (...) {
-            restore();
-            throw;
-        }
+        if (before_ == device) before_ = -1;   // nothing to put back
+        else check(cudaSetDevice(device), "cudaSetDevice");
     }
-    ~OnDevice() { restore(); }
+    ~OnDevice() {
+        if (before_ >= 0) cudaSetDevice(before_);
+    }
     OnDevice(const OnDevice&) = delete;
     OnDevice& operator=(const OnDevice&) = delete;
     int sms() const { return info_->sms; }
 
 private:
-    void restore() {
-        if (before_ >= 0) cudaSetDevice(before_);
-    }
+    const DeviceInfo* info_;
     int before_ = -1;
-    const DeviceInfo* info_ = nullptr;
 };
 
 void require(bool ok, const std::string& what) {

@@ -300,7 +300,7 @@ def test_refusals_and_empty(ops, torch):
         (lambda: ops.sample_moves(l, n.double()), "noise: float32"),
         (lambda: ops.sample_moves(l, n[:, :39]), "noise: float32"),
         (lambda: ops.sample_moves(l, None), "null noise"),
-        (lambda: ops.sample_moves(l, n.cpu()), "noise is on cpu"),
+        (lambda: ops.sample_moves(l, n.cpu()), "it is on cpu"),
         (lambda: ops.sample_moves(l, n, legal=torch.ones(3, 40, device="cuda")), "legal: bool or uint8"),
         (lambda: ops.sample_moves(l, n, temperature=-1.0), "temperature"),
         (lambda: ops.sample_moves(l, n, top_p=1.2), "top_p"),
