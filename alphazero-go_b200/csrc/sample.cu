@@ -19,6 +19,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "ops.hpp"
 #include "sm100.cuh"
@@ -343,8 +344,9 @@ __global__ void __launch_bounds__(128) sample_warp_kernel(const SampleArgs a) {
 // keys is halved as in find_threshold.
 //
 // Lower bounds keep most logits out of the histogram: with k <= the number of
-// warps (threads) that hold a logit, the k-th largest is at least the least
-// of their maxima; and logits with w < (1 - p) Z / cols have together less
+// groups of threads that hold a logit, the k-th largest is at least the least
+// of the groups' maxima (groups of 1, 2, .. 32 threads: the largest that are
+// still enough); and logits with w < (1 - p) Z / cols have together less
 // than (1 - p) Z, so the prefix that top-p keeps ends above them.
 
 constexpr int kMaxCluster = 8, kMaxRowWarps = 8;
@@ -356,17 +358,26 @@ constexpr float kNoChance = -19.6f;
 // Descending order of logits, ties by ascending column, as descending numbers.
 __device__ __forceinline__ uint64_t place_of(uint32_t key, int i) { return uint64_t(key) << 32 | uint32_t(~uint32_t(i)); }
 
+constexpr int kGroupSizes = 6;   // groups of 2^0 .. 2^5 threads
 struct Part {   // what one CTA knows of its slice
-    float top;             // largest logit
-    float z;               // sum of w relative to `top`
-    float warp_low;        // least of its warps' largest logits
-    float thread_low;      // least of its threads'
-    int valid, warps, threads;   // logits above -inf, warps and threads that hold one
+    float top;                // largest logit
+    float z;                  // sum of w relative to `top`
+    int valid;                // logits above -inf
+    float low[kGroupSizes];   // least of its groups' largest logits
+    int groups[kGroupSizes];  // groups that hold a logit
 };
 
-struct RowShared {
+struct __align__(16) RowShared {
     uint32_t hist_n[kBins], hist_w[kBins];            // this CTA's; then the lists
-    uint32_t share_n[kBins / 2], share_w[kBins / 2];  // a cluster's CTA: its share of the bins, added over the cluster
+    union {
+        struct {   // a cluster's CTA: its share of the bins, added over the cluster
+            uint32_t share_n[kBins / 2], share_w[kBins / 2];
+        };
+        struct {   // before that: of each warp's groups
+            float low[kGroupSizes][kMaxRowWarps];
+            int groups[kGroupSizes][kMaxRowWarps];
+        };
+    };
     uint16_t upper[kUpper];                           // the slice's upper columns, a part for each warp
     Part part[kMaxCluster];
     float f[2][kMaxCluster];
@@ -737,14 +748,20 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
     // The slice's largest logit, and the sum of w relative to it.
     float mine = neg_inf();
     sl.load([&](float l) { mine = fmaxf(mine, l); });
-    const float of_warp = warp_max(mine);
-    {
-        const bool some = mine > neg_inf();
-        float low = some ? -mine : neg_inf();
-        low = warp_max(low);
-        const int threads = __popc(__ballot_sync(0xFFFFFFFFu, some));
-        if (lane == 0) sh.wf[warp] = of_warp, sh.wg[warp] = low, sh.wn[warp] = threads;
+    float of_group = mine;
+    if (rp.first_k() > 0) {
+#pragma unroll
+        for (int g = 0; g < kGroupSizes; ++g) {
+            if (g) of_group = fmaxf(of_group, __shfl_xor_sync(0xFFFFFFFFu, of_group, 1 << (g ? g - 1 : 0)));
+            const bool some = of_group > neg_inf();
+            const uint32_t low = __reduce_min_sync(0xFFFFFFFFu, some ? key_of(of_group) : 0xFF800000u);
+            const int groups = __popc(__ballot_sync(0xFFFFFFFFu, some)) >> g;
+            if (lane == 0) sh.low[g][warp] = logit_of_key(low), sh.groups[g][warp] = groups;
+        }
+    } else {
+        of_group = warp_max(of_group);
     }
+    if (lane == 0) sh.wf[warp] = of_group;
     __syncthreads();
     float m = neg_inf();
     for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sh.wf[w]);
@@ -767,35 +784,38 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
     }
     if constexpr (!kSolo) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // every CTA runs
     __syncthreads();
-    if (warp == 0) {
-        const bool has = lane < kWarps && sh.wf[lane] > neg_inf();
-        Part p;
-        p.top = m;
-        p.z = warp_sum(lane < kWarps ? sh.wh[lane] : 0.0f);
-        p.warp_low = -warp_max(has ? -sh.wf[lane] : neg_inf());
-        p.thread_low = -warp_max(has ? sh.wg[lane] : neg_inf());
-        p.valid = int(__reduce_add_sync(0xFFFFFFFFu, lane < kWarps ? unsigned(sh.wk[lane]) : 0u));
-        p.warps = __popc(__ballot_sync(0xFFFFFFFFu, has));
-        p.threads = int(__reduce_add_sync(0xFFFFFFFFu, lane < kWarps ? unsigned(sh.wn[lane]) : 0u));
-        if (lane < ranks) {
-            const uint32_t to = crew.at(&sh.part[rank], lane);
-            const uint32_t* words = reinterpret_cast<const uint32_t*>(&p);
+    Part all;   // (every warp, from its own reads; the sums' order is fixed)
+    all.top = m;
+    all.z = warp_sum(lane < kWarps ? sh.wh[lane] : 0.0f);
+    all.valid = int(__reduce_add_sync(0xFFFFFFFFu, lane < kWarps ? unsigned(sh.wk[lane]) : 0u));
+    if (rp.first_k() > 0) {
 #pragma unroll
-            for (int i = 0; i < int(sizeof(Part) / 4); ++i) put_u(to + uint32_t(i) * 4, words[i]);
+        for (int g = 0; g < kGroupSizes; ++g) {
+            all.low[g] = logit_of_key(__reduce_min_sync(0xFFFFFFFFu, lane < kWarps ? key_of(sh.low[g][lane]) : 0xFF800000u));
+            all.groups[g] = int(__reduce_add_sync(0xFFFFFFFFu, lane < kWarps ? unsigned(sh.groups[g][lane]) : 0u));
         }
     }
-    crew.barrier();
-    Part all;
-    {   // lane r has CTA r's part; the sums' order is fixed
-        Part p{neg_inf(), 0.0f, inf, inf, 0, 0, 0};
-        if (lane < ranks) p = sh.part[lane];
+    if constexpr (!kSolo) {   // and of the cluster: lane r takes CTA r's
+        if (warp == 0 && lane < ranks) {
+            const uint32_t to = crew.at(&sh.part[rank], lane);
+            const uint32_t* words = reinterpret_cast<const uint32_t*>(&all);
+#pragma unroll
+            for (int i = 0; i < int(sizeof(Part) / 4); ++i)
+                if (i < 3 || rp.first_k() > 0) put_u(to + uint32_t(i) * 4, words[i]);
+        }
+        crew.barrier();
+        const Part& p = sh.part[lane < ranks ? lane : 0];
+        const bool in = lane < ranks;
         all.top = warp_max(p.top);
-        all.z = warp_sum(p.top == all.top ? p.z : p.z * ex2((p.top - all.top) * c));
-        all.warp_low = -warp_max(-p.warp_low);
-        all.thread_low = -warp_max(-p.thread_low);
-        all.valid = int(__reduce_add_sync(0xFFFFFFFFu, unsigned(p.valid)));
-        all.warps = int(__reduce_add_sync(0xFFFFFFFFu, unsigned(p.warps)));
-        all.threads = int(__reduce_add_sync(0xFFFFFFFFu, unsigned(p.threads)));
+        all.z = warp_sum(!in ? 0.0f : p.top == all.top ? p.z : p.z * ex2((p.top - all.top) * c));
+        all.valid = int(__reduce_add_sync(0xFFFFFFFFu, in ? unsigned(p.valid) : 0u));
+        if (rp.first_k() > 0) {
+#pragma unroll
+            for (int g = 0; g < kGroupSizes; ++g) {
+                all.low[g] = logit_of_key(__reduce_min_sync(0xFFFFFFFFu, key_of(p.low[g])));
+                all.groups[g] = int(__reduce_add_sync(0xFFFFFFFFu, in ? unsigned(p.groups[g]) : 0u));
+            }
+        }
     }
     m = all.top;
     int turn = 0;
@@ -818,7 +838,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
             sl.only_infinite();
             m = 0.0f;
             all.valid = int(all.z);
-            all.warp_low = all.thread_low = 0.0f;
+#pragma unroll
+            for (int g = 0; g < kGroupSizes; ++g) all.low[g] = 0.0f;
         }
         const float* noise = a.noise + size_t(row) * size_t(a.noise_ld) + i0;
         const int k = rp.first_k();
@@ -860,7 +881,10 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
             // first; should the cut lie below, the bound itself is taken.
             float low, sure;
             if (by_k) {
-                const float l = k <= all.warps ? all.warp_low : k <= all.threads ? all.thread_low : neg_inf();
+                float l = neg_inf();
+#pragma unroll
+                for (int g = 0; g < kGroupSizes; ++g)
+                    if (k <= all.groups[g]) l = all.low[g];
                 sure = low = fmaxf((l - m) * c, -40.0f);
             } else {
                 sure = fmaxf(__log2f((1.0f - rp.top_p) * 0.99f * all.z / float(a.cols)), -40.0f);
@@ -913,7 +937,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
             // the mass that the cut is taken from. `final`: the last filter, so
             // that what lies above its cut is raced on the way. (sh.first,
             // sh.last and sh.list_n are at their starts before it.)
-            const auto settle = [&](int count, double target, bool final, float* kept) -> bool {
+            const auto settle = [&](int count, float target, bool final, float* kept) -> bool {
 #pragma unroll
                 for (int j = 0; j < Sums<Crew>::kPer; ++j) {
                     const int b = t * Sums<Crew>::kPer + j;
@@ -922,9 +946,9 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
                     } else {
                         // A fixed-point sum is off by half a unit a logit, and by
                         // the masses' own rounding, a few 2^-22 of it.
-                        const double goal = target * double(fixed), slack = 0.5 * double(upto.n[j]) + 4096.0;
-                        if (double(upto.w[j]) + slack >= goal) atomicMin(&sh.first, b);
-                        if (double(upto.w[j]) - slack >= goal) atomicMin(&sh.last, b);
+                        const float goal = target * fixed, slack = 0.5f * float(upto.n[j]) + 4096.0f, w = float(upto.w[j]);
+                        if (w + slack >= goal) atomicMin(&sh.first, b);
+                        if (w - slack >= goal) atomicMin(&sh.last, b);
                     }
                 }
                 __syncthreads();
@@ -1005,13 +1029,15 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
                     if (t + j * kThreads < n) merged[t + j * kThreads] = place[j];
                 __syncthreads();
                 int before[kSlots] = {};
-                if (t < n)
-#pragma unroll 8
-                    for (int q = 0; q < n; ++q) {
-                        const uint64_t other = merged[q];
+                if (t < n) {
+                    const ulonglong2* two = reinterpret_cast<const ulonglong2*>(merged);
+#pragma unroll 4
+                    for (int q = 0; q < n; q += 2) {
+                        const ulonglong2 other = two[q >> 1];
 #pragma unroll
-                        for (int j = 0; j < kSlots; ++j) before[j] += other > place[j];
+                        for (int j = 0; j < kSlots; ++j) before[j] += (other.x > place[j]) + (other.y > place[j] && q + 1 < n);
                     }
+                }
                 __syncthreads();
 #pragma unroll
                 for (int j = 0; j < kSlots; ++j)
@@ -1019,8 +1045,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
                 __syncthreads();
                 // The sums run down the sorted list: the same for every CTA and
                 // run. A lane takes `each` neighbours.
-                if (warp == 0) {
-                    constexpr int kEach = kList / 32;
+                const auto cut_list = [&](auto each_most) {
+                    constexpr int kEach = decltype(each_most)::value;
                     const int each = (n + 31) / 32;
                     const int live = count > 0 ? min(n, count - s.count) : n;   // of the list, what top-k keeps
                     float w[kEach], sum = 0.0f;
@@ -1041,11 +1067,11 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
                     ahead_of_me = s.mass + (lane ? ahead_of_me : 0.0f);
                     int stay = live;
                     if (count == 0 || (whole && by_p)) {
-                        if (count > 0) target = double(rp.top_p) * double(total);
+                        const float goal = count > 0 ? rp.top_p * total : target;
                         int here = 0;
 #pragma unroll
                         for (int j = 0; j < kEach; ++j) {
-                            here += j < each && lane * each + j < live && double(ahead_of_me) < target;
+                            here += j < each && lane * each + j < live && ahead_of_me < goal;
                             ahead_of_me += w[j];
                         }
                         stay = int(__reduce_add_sync(0xFFFFFFFFu, unsigned(here)));
@@ -1054,6 +1080,10 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
                         sh.cut = stay > 0 ? merged[stay - 1] : merged[0] + 1;
                         sh.kept = total;
                     }
+                };
+                if (warp == 0) {
+                    if (n <= 64) cut_list(std::integral_constant<int, 2>());
+                    else cut_list(std::integral_constant<int, kList / 32>());
                 }
                 __syncthreads();
                 *kept = sh.kept;
@@ -1077,7 +1107,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
             for (;;) {
                 if (count_now) count_bins();
                 count_now = false;
-                settled = settle(k_stage ? k : 0, double(rp.top_p) * double(kept), !k_stage || !by_p, &kept);
+                settled = settle(k_stage ? k : 0, rp.top_p * kept, !k_stage || !by_p, &kept);
                 if (!settled) {
                     if (k_stage || !(low > sure) || sh.last < kBins) break;
                     low = sure;   // the cut lies lower than was tried
@@ -1245,10 +1275,10 @@ cudaError_t launch_sample_t(const SampleArgs& a, cudaStream_t s) {
         else sample_warp_kernel<T, 32><<<grid, 128, 0, s>>>(a);
         return cudaGetLastError();
     }
-    // Slices of at most 16384 columns (64 KB of float32: three CTAs an SM)
-    // while eight CTAs can hold the row; small rows in small CTAs, of which
-    // more run at once.
-    const int ranks = a.cols <= 16384 ? 1 : a.cols <= 32768 ? 2 : a.cols <= 65536 ? 4 : kMaxCluster;
+    // Up to 16384 columns one CTA has the row (1024 rows of 16384: 45 us, with
+    // two of 8192 each 75 us); beyond, slices of at most 8192 while eight CTAs
+    // can hold the row so (8 rows of 50001: 13 us, with 16384 19 us).
+    const int ranks = a.cols <= 16384 ? 1 : a.cols <= 32768 ? 4 : kMaxCluster;
     const int per = (a.cols + ranks - 1) / ranks;
     const size_t smem = size_t(per) * sizeof(T) + 32;   // up to 16 bytes of alignment at either end
     if (a.cols <= 8192) return launch_rows<T, true, 128, true>(a, 1, per, smem, s);
