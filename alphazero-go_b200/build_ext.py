@@ -2,7 +2,9 @@
 sm_100a only (SASS, no PTX) with the CUDA runtime linked statically, so the
 library loads on a machine without a GPU (the driver API is reached at run
 time through cudaGetDriverEntryPoint). Translation units compile in
-parallel into _build/ (git-ignored), then link.
+parallel into _build/ (git-ignored), then link. Beside it _azb_torch.so, the
+operators' binding for torch tensors (binding/azb_torch.cpp, g++ against the
+installed torch's headers).
 
     python alphazero-go_b200/build_ext.py [--force]
 """
@@ -81,8 +83,13 @@ def _object(src: str, khash: str) -> tuple[list[str], str]:
 
 def build(force: bool = False, verbose: bool = False) -> str:
     """Compiles the translation units in parallel into _build/, then links."""
-    if not force and up_to_date():
-        return OUT
+    if force or not up_to_date():
+        _build_engine(force, verbose)
+    _build_binding(force, verbose)
+    return OUT
+
+
+def _build_engine(force: bool, verbose: bool) -> None:
     from concurrent.futures import ThreadPoolExecutor
 
     khash = kernel_hash()
@@ -116,7 +123,41 @@ def build(force: bool = False, verbose: bool = False) -> str:
     for f in os.listdir(OBJ):   # objects of earlier sources
         if f.endswith(".o") and f not in keep:
             os.remove(os.path.join(OBJ, f))
-    return OUT
+
+
+BINDING = os.path.join(HERE, "binding", "azb_torch.cpp")
+BINDING_OUT = os.path.join(HERE, "_azb_torch.so")
+
+
+def _build_binding(force: bool, verbose: bool) -> None:
+    """_azb_torch.so, rebuilt when its source, the C ABI, torch or Python changes."""
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-isystem", os.path.join(root, "include"), "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           "-isystem", sysconfig.get_paths()["include"], "-isystem", os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include"),
+           "-I", INCLUDE, BINDING, "-o", BINDING_OUT + ".tmp", "-L", HERE, "-l:libazb200.so",
+           "-L", os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10",
+           "-Wl,-rpath,$ORIGIN"]
+    h = hashlib.sha256(" ".join(cmd + [torch.__version__, sys.version]).encode())
+    for path in (BINDING, os.path.join(INCLUDE, "azb200.h")):
+        with open(path, "rb") as f:
+            h.update(f.read())
+    key_path, key = os.path.join(OBJ, "azb_torch.key"), h.hexdigest()
+    if not force and os.path.exists(BINDING_OUT) and os.path.exists(key_path) and open(key_path).read() == key:
+        return
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"azb_torch.cpp: g++ failed ({r.returncode}):\n{r.stdout}\n{r.stderr}")
+    os.replace(BINDING_OUT + ".tmp", BINDING_OUT)
+    os.makedirs(OBJ, exist_ok=True)
+    with open(key_path, "w") as f:
+        f.write(key)
 
 
 if __name__ == "__main__":

@@ -230,6 +230,12 @@ def test_product_is_repeatable_and_takes_vectors(ops, torch):
     assert torch.equal(v, ops.mx4_product(x[:1], w, dtype=torch.float32)[0])
 
 
+def test_mx4_from_its_parts(ops, torch):
+    q = ops.mx4_quantise(gpu(torch, normals(3, 45, 100), "float32"))
+    again = ops.Mx4(q.codes.clone(), q.scales.clone(), 45, 100)
+    assert torch.equal(ops.mx4_values(again), ops.mx4_values(q)) and again.nbytes() == q.nbytes()
+
+
 def test_empty_sides(ops, torch):
     w = ops.mx4_quantise(gpu(torch, normals(2, 30, 40), "float32"))
     assert ops.mx4_product(torch.empty(0, 40, device="cuda"), w).shape == (0, 30)
@@ -272,6 +278,8 @@ def test_refusals(ops, torch):
         (lambda: ops.mx4_product(x, w, bias=torch.ones(3, device="cuda")), "bias: 4 adjacent"),
         (lambda: ops.mx4_product(x, w, bias=torch.ones(4)), "bias on cpu"),
         (lambda: ops.mx4_product(x.cpu(), w), "CUDA tensor"),
+        (lambda: ops.mx4_product(w, ops.mx4_quantise(x[:, :32])), "x has 64 columns, w 32"),
+        (lambda: ops.Mx4(w.codes, w.scales[:-1], 4, 64), "bytes of codes and scales"),
     ]:
         with pytest.raises(ValueError, match=text):
             call()

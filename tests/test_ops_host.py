@@ -118,6 +118,8 @@ def test_python_refuses_host_tensors():
     with pytest.raises(ValueError, match="CUDA tensor"):
         A.mx4_quantise(x)
     with pytest.raises(ValueError, match="CUDA tensor"):
+        A.mx4_quantise([1.0])
+    with pytest.raises(ValueError, match="CUDA tensor"):
         A.sample_moves(x, x)
     with pytest.raises(ValueError, match="an Mx4 is needed"):
         A.mx4_product(x, x)
