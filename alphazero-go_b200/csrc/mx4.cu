@@ -282,6 +282,7 @@ struct ProductTile {
     void* out;
     long long ld;
     int early_w;           // w and its scales may be read before the previous launch ends
+    int out_fours;         // four neighbouring outputs may be stored at once
     const void* x;         // plain x, where the kernel quantises it itself, and its rows
     long long x_ld;
     int k, x_bytes;        // x_bytes: the widest load that its rows' alignment allows
@@ -342,11 +343,52 @@ __device__ __forceinline__ bool elect_one() {
     return p != 0;
 }
 
+__device__ __forceinline__ float activated(const ProductTile& p, float v) { return p.relu && v < 0.0f ? 0.0f : v; }   // keeps a NaN
+
+// A lane's four of a tile's 128 outputs of a row: neighbours where they can
+// be stored at once or come from other CTAs' parts, else every 32nd, so that
+// a warp's stores are neighbours.
+__device__ __forceinline__ int out_place(const ProductTile& p, int lane, int e) {
+    return p.out_fours || p.splits > 1 ? lane * 4 + e : lane + 32 * e;
+}
+
 template <typename T>
-__device__ __forceinline__ void store_out(const ProductTile& p, int row, int col, float v, float bias) {
-    v += bias;
-    if (p.relu) v = v < 0.0f ? 0.0f : v;   // keeps a NaN
-    static_cast<T*>(p.out)[size_t(row) * size_t(p.ld) + size_t(col)] = T(v);
+__device__ __forceinline__ void store_four(const ProductTile& p, int row, int n0, int lane, const float (&sum)[4], const float (&bias)[4]) {
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = activated(p, sum[e] + bias[e]);
+    T* to = static_cast<T*>(p.out) + size_t(row) * size_t(p.ld) + n0;
+    if (p.out_fours && n0 + lane * 4 + 4 <= p.n) {
+        if constexpr (sizeof(T) == 2) {
+            uint2 w;
+            reinterpret_cast<__nv_bfloat162*>(&w)[0] = __floats2bfloat162_rn(y[0], y[1]);
+            reinterpret_cast<__nv_bfloat162*>(&w)[1] = __floats2bfloat162_rn(y[2], y[3]);
+            *reinterpret_cast<uint2*>(to + lane * 4) = w;
+        } else {
+            *reinterpret_cast<float4*>(to + lane * 4) = make_float4(y[0], y[1], y[2], y[3]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (n0 + out_place(p, lane, e) < p.n) to[out_place(p, lane, e)] = T(y[e]);
+    }
+}
+
+// The four of `row` of a part in this CTA's shared memory.
+__device__ __forceinline__ void load_four(const ProductTile& p, const float* row, int lane, float (&v)[4]) {
+    if (p.out_fours) {
+        const float4 f = *reinterpret_cast<const float4*>(row + lane * 4);
+        v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = row[lane + 32 * e];
+    }
+}
+
+// The same of a part in another CTA's, at a shared::cluster address.
+__device__ __forceinline__ void load_four_of(uint32_t row, int lane, float (&v)[4]) {
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(row + uint32_t(lane) * 16) : "memory");
 }
 
 // A block of 32 elements of plain x.
@@ -392,8 +434,7 @@ __global__ void __launch_bounds__(kPThreads)
     const int split = int(blockIdx.x) % p.splits;
     const int n0 = int(blockIdx.x) / p.splits * kPTile, x0 = int(blockIdx.y) * p.tn;
     // This CTA's chunks of K: an even share, in order.
-    const int c_begin = int((long long)p.chunks * split / p.splits);
-    const int c_end = int((long long)p.chunks * (split + 1) / p.splits);
+    const int c_begin = p.chunks * split / p.splits, c_end = p.chunks * (split + 1) / p.splits;
     const int ahead = min(p.stages, c_end - c_begin);
     const uint32_t stage = stage_bytes(p.tn), x_bytes = uint32_t(p.tn) * kPChunkBytes;
     const int x_tile = x0 >> 7, x_tiles = (p.m + 127) >> 7;
@@ -493,8 +534,6 @@ __global__ void __launch_bounds__(kPThreads)
     __syncwarp();
 
     const int quarter = warp & 3;                 // the TMEM lanes this warp may read
-    const int j = n0 + quarter * 32 + lane;       // this thread's row of w: an output column
-    const float bias = p.bias && j < p.n ? p.bias[j] : 0.0f;
     const int live = min(p.tn, p.m - x0);         // the tile's rows of x
     float* part = reinterpret_cast<float*>(base);
     if constexpr (kPlain) {
@@ -530,6 +569,9 @@ __global__ void __launch_bounds__(kPThreads)
         mbar_wait(&done, 0, &g_mx4_error, kErrWaitEpilogue);
         tc_fence_after();
         if (p.early_w) grid_dependency_wait();    // the output may be what earlier launches read
+        // The accumulator into shared memory (the stages are done with), a
+        // row of x after the other: from there a warp stores a row's 128
+        // outputs at a time, neighbours together.
         for (int c0 = 0; c0 < live; c0 += 32) {
             uint32_t v[32];
             if (live - c0 > 16) {
@@ -542,15 +584,9 @@ __global__ void __launch_bounds__(kPThreads)
             }
             tmem_wait_ld();
             tmem_hold(v);
-            if (p.splits > 1) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (c0 + i < live) part[(c0 + i) * kPTile + quarter * 32 + lane] = __uint_as_float(v[i]);
-            } else if (j < p.n) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (c0 + i < live) store_out<T>(p, x0 + c0 + i, j, __uint_as_float(v[i]), bias);
-            }
+            for (int i = 0; i < 32; ++i)
+                if (c0 + i < live) part[(c0 + i) * kPTile + quarter * 32 + lane] = __uint_as_float(v[i]);
         }
     }
     // TMEM goes back before any wait for another CTA: a CTA that waits for a
@@ -558,37 +594,57 @@ __global__ void __launch_bounds__(kPThreads)
     tc_fence_before();
     __syncthreads();
     if (warp == 1) tmem_dealloc(tmem, p.tmem_cols);
-    if (p.splits > 1) {
-        // The parts' sum, in order of K (the same bits on every run): CTA
-        // `split` finishes rows split, split + splits, ... of the tile.
-        cluster_sync();
-        if (warp >= 2) {
-            constexpr int kAhead = 4;   // rows whose parts are all asked for before the first sum
-            for (int i0 = split; i0 < live; i0 += p.splits * kAhead) {
-                float v[kAhead][kPMaxSplits];
+    float bias[4];
 #pragma unroll
-                for (int u = 0; u < kAhead; ++u) {
-                    const int i = min(i0 + u * p.splits, live - 1);
-#pragma unroll
-                    for (int r = 0; r < kPMaxSplits; ++r)
-                        if (r < p.splits) {
-                            const uint32_t a = mapa(smem_u32(part + i * kPTile + quarter * 32 + lane), uint32_t(r));
-                            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[u][r]) : "r"(a) : "memory");
-                        }
-                }
-#pragma unroll
-                for (int u = 0; u < kAhead; ++u) {
-                    const int i = i0 + u * p.splits;
-                    float sum = v[u][0];
-#pragma unroll
-                    for (int r = 1; r < kPMaxSplits; ++r)
-                        if (r < p.splits) sum += v[u][r];
-                    if (i < live && j < p.n) store_out<T>(p, x0 + i, j, sum, bias);
-                }
-            }
-        }
-        cluster_sync();
+    for (int e = 0; e < 4; ++e) {
+        const int n = n0 + out_place(p, lane, e);
+        bias[e] = p.bias && n < p.n ? p.bias[n] : 0.0f;
     }
+    if (p.splits == 1) {
+        constexpr int kAhead = 4, kStep = kPThreads / 32;
+        for (int i0 = warp; i0 < live; i0 += kStep * kAhead) {
+            float v[kAhead][4];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+                if (i0 + u * kStep < live) load_four(p, part + (i0 + u * kStep) * kPTile, lane, v[u]);
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+                if (i0 + u * kStep < live) store_four<T>(p, x0 + i0 + u * kStep, n0, lane, v[u], bias);
+        }
+        return;
+    }
+    // The parts' sum, in order of K (the same bits on every run): CTA `split`
+    // finishes rows split, split + splits, ... of the tile.
+    cluster_sync();
+    constexpr int kAhead = 4;   // rows whose parts are all asked for before the first sum
+    const int step = p.splits * (kPThreads / 32);
+    for (int i0 = split + p.splits * warp; i0 < live; i0 += step * kAhead) {
+        float v[kAhead][kPMaxSplits][4];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (i0 + u * step >= live) break;
+            const uint32_t at = smem_u32(part + (i0 + u * step) * kPTile);
+#pragma unroll
+            for (int r = 0; r < kPMaxSplits; ++r)
+                if (r < p.splits) load_four_of(mapa(at, uint32_t(r)), lane, v[u][r]);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int i = i0 + u * step;
+            if (i >= live) break;
+            float sum[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                sum[e] = v[u][0][e];
+#pragma unroll
+                for (int r = 1; r < kPMaxSplits; ++r)
+                    if (r < p.splits) sum[e] += v[u][r][e];
+            }
+            store_four<T>(p, x0 + i, n0, lane, sum, bias);
+        }
+    }
+    __syncwarp();
+    cluster_sync();   // no CTA leaves while another reads its part
 }
 
 // ------------------------------------------------- product by CTA pairs
@@ -960,19 +1016,23 @@ ProductPlan plan_of(long long m, long long n, long long k) {
     for (const int tn : {128, 256})
         if (m > 128 && (m + tn - 1) / tn * p.n_tiles >= kSms) p.tn = tn;
     p.x_tiles = int((m + p.tn - 1) / p.tn);
-    // Up to 64 columns two CTAs share an SM (four stages each), so that one's
-    // issue and waits fill the other's; K is shared by a cluster of CTAs while
-    // there are slots for them and every CTA keeps a chunk or more.
-    const int slots = p.tn <= 64 ? 2 * kSms : kSms;
+    // Up to 64 columns a CTA takes half an SM's memory. K is shared by a
+    // cluster of CTAs while there are SMs for them (over a long K two CTAs an
+    // SM, so that one's waits fill the other's: 1 x 8192 x 8192 8.2 us so, 8.9
+    // us with one; 64 x 4096 x 4096 9.0 and 7.6), every CTA keeps a chunk or
+    // more and there are enough of them to pay for the exchange (1024 x 362 x
+    // 722, three chunks: 6.4 us in one piece, 8.7 us in two).
+    const int slots = p.tn <= 64 && chunks >= 32 ? 2 * kSms : kSms;
     p.splits = 1;
-    while (p.splits < kPMaxSplits && (long long)p.n_tiles * p.x_tiles * p.splits * 2 <= slots && p.splits * 2 <= chunks)
+    while (chunks >= 4 && p.splits < kPMaxSplits && (long long)p.n_tiles * p.x_tiles * p.splits * 2 <= slots &&
+           p.splits * 2 <= chunks)
         p.splits *= 2;
     p.per_cta = (chunks + p.splits - 1) / p.splits;
     const size_t budget = p.tn <= 64 ? size_t(108) << 10 : size_t(220) << 10;
     p.stages = int(std::min<size_t>(kPMaxStages, budget / stage_bytes(p.tn)));
     p.stages = std::max(1, std::min(p.stages, p.per_cta));
-    // The parts of a shared K reuse the stages' memory: 512 bytes a column.
-    while (p.splits > 1 && size_t(p.stages) * stage_bytes(p.tn) < size_t(p.tn) * kPTile * 4) ++p.stages;
+    // The accumulator passes through the stages' memory: 512 bytes a column.
+    while (size_t(p.stages) * stage_bytes(p.tn) < size_t(p.tn) * kPTile * 4) ++p.stages;
     p.quantises = m <= kPPlainRows && p.per_cta <= kPPlainChunks;
     return p;
 }
@@ -1007,6 +1067,7 @@ cudaError_t launch_mx4_product(const MxProductArgs& a, int sms, cudaStream_t s) 
     p.out = a.out;
     p.ld = a.ld;
     p.early_w = a.after_quantise ? 1 : 0;
+    p.out_fours = reinterpret_cast<uintptr_t>(a.out) % (4 * elem_size(a.type)) == 0 && a.ld % 4 == 0;
     p.x = a.x;
     p.x_ld = a.x_ld;
     p.k = int(a.k);
