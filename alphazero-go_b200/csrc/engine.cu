@@ -346,6 +346,12 @@ CUtensorMap make_scale_map(const void* base, uint64_t tiles) {
     return make_map_2d(CU_TENSOR_MAP_DATA_TYPE_UINT32, base, 128, tiles, 512, 128, 2, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
+CUtensorMap make_out_map(void* base, int type, uint64_t cols, uint64_t rows, uint64_t ld) {
+    const uint32_t es = uint32_t(elem_size(type));
+    return make_map_2d(type == kElemBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, base, cols, rows,
+                       ld * es, 128 / es, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 // ---------------------------------------------------------------- weights
 
 int stem_k_for(const NetShape& s, int precision) { return round_up(9 * s.planes(), chunk_channels(precision)); }

@@ -659,9 +659,11 @@ __global__ void __launch_bounds__(kPThreads)
 // storing.
 //
 // kRowsOnLanes: TMEM's lanes are rows of x, so a thread holds neighbouring
-// outputs of one row and stores 16 bytes at a time (p.vec: `out` is aligned
-// for that); otherwise they are rows of w and a warp stores 32 neighbouring
-// outputs at a time, whatever the alignment.
+// outputs of one row; its warp lays them out in shared memory, 32 rows of 128
+// bytes at a time, and TMA stores them (where `out` is aligned for it; 16-byte
+// stores of 32 lanes into 32 rows took 6600 cycles a tile). Otherwise the
+// lanes are rows of w and a warp stores 32 neighbouring outputs at a time,
+// whatever the alignment.
 struct PairTile {
     int lanes, cols;                 // rows of the operand on the lanes and of the other
     int lane_tiles, tiles;           // tiles along the lanes, and in all
@@ -672,8 +674,12 @@ struct PairTile {
     long long ld;
 };
 
-constexpr int kPairFromTiles = 32;
-constexpr int kPairThreads = 320, kPairEpiWarps = 8, kPairStages = 6;
+// From so many tiles, and more than 128 rows on either side: 64 tiles of
+// 1024 x 4096 x 2048 9.9 us by pairs and 16.2 us without, 32 of 512 x 4096 x
+// 4096 12.5 and 10.7.
+constexpr int kPairFromTiles = 48;
+constexpr int kPairThreads = 320, kPairEpiWarps = 8, kPairStages = 5;
+constexpr uint32_t kPairBox = 32 * 128;   // an epilogue warp's rows on their way out
 constexpr uint32_t kPairScaleCols = 24, kPairTmemCols = 512;   // per stage: 2 x 4 of the lanes' scales, 2 x 8 of the columns'
 constexpr uint32_t kPairStageBytes = 2 * kPWBytes + 1024 + 2048;
 
@@ -694,7 +700,8 @@ __device__ __forceinline__ void umma_mx4_pair(uint32_t tmem_d, uint64_t adesc, u
 template <typename T, bool kRowsOnLanes>
 __global__ void __launch_bounds__(kPairThreads, 1)
     mx4_pair_kernel(const __grid_constant__ CUtensorMap ml, const __grid_constant__ CUtensorMap mc,
-                    const __grid_constant__ CUtensorMap sl, const __grid_constant__ CUtensorMap sc, const PairTile p) {
+                    const __grid_constant__ CUtensorMap sl, const __grid_constant__ CUtensorMap sc,
+                    const __grid_constant__ CUtensorMap mo, const PairTile p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     __shared__ __align__(8) uint64_t full[kPairStages], empty[kPairStages], acc_full, acc_empty, done;
@@ -810,6 +817,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         const uint32_t taddr = tmem + (uint32_t(quarter) << 21) + uint32_t(half) * 128;
         const uint32_t to_leader = mapa(smem_u32(&acc_empty), 0);
         T* const out = static_cast<T*>(p.out);
+        const float floor = p.relu ? 0.0f : __uint_as_float(0xFF800000u);
+        uint8_t* const boxes = base + size_t(kPairStages) * kPairStageBytes;   // 1024-byte aligned, as the swizzle needs
+        uint8_t* const box = boxes + size_t(warp - 2) * kPairBox;
+        float* const bias_of = reinterpret_cast<float*>(boxes + kPairEpiWarps * kPairBox) + (warp - 2) * 128;   // of its columns
         uint32_t j = 0;
         for (int tile = int(blockIdx.x) >> 1; tile < p.tiles; tile += pairs, ++j) {
             if (!mbar_wait(&acc_full, j & 1u, &g_mx4_error, kErrWaitEpilogue)) break;
@@ -827,37 +838,43 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             const int c0 = tile / p.lane_tiles * 256 + half * 128;
             const auto act = [&](uint32_t bits, float bias) {
                 const float y = __uint_as_float(bits) + bias;
-                return p.relu && y < 0.0f ? 0.0f : y;   // keeps a NaN
+                return y < floor ? floor : y;   // keeps a NaN
             };
             if constexpr (kRowsOnLanes) {
-                if (l >= p.lanes) continue;
-                T* const dst = out + size_t(l) * size_t(p.ld) + c0;
+                constexpr int kW = 16 / int(sizeof(T)), kCols = 8 * kW;   // columns in 16 and in 128 bytes
+                __syncwarp();
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    constexpr int kW = 16 / int(sizeof(T));
+                for (int e = 0; e < 4; ++e) {
+                    const int i = lane + 32 * e;
+                    bias_of[i] = p.bias && c0 + i < p.cols ? __ldg(p.bias + c0 + i) : 0.0f;
+                }
 #pragma unroll
-                    for (int i = 0; i < 32; i += kW) {
-                        const int c = c0 + q * 32 + i;
+                for (int q = 0; q < 128 / kCols; ++q) {
+                    if (lane == 0) bulk_wait_read<0>();   // the box's previous store has read it
+                    __syncwarp();
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
                         float y[kW];
 #pragma unroll
-                        for (int e = 0; e < kW; ++e) y[e] = act(v[q][i + e], p.bias && c + e < p.cols ? __ldg(p.bias + c + e) : 0.0f);
-                        if (c + kW <= p.cols) {
-                            uint4 w;
-                            if constexpr (sizeof(T) == 2) {
+                        for (int e = 0; e < kW; ++e) {
+                            const int i = q * kCols + u * kW + e;
+                            y[e] = act(v[i >> 5][i & 31], bias_of[i]);
+                        }
+                        uint4 w;
+                        if constexpr (sizeof(T) == 2) {
 #pragma unroll
-                                for (int e = 0; e < kW; e += 2)
-                                    reinterpret_cast<__nv_bfloat162*>(&w)[e >> 1] = __floats2bfloat162_rn(y[e], y[e + 1]);
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < kW; ++e) reinterpret_cast<float*>(&w)[e] = y[e];
-                            }
-                            *reinterpret_cast<uint4*>(dst + q * 32 + i) = w;
+                            for (int e = 0; e < kW; e += 2)
+                                reinterpret_cast<__nv_bfloat162*>(&w)[e >> 1] = __floats2bfloat162_rn(y[e], y[e + 1]);
                         } else {
 #pragma unroll
-                            for (int e = 0; e < kW; ++e)
-                                if (c + e < p.cols) dst[q * 32 + i + e] = T(y[e]);
+                            for (int e = 0; e < kW; ++e) reinterpret_cast<float*>(&w)[e] = y[e];
                         }
+                        *reinterpret_cast<uint4*>(box + lane * 128 + ((u ^ (lane & 7)) << 4)) = w;   // (128-byte swizzle)
                     }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0 && l < p.lanes && c0 + q * kCols < p.cols) tma_store_2d(&mo, box, c0 + q * kCols, l);
+                    if (lane == 0) bulk_commit();
                 }
             } else {
                 if (l >= p.lanes) continue;
@@ -872,6 +889,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                     }
             }
         }
+        if (kRowsOnLanes && lane == 0) bulk_wait_all();
     }
     __syncwarp();
     tc_fence_before();
@@ -908,7 +926,8 @@ cudaError_t launch_pair(const MxProductArgs& a, int sms, cudaStream_t s) {
     const CUtensorMap mc = make_byte_map(cc, uint64_t(cs.pitch()), uint64_t(cs.rows), 128);
     const CUtensorMap sl = make_scale_map(lsc, uint64_t(ls.row_tiles()) * uint64_t(ls.scale_tiles()));
     const CUtensorMap sc = make_scale_map(csc, uint64_t(cs.row_tiles()) * uint64_t(cs.scale_tiles()));
-    const size_t smem = 1024 + size_t(kPairStages) * kPairStageBytes;
+    const CUtensorMap mo = kRowsOnLanes ? make_out_map(a.out, a.type, uint64_t(a.n), uint64_t(a.m), uint64_t(a.ld)) : ml;
+    const size_t smem = 1024 + size_t(kPairStages) * kPairStageBytes + (kRowsOnLanes ? kPairEpiWarps * (kPairBox + 512) : 0);
     if (const cudaError_t e = open_smem<mx4_pair_kernel<T, kRowsOnLanes>>(smem); e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(2 * std::min(p.tiles, sms / 2)));
@@ -922,10 +941,10 @@ cudaError_t launch_pair(const MxProductArgs& a, int sms, cudaStream_t s) {
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = a.after_quantise ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, mx4_pair_kernel<T, kRowsOnLanes>, ml, mc, sl, sc, p);
+    return cudaLaunchKernelEx(&cfg, mx4_pair_kernel<T, kRowsOnLanes>, ml, mc, sl, sc, mo, p);
 }
 
-// Whether rows of `out` can be stored 16 bytes at a time.
+// Whether TMA can store rows of `out`.
 bool out_aligned(const MxProductArgs& a) {
     return reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && size_t(a.ld) * elem_size(a.type) % 16 == 0;
 }

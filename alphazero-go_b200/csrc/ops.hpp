@@ -99,5 +99,8 @@ CUtensorMap make_byte_map(const void* base, uint64_t pitch, uint64_t rows, uint3
 
 // A map of `tiles` scale tiles of 512 bytes, in boxes of two.
 CUtensorMap make_scale_map(const void* base, uint64_t tiles);
+// A map of rows x cols elements of an ElemType (rows `ld` elements apart, a
+// multiple of 16 bytes) in boxes of 32 rows x 128 bytes, 128-byte swizzle.
+CUtensorMap make_out_map(void* base, int type, uint64_t cols, uint64_t rows, uint64_t ld);
 
 }  // namespace azb

@@ -161,7 +161,8 @@ def test_strided_outputs_leave_the_rest_alone(ops, torch):
 
 SHAPES = [(1, 1, 1), (1, 128, 256), (1, 362, 722), (1, 1000, 4096), (3, 5, 33), (15, 129, 65), (16, 64, 64),
           (17, 300, 511), (33, 127, 2000), (64, 256, 1025), (65, 31, 300), (100, 640, 96), (128, 128, 128),
-          (129, 130, 257), (192, 4000, 64), (300, 362, 722), (1000, 1100, 320), (2100, 2500, 31), (1, 3, 9000)]
+          (129, 130, 257), (192, 4000, 64), (300, 362, 722), (1000, 1100, 320), (2100, 2500, 31), (1, 3, 9000),
+          (2049, 2311, 513), (1793, 1936, 1000), (9000, 130, 70), (130, 20000, 65)]
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
