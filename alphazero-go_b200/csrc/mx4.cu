@@ -154,7 +154,7 @@ constexpr int kCastThreads = 256, kCastWarps = kCastThreads / 32, kCastUnroll = 
               kCastSpan = kCastStep * kCastUnroll;
 
 template <typename T, int kBytes>
-__global__ void __launch_bounds__(kCastThreads, 4) mx4_quantise_kernel(const MxCastArgs a) {
+__global__ void __launch_bounds__(kCastThreads, 5) mx4_quantise_kernel(const MxCastArgs a) {
     const MxShape s = a.shape;
     const int lane = threadIdx.x & 31;
     const long long c0 = (long long)blockIdx.y * kCastSpan + lane * 16;
