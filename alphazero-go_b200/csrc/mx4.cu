@@ -155,6 +155,10 @@ constexpr int kCastThreads = 256, kCastWarps = kCastThreads / 32, kCastUnroll = 
 
 template <typename T, int kBytes>
 __global__ void __launch_bounds__(kCastThreads, 5) mx4_quantise_kernel(const MxCastArgs a) {
+    // Past the wait every earlier launch has completed, so that the next may
+    // start (it waits itself, or reads only what earlier ones wrote).
+    grid_dependency_wait();
+    grid_launch_dependents();
     const MxShape s = a.shape;
     const int lane = threadIdx.x & 31;
     const long long c0 = (long long)blockIdx.y * kCastSpan + lane * 16;
@@ -181,7 +185,6 @@ __global__ void __launch_bounds__(kCastThreads, 5) mx4_quantise_kernel(const MxC
             if ((lane & 7) == 0 && (block >> 2) < tiles) *reinterpret_cast<uint32_t*>(scales + (block >> 2) * 512) = word;
         }
     }
-    grid_launch_dependents();
 }
 
 // The inverse; a thread takes 8 elements, so that a warp's 16-byte stores of
@@ -192,6 +195,8 @@ constexpr int kValuesUnroll = 4, kValuesStep = 256, kValuesSpan = kValuesStep * 
 
 template <typename T, int kBytes>
 __global__ void __launch_bounds__(kCastThreads, 5) mx4_values_kernel(const MxCastArgs a) {
+    grid_dependency_wait();
+    grid_launch_dependents();
     const MxShape s = a.shape;
     const int lane = threadIdx.x & 31;
     const long long c0 = (long long)blockIdx.y * kValuesSpan + lane * 8;
@@ -470,6 +475,7 @@ __global__ void __launch_bounds__(kPThreads)
         if (!p.early_w) grid_dependency_wait();
         for (int i = 0; i < ahead; ++i) load_w(c_begin + i, i);
         if (p.early_w) grid_dependency_wait();
+        grid_launch_dependents();
         for (int i = 0; i < ahead; ++i) load_x(c_begin + i, i);
     }
     if (warp == 1) tmem_alloc(&tmem_slot, p.tmem_cols);
@@ -539,6 +545,7 @@ __global__ void __launch_bounds__(kPThreads)
     if constexpr (kPlain) {
         if (warp >= 2) {
             const int t = int(threadIdx.x) - 64;
+            grid_dependency_wait();
             // Block b of row r of chunk c into stage s, as TMA and the scales'
             // copies lay them out. (x is one tile of at most 16 rows; rows past
             // m stay as they are: they reach no column that is stored.)
@@ -568,7 +575,6 @@ __global__ void __launch_bounds__(kPThreads)
     if (warp >= 2) {
         mbar_wait(&done, 0, &g_mx4_error, kErrWaitEpilogue);
         tc_fence_after();
-        if (p.early_w) grid_dependency_wait();    // the output may be what earlier launches read
         // The accumulator into shared memory (the stages are done with), a
         // row of x after the other: from there a warp stores a row's 128
         // outputs at a time, neighbours together.
@@ -731,6 +737,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     grid_dependency_wait();
+    grid_launch_dependents();
 
     if (warp == 0) {
         if (elect_one()) {
@@ -940,7 +947,7 @@ cudaError_t launch_pair(const MxProductArgs& a, int sms, cudaStream_t s) {
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = a.after_quantise ? 2 : 1;
+    cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, mx4_pair_kernel<T, kRowsOnLanes>, ml, mc, sl, sc, mo, p);
 }
 
@@ -950,7 +957,7 @@ bool out_aligned(const MxProductArgs& a) {
 }
 
 template <typename T, int kGroups, typename X>
-cudaError_t launch_product_t(const CUtensorMap& mw, const CUtensorMap& mx, const ProductTile& p, dim3 grid, bool pdl,
+cudaError_t launch_product_t(const CUtensorMap& mw, const CUtensorMap& mx, const ProductTile& p, dim3 grid,
                              cudaStream_t s) {
     const size_t smem = 1024 + size_t(p.stages) * stage_bytes(p.tn);
     if (const cudaError_t e = open_smem<mx4_product_kernel<T, kGroups, X>>(smem); e != cudaSuccess) return e;
@@ -961,15 +968,11 @@ cudaError_t launch_product_t(const CUtensorMap& mw, const CUtensorMap& mx, const
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
     int na = 0;
+    attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[na++].val.programmaticStreamSerializationAllowed = 1;
     if (p.splits > 1) {
         attr[na].id = cudaLaunchAttributeClusterDimension;
-        attr[na].val.clusterDim = {unsigned(p.splits), 1, 1};
-        ++na;
-    }
-    if (pdl) {
-        attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[na].val.programmaticStreamSerializationAllowed = 1;
-        ++na;
+        attr[na++].val.clusterDim = {unsigned(p.splits), 1, 1};
     }
     cfg.attrs = attr;
     cfg.numAttrs = unsigned(na);
@@ -981,33 +984,35 @@ cudaError_t launch_product_t(const CUtensorMap& mw, const CUtensorMap& mx, const
 cudaError_t launch_mx4_quantise(const MxCastArgs& a, int sms, cudaStream_t s) {
     const dim3 grid = cast_grid(a.shape.row_tiles() * 128, a.shape.scale_tiles() * 128, kCastSpan, sms);
     const int bytes = row_bytes(a.plain, a.shape.rows, a.ld, a.type);
+    cudaError_t e;
     if (a.type == kElemBF16) {
-        if (bytes == 16) mx4_quantise_kernel<__nv_bfloat16, 16><<<grid, kCastThreads, 0, s>>>(a);
-        else if (bytes == 8) mx4_quantise_kernel<__nv_bfloat16, 8><<<grid, kCastThreads, 0, s>>>(a);
-        else if (bytes == 4) mx4_quantise_kernel<__nv_bfloat16, 4><<<grid, kCastThreads, 0, s>>>(a);
-        else mx4_quantise_kernel<__nv_bfloat16, 2><<<grid, kCastThreads, 0, s>>>(a);
+        if (bytes == 16) e = launch_pdl(mx4_quantise_kernel<__nv_bfloat16, 16>, grid, dim3(kCastThreads), 0, s, a);
+        else if (bytes == 8) e = launch_pdl(mx4_quantise_kernel<__nv_bfloat16, 8>, grid, dim3(kCastThreads), 0, s, a);
+        else if (bytes == 4) e = launch_pdl(mx4_quantise_kernel<__nv_bfloat16, 4>, grid, dim3(kCastThreads), 0, s, a);
+        else e = launch_pdl(mx4_quantise_kernel<__nv_bfloat16, 2>, grid, dim3(kCastThreads), 0, s, a);
     } else {
-        if (bytes == 16) mx4_quantise_kernel<float, 16><<<grid, kCastThreads, 0, s>>>(a);
-        else if (bytes == 8) mx4_quantise_kernel<float, 8><<<grid, kCastThreads, 0, s>>>(a);
-        else mx4_quantise_kernel<float, 4><<<grid, kCastThreads, 0, s>>>(a);
+        if (bytes == 16) e = launch_pdl(mx4_quantise_kernel<float, 16>, grid, dim3(kCastThreads), 0, s, a);
+        else if (bytes == 8) e = launch_pdl(mx4_quantise_kernel<float, 8>, grid, dim3(kCastThreads), 0, s, a);
+        else e = launch_pdl(mx4_quantise_kernel<float, 4>, grid, dim3(kCastThreads), 0, s, a);
     }
-    return cudaGetLastError();
+    return e;
 }
 
 cudaError_t launch_mx4_values(const MxCastArgs& a, int sms, cudaStream_t s) {
     const dim3 grid = cast_grid(a.shape.rows, a.shape.cols, kValuesSpan, sms);
     const int bytes = row_bytes(a.plain, a.shape.rows, a.ld, a.type);
+    cudaError_t e;
     if (a.type == kElemBF16) {
-        if (bytes == 16) mx4_values_kernel<__nv_bfloat16, 16><<<grid, kCastThreads, 0, s>>>(a);
-        else if (bytes == 8) mx4_values_kernel<__nv_bfloat16, 8><<<grid, kCastThreads, 0, s>>>(a);
-        else if (bytes == 4) mx4_values_kernel<__nv_bfloat16, 4><<<grid, kCastThreads, 0, s>>>(a);
-        else mx4_values_kernel<__nv_bfloat16, 2><<<grid, kCastThreads, 0, s>>>(a);
+        if (bytes == 16) e = launch_pdl(mx4_values_kernel<__nv_bfloat16, 16>, grid, dim3(kCastThreads), 0, s, a);
+        else if (bytes == 8) e = launch_pdl(mx4_values_kernel<__nv_bfloat16, 8>, grid, dim3(kCastThreads), 0, s, a);
+        else if (bytes == 4) e = launch_pdl(mx4_values_kernel<__nv_bfloat16, 4>, grid, dim3(kCastThreads), 0, s, a);
+        else e = launch_pdl(mx4_values_kernel<__nv_bfloat16, 2>, grid, dim3(kCastThreads), 0, s, a);
     } else {
-        if (bytes == 16) mx4_values_kernel<float, 16><<<grid, kCastThreads, 0, s>>>(a);
-        else if (bytes == 8) mx4_values_kernel<float, 8><<<grid, kCastThreads, 0, s>>>(a);
-        else mx4_values_kernel<float, 4><<<grid, kCastThreads, 0, s>>>(a);
+        if (bytes == 16) e = launch_pdl(mx4_values_kernel<float, 16>, grid, dim3(kCastThreads), 0, s, a);
+        else if (bytes == 8) e = launch_pdl(mx4_values_kernel<float, 8>, grid, dim3(kCastThreads), 0, s, a);
+        else e = launch_pdl(mx4_values_kernel<float, 4>, grid, dim3(kCastThreads), 0, s, a);
     }
-    return cudaGetLastError();
+    return e;
 }
 
 namespace {
@@ -1096,10 +1101,10 @@ cudaError_t launch_mx4_product(const MxProductArgs& a, int sms, cudaStream_t s) 
     const dim3 grid(unsigned(plan.n_tiles * p.splits), unsigned(plan.x_tiles));
     const auto launch = [&](auto out) {
         using T = decltype(out);
-        if (a.x) return a.x_type == kElemBF16 ? launch_product_t<T, 1, __nv_bfloat16>(mw, mx, p, grid, false, s)
-                                              : launch_product_t<T, 1, float>(mw, mx, p, grid, false, s);
-        return p.tn > 128 ? launch_product_t<T, 2, void>(mw, mx, p, grid, a.after_quantise, s)
-                          : launch_product_t<T, 1, void>(mw, mx, p, grid, a.after_quantise, s);
+        if (a.x) return a.x_type == kElemBF16 ? launch_product_t<T, 1, __nv_bfloat16>(mw, mx, p, grid, s)
+                                              : launch_product_t<T, 1, float>(mw, mx, p, grid, s);
+        return p.tn > 128 ? launch_product_t<T, 2, void>(mw, mx, p, grid, s)
+                          : launch_product_t<T, 1, void>(mw, mx, p, grid, s);
     };
     return a.type == kElemBF16 ? launch(__nv_bfloat16()) : launch(0.0f);
 }

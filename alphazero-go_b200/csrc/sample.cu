@@ -182,6 +182,8 @@ __device__ Threshold find_threshold(const RowParams& rp, uint32_t top, uint32_t 
 // cheap bounds of their keys leave in it.
 template <typename T, int kPer>
 __global__ void __launch_bounds__(128) sample_warp_kernel(const SampleArgs a) {
+    grid_dependency_wait();     // every earlier launch has completed,
+    grid_launch_dependents();   // so the next may start
     const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
     if (row >= a.rows) return;
     const int lane = threadIdx.x & 31;
@@ -735,6 +737,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
     const long long row = kSolo ? blockIdx.x : blockIdx.x / unsigned(ranks);
     const Crew crew{rank, ranks};
     if constexpr (!kSolo) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // this CTA runs: its memory may be written
+    grid_dependency_wait();
+    grid_launch_dependents();
     const RowParams rp(a, row);
     Slice<T, kResident, kThreads> sl;
     const int i0 = min(rank * per, a.cols);
@@ -1258,11 +1262,13 @@ cudaError_t launch_rows(const SampleArgs& a, int ranks, int per, size_t smem, cu
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim = {unsigned(ranks), 1, 1};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim = {unsigned(ranks), 1, 1};
     cfg.attrs = attr;
-    cfg.numAttrs = kSolo ? 0 : 1;
+    cfg.numAttrs = kSolo ? 1 : 2;
     return cudaLaunchKernelEx(&cfg, kernel, a, ranks, per);
 }
 
@@ -1270,10 +1276,9 @@ template <typename T>
 cudaError_t launch_sample_t(const SampleArgs& a, cudaStream_t s) {
     const int grid = int((a.rows + 3) / 4);
     if (a.cols <= 1024) {
-        if (a.cols <= 128) sample_warp_kernel<T, 4><<<grid, 128, 0, s>>>(a);
-        else if (a.cols <= 384) sample_warp_kernel<T, 12><<<grid, 128, 0, s>>>(a);
-        else sample_warp_kernel<T, 32><<<grid, 128, 0, s>>>(a);
-        return cudaGetLastError();
+        if (a.cols <= 128) return launch_pdl(sample_warp_kernel<T, 4>, dim3(unsigned(grid)), dim3(128), 0, s, a);
+        if (a.cols <= 384) return launch_pdl(sample_warp_kernel<T, 12>, dim3(unsigned(grid)), dim3(128), 0, s, a);
+        return launch_pdl(sample_warp_kernel<T, 32>, dim3(unsigned(grid)), dim3(128), 0, s, a);
     }
     // Up to 16384 columns one CTA has the row (1024 rows of 16384: 45 us, with
     // two of 8192 each 75 us); beyond, slices of at most 8192 while eight CTAs
