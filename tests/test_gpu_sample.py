@@ -119,6 +119,58 @@ def test_sizes_and_filters(ops, torch, cols, filters, dtype):
     check(ops, torch, logits, noise, legal, dtype, **filters)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("cols", [70001, 131072, 450001])
+def test_wide_rows(ops, torch, cols, dtype):
+    """Rows beyond what shared memory holds."""
+    logits, noise, r = data(cols, 3, cols)
+    legal = r.random((3, cols)) < 0.6
+    logits[1, ::7] = np.nan
+    logits[2, 5::3] = -np.inf
+    for f in FILTERS:
+        check(ops, torch, logits, noise, None, dtype, **f)
+    check(ops, torch, logits, noise, legal, dtype, top_k=50, top_p=0.9)
+    check(ops, torch, logits, noise, legal, dtype, min_p=0.1)
+    check(ops, torch, logits, noise, legal, dtype, temperature=0.0)
+    check(ops, torch, logits, noise, legal, dtype, top_k=3000, top_p=0.999)
+
+
+@pytest.mark.parametrize("cols", [20000, 100001])
+def test_wide_rows_with_ties_and_infinities(ops, torch, cols):
+    logits, noise, r = data(8, 4, cols, 1.0)
+    for f in FILTERS:
+        check(ops, torch, np.round(logits), noise, **f)
+    check(ops, torch, np.zeros_like(logits), noise, top_k=777)
+    check(ops, torch, np.zeros_like(logits), noise, top_p=0.25)
+    logits[0, [5, 77, cols - 1]] = np.inf
+    logits[1, cols - 1] = np.inf
+    logits[2] = -np.inf
+    logits[3] = np.nan
+    logits[3, cols // 2] = -3e38
+    for f in FILTERS:
+        m, lp = check(ops, torch, logits, noise, **f)
+        assert m[1] == cols - 1 and m[2] == -1 and m[3] == cols // 2 and lp[3] == 0
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_wide_rows_with_strides(ops, torch, dtype):
+    """Rows of odd length and offset, of logits, legality and noise alike."""
+    cols = 70003
+    logits, noise, r = data(12, 5, cols + 9)
+    legal = r.random((5, cols + 9)) < 0.5
+    if dtype == "bfloat16":
+        logits = torch.as_tensor(logits).to(torch.bfloat16).float().numpy()
+    L, N = torch.as_tensor(logits, device="cuda").to(getattr(torch, dtype)), torch.as_tensor(noise, device="cuda")
+    A = torch.as_tensor(legal, device="cuda")
+    for off in (0, 1, 3, 8):
+        cut = slice(off, off + cols)
+        m, lp = ops.sample_moves(L[:, cut], N[:, cut], legal=A[:, cut], top_p=0.9)
+        for row in range(5):
+            moves, ref = reference(logits[row, cut], noise[row, cut], legal[row, cut], 1.0, 0, 0.9, 0.0)
+            assert int(m[row]) in moves
+            assert abs(float(lp[row]) - ref[int(m[row])]) <= 1e-5 + 3e-7 * abs(ref[int(m[row])])
+
+
 @pytest.mark.parametrize("cols", [362, 3000])
 def test_many_ties(ops, torch, cols):
     """Logits on a coarse grid: every cut falls inside a group of equal ones."""
