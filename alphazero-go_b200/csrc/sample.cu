@@ -850,6 +850,38 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
         const bool by_k = k > 0 && k < all.valid, by_p = rp.filters_p() && rp.top_p > 0.0f && k != 1;
         uint64_t cut = place_of(kKeyLow, 0x7FFFFFFF);   // the last place kept
         bool raced = false;
+        // A warp's race of kN columns a lane, those with a bit in `in`. With
+        // d = 1 - u: d <= -log u <= d / u, so that in log2 a column's key lies
+        // between reach and reach + lg2(u). The two logarithms (accurate, where
+        // the bounds' are approximate: the margins) are taken only where the
+        // upper bound reaches the warp's best so far, at first its best lower
+        // bound. ok(l, i): whether a column is in the race after all.
+        float lead = neg_inf();
+        const auto race_some = [&](auto n, const float* l, const float* u, uint32_t in, auto column, auto ok) {
+            constexpr int kN = decltype(n)::value;
+            const auto reach = [&](int g) { return (l[g] - m) * c - lg2(fmaxf(1.0f - u[g], 5.9604645e-8f)); };
+            if (lead == neg_inf()) {
+                float least = neg_inf();
+#pragma unroll
+                for (int g = 0; g < (kN < 4 ? kN : 4); ++g)   // (of a few: it is asked of columns that may yet drop out)
+                    if ((in >> g & 1u) && ok(l[g], column(g))) least = fmaxf(least, reach(g) + lg2(clamped(u[g])));
+                lead = logit_of_key(__reduce_max_sync(0xFFFFFFFFu, key_of(least))) - 2e-3f;
+            }
+            uint32_t marks = 0;
+#pragma unroll
+            for (int g = 0; g < kN; ++g) marks |= reach(g) >= lead ? 1u << g : 0u;
+            for (marks &= in; marks; marks &= marks - 1) {
+                const int b = __ffs(int(marks)) - 1;
+                float lb = l[0], ub = u[0];
+#pragma unroll
+                for (int g = 1; g < kN; ++g)
+                    if (g == b) lb = l[g], ub = u[g];
+                if (ok(lb, column(b))) run_race(lb, i0 + column(b), ub);
+            }
+            __syncwarp();
+            const uint32_t k = __reduce_max_sync(0xFFFFFFFFu, uint32_t(best >> 32));
+            if (k) lead = fmaxf(lead, logit_of_key(k) * kLog2e - 1e-3f);
+        };
         const auto passes_min_p = [&](float l) { return l == m || !(rp.min_p > 0.0f) || ex2((l - m) * c) >= rp.min_p; };
         // A little below the logit of log2 w = y (and never -inf, which stands
         // around the slice).
@@ -869,14 +901,17 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
             }
         };
         if (by_k || by_p) {
+            float listed = inf;   // every logit of at least this is among the upper ones
             const auto at = [&](uint32_t key) {
                 Weighed s{0, 0.0f};
-                sl.each([&](float l, int) {
+                const auto add = [&](float l, int) {
                     if (key_of(l) >= key) {
                         ++s.count;
                         s.mass += ex2((l - m) * c);
                     }
-                });
+                };
+                if (key >= key_of(listed)) each_upper(listed, add);
+                else sl.each(add);
                 return team_add(crew, s, sh, turn);
             };
             // What the histogram covers: log2 w from `low` to 0. Any range that
@@ -903,9 +938,10 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
                 steps = float(kBins - 1) / -low;
                 for (int b = t; b < kBins; b += kThreads) sh.hist_n[b] = sh.hist_w[b] = 0;
                 if (t == 0) sh.first = sh.last = kBins, sh.list_n = 0;
-                upper_n = sl.list_above(logit_below(low), part);
+                listed = logit_below(low);
+                upper_n = sl.list_above(listed, part);
                 __syncthreads();
-                each_upper(logit_below(low), [&](float l, int) {
+                each_upper(listed, [&](float l, int) {
                     const float y = (l - m) * c;
                     if (y >= low) {
                         const int b = bin_of(y);
@@ -991,22 +1027,25 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
                     });
                 } else {
                     constexpr int kAhead = 4;   // numbers asked for before the first is used
-                    for (int j0 = lane; j0 < upper_n; j0 += 32 * kAhead) {
+                    for (int b0 = 0; b0 < upper_n; b0 += 32 * kAhead) {
+                        const int j0 = b0 + lane;
                         int i[kAhead];
-                        float u[kAhead];
+                        float l[kAhead], u[kAhead];
                         uint32_t in = 0;
 #pragma unroll
-                        for (int g = 0; g < kAhead; ++g)
-                            if (j0 + 32 * g < upper_n) {
-                                i[g] = part[j0 + 32 * g];
-                                if (place_in(sl.at(i[g]), i[g])) {
-                                    in |= 1u << g;
-                                    u[g] = __ldg(noise + i[g]);
-                                }
+                        for (int g = 0; g < kAhead; ++g) {
+                            i[g] = 0, l[g] = neg_inf(), u[g] = 0.0f;
+                            if (j0 + 32 * g >= upper_n) continue;
+                            i[g] = part[j0 + 32 * g];
+                            l[g] = sl.at(i[g]);
+                            if (place_in(l[g], i[g])) {
+                                in |= 1u << g;
+                                u[g] = __ldg(noise + i[g]);
                             }
-#pragma unroll
-                        for (int g = 0; g < kAhead; ++g)
-                            if (in >> g & 1u) run_race(sl.at(i[g]), i0 + i[g], u[g]);
+                        }
+                        if (final)
+                            race_some(std::integral_constant<int, kAhead>(), l, u, in, [&](int b) { return int(part[j0 + 32 * b]); },
+                                      [](float, int) { return true; });
                     }
                 }
                 s = team_add(crew, s, sh, turn);   // (also: every list is written)
@@ -1135,7 +1174,9 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
                     while (end - lo > 1) {
                         const int mid = lo + (end - lo) / 2;
                         Weighed s{0, 0.0f};
-                        sl.each([&](float l, int i) { s.count += i0 + i < mid && key_of(l) == th.key; });
+                        const auto add = [&](float l, int i) { s.count += i0 + i < mid && key_of(l) == th.key; };
+                        if (th.key >= key_of(listed)) each_upper(listed, add);
+                        else sl.each(add);
                         if (team_add(crew, s, sh, turn).count >= th.ties) end = mid;
                         else lo = mid;
                     }
@@ -1162,26 +1203,13 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
                     });
             }
             if (upper_n < 0) {
-                // -log u >= 1 - u, so that log2(w) - log2(1 - u) bounds a
-                // column's key from above: the two logarithms (accurate, where
-                // the bound's are approximate: the margin) are taken only
-                // where the bound reaches the warp's best so far.
-                float lead = neg_inf();   // the warp's best key, in log2
-                const auto bound = [&](float l, float u) { return (l - m) * c - lg2(fmaxf(1.0f - u, 5.9604645e-8f)) + 1e-3f; };
-                const auto consider = [&](float l, int i, float u) {
-                    if (bound(l, u) >= lead && stays(l, i)) run_race(l, i0 + i, u);
-                };
-                const auto follow = [&] {
-                    const uint32_t k = __reduce_max_sync(0xFFFFFFFFu, uint32_t(best >> 32));
-                    if (k) lead = logit_of_key(k) * kLog2e;
-                };
                 if constexpr (kResident) {
                     using P = Pack<T>;
-                    constexpr int W = P::kWidth, kAhead = 16 / W;
+                    constexpr int W = P::kWidth, kAhead = 16 / W, kN = kAhead * W;
                     const int np = sl.packs();
                     const bool wide = (reinterpret_cast<uintptr_t>(noise) - 4u * unsigned(sl.shift)) % 16 == 0;
                     for (int w0 = t & ~31; w0 < np; w0 += kThreads * kAhead) {   // a warp's lanes stay together
-                        float u[kAhead * W];
+                        float l[kN], u[kN];
 #pragma unroll
                         for (int g = 0; g < kAhead; ++g) {
                             const int v = w0 + lane + g * kThreads, i = v * W - sl.shift;
@@ -1197,31 +1225,27 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
                                     u[g * W + e] = v < np && i + e >= 0 && i + e < sl.n ? __ldg(noise + i + e) : 0.0f;
                             }
                         }
+                        uint32_t in = 0;
 #pragma unroll
                         for (int g = 0; g < kAhead; ++g) {
                             const int v = w0 + lane + g * kThreads;
                             P p;
-                            float most = neg_inf();
                             if (v < np) {
                                 p = sl.mem[v];
-#pragma unroll
-                                for (int e = 0; e < W; ++e) most = fmaxf(most, bound(p.get(e), u[g * W + e]));
+                                in |= ((1u << W) - 1u) << (g * W);
                             }
-                            if (!__any_sync(0xFFFFFFFFu, most >= lead)) continue;
-                            if (v < np) {
 #pragma unroll
-                                for (int e = 0; e < W; ++e) consider(p.get(e), v * W - sl.shift + e, u[g * W + e]);
-                            }
-                            __syncwarp();
-                            follow();
+                            for (int e = 0; e < W; ++e) l[g * W + e] = v < np ? p.get(e) : neg_inf();
                         }
+                        const auto column = [&](int b) { return (w0 + lane + b / W * kThreads) * W - sl.shift + b % W; };
+                        race_some(std::integral_constant<int, kN>(), l, u, in, column, stays);
                     }
                 } else {
                     for (int w0 = t & ~31; w0 < sl.n; w0 += kThreads) {
                         const int i = w0 + lane;
-                        if (i < sl.n) consider(sl.direct(i), i, __ldg(noise + i));
-                        __syncwarp();
-                        follow();
+                        const bool there = i < sl.n;
+                        const float l = there ? sl.direct(i) : neg_inf(), u = there ? __ldg(noise + i) : 0.0f;
+                        race_some(std::integral_constant<int, 1>(), &l, &u, there, [&](int) { return i; }, stays);
                     }
                 }
             }
