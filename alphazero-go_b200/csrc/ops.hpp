@@ -91,12 +91,11 @@ struct SampleArgs {
     long long* moves;
     float* logprob;          // or null
 };
-cudaError_t launch_sample_moves(const SampleArgs& a, int sms, cudaStream_t s);
+cudaError_t launch_sample_moves(const SampleArgs& a, cudaStream_t s);
 
 // A map of `rows` rows of `pitch` bytes (pitch a multiple of 16) in boxes of
 // 128 bytes x box_rows rows, 128-byte swizzle.
 CUtensorMap make_byte_map(const void* base, uint64_t pitch, uint64_t rows, uint32_t box_rows);
-
 // A map of `tiles` scale tiles of 512 bytes, in boxes of two.
 CUtensorMap make_scale_map(const void* base, uint64_t tiles);
 // A map of rows x cols elements of an ElemType (rows `ld` elements apart, a

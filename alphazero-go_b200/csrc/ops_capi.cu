@@ -215,7 +215,7 @@ int azb_sample_moves(int device, const azb_sample_args* p, void* stream, char* e
                            p->temperature, p->top_p, p->min_p, p->top_k, p->temperature_rows, p->top_p_rows,
                            p->min_p_rows, p->top_k_rows, reinterpret_cast<long long*>(p->moves), p->logprob};
         const OnDevice on(device);
-        check(launch_sample_moves(a, on.sms(), stream_of(stream)), fn);
+        check(launch_sample_moves(a, stream_of(stream)), fn);
     });
 }
 

@@ -14,8 +14,9 @@
 // integers) and, where several logits equal it, how many of those. The
 // threshold is found by halving the range of keys, each time counting and
 // weighing the logits at or above the middle, until one logit (or one group
-// of equal ones) is left in the range. Counts are exact and sums run in a
-// fixed order, so a row's move does not depend on the batch or the run.
+// of equal ones) is left in the range (rows beyond a warp: mostly from a
+// histogram). Counts are exact and sums run in a fixed order, so a row's move
+// does not depend on the batch or the run.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -180,6 +181,12 @@ __device__ Threshold find_threshold(const RowParams& rp, uint32_t top, uint32_t 
 // for at once, the reductions are single instructions where the type allows,
 // and the race's two accurate logarithms are taken only for the columns that
 // cheap bounds of their keys leave in it.
+//
+// Bound by the latency of its steps: one row of 362 in 2.9 us, with top-k and
+// top-p, whose halvings follow one another, 5.9 us; 1024 rows of 362 with all
+// filters 8.7 us, 27% of the issue slots used. (Masses in fixed point, one
+// instruction a sum instead of five exchanges: 8.5 us, but 1024 rows of 1000
+// 19.4 instead of 18.6.)
 template <typename T, int kPer>
 __global__ void __launch_bounds__(128) sample_warp_kernel(const SampleArgs a) {
     grid_dependency_wait();     // every earlier launch has completed,
@@ -343,7 +350,16 @@ __global__ void __launch_bounds__(128) sample_warp_kernel(const SampleArgs a) {
 // rounding; the logits in it (a list of at most kList) are sorted and the
 // exact cut found among them, on top of the exact count and mass of what lies
 // above. Where the list would be longer (many equal logits, say) the range of
-// keys is halved as in find_threshold.
+// keys is halved as in find_threshold, over the listed upper logits.
+//
+// 512 rows of 131072 (fp32, top-p 0.9) take 270 us: 469 MB from DRAM (the
+// kept columns' numbers come in sectors of 32 bytes), a fifth of its rate. A
+// CTA lives 25 us, of which the load takes 3.4, the sum 1.9, the first
+// exchange 2.2, the list and histogram 5.1 with their exchange, the cut 9
+// with four more; three CTAs an SM (their slices fill it) overlap these, the
+// barriers of a cluster's eight being what is waited for. Without filters
+// 178 us. (One CTA a row, its passes reading L2: 375 us, and one row 76 us
+// where a cluster takes 18.)
 //
 // Lower bounds keep most logits out of the histogram: with k <= the number of
 // groups of threads that hold a logit, the k-th largest is at least the least
@@ -1318,8 +1334,7 @@ cudaError_t launch_sample_t(const SampleArgs& a, cudaStream_t s) {
 
 }  // namespace
 
-cudaError_t launch_sample_moves(const SampleArgs& a, int sms, cudaStream_t s) {
-    (void)sms;
+cudaError_t launch_sample_moves(const SampleArgs& a, cudaStream_t s) {
     return a.type == kElemBF16 ? launch_sample_t<__nv_bfloat16>(a, s) : launch_sample_t<float>(a, s);
 }
 
