@@ -146,15 +146,15 @@ __device__ __forceinline__ size_t scale_offset(const MxShape& s, long long row, 
 
 // A thread takes 16 elements, two neighbours one block; a warp 512 neighbours
 // of a row at a time, kCastUnroll of those with all loads in flight before
-// the first is used. blockIdx.y: the span of columns; rows are shared out
-// over blockIdx.x and the block's warps. Rows up to the next multiple of 128
+// the first is used. blockIdx.x: the span of columns (there may be more than
+// 65535); rows are shared out over blockIdx.y and the block's warps. Rows up to the next multiple of 128
 // and blocks up to the next multiple of 4 are visited too: their scales are
 // set to zero. kBytes: the widest load that every row's alignment allows.
 //
 // Bound by DRAM where the matrix is large: 16384 x 8192 of bfloat16 in 53 us
 // with nothing in L2 (5.4 TB/s of 268 MB read and the codes written). Five
 // blocks an SM (at most 51 registers) and two steps in flight: there and back
-// 118 us, with four blocks 121. Few rows are bound by the launch: 3 us.
+// 113 us, with four blocks 3 us more. Few rows are bound by the launch: 3 us.
 constexpr int kCastThreads = 256, kCastWarps = kCastThreads / 32, kCastUnroll = 2, kCastStep = 512,
               kCastSpan = kCastStep * kCastUnroll;
 
@@ -166,9 +166,9 @@ __global__ void __launch_bounds__(kCastThreads, 5) mx4_quantise_kernel(const MxC
     grid_launch_dependents();
     const MxShape s = a.shape;
     const int lane = threadIdx.x & 31;
-    const long long c0 = (long long)blockIdx.y * kCastSpan + lane * 16;
+    const long long c0 = (long long)blockIdx.x * kCastSpan + lane * 16;
     const long long rows = s.row_tiles() * 128, blocks = s.blocks(), tiles = s.scale_tiles();
-    for (long long row = (long long)blockIdx.x * kCastWarps + (threadIdx.x >> 5); row < rows; row += (long long)gridDim.x * kCastWarps) {
+    for (long long row = (long long)blockIdx.y * kCastWarps + (threadIdx.x >> 5); row < rows; row += (long long)gridDim.y * kCastWarps) {
         const T* src = static_cast<const T*>(a.plain) + size_t(row) * size_t(a.ld);
         const long long cols = row < s.rows ? s.cols : 0;
         Run<T, 16> v[kCastUnroll];
@@ -205,8 +205,8 @@ __global__ void __launch_bounds__(kCastThreads, 5) mx4_values_kernel(const MxCas
     grid_launch_dependents();
     const MxShape s = a.shape;
     const int lane = threadIdx.x & 31;
-    const long long c0 = (long long)blockIdx.y * kValuesSpan + lane * 8;
-    for (long long row = (long long)blockIdx.x * kCastWarps + (threadIdx.x >> 5); row < s.rows; row += (long long)gridDim.x * kCastWarps) {
+    const long long c0 = (long long)blockIdx.x * kValuesSpan + lane * 8;
+    for (long long row = (long long)blockIdx.y * kCastWarps + (threadIdx.x >> 5); row < s.rows; row += (long long)gridDim.y * kCastWarps) {
         const uint8_t* codes = a.codes + size_t(row) * size_t(s.pitch());
         const uint8_t* scales = a.scales + scale_offset(s, row, 0);
         uint32_t q[kValuesUnroll], scale[kValuesUnroll];
@@ -267,7 +267,7 @@ int row_bytes(const void* p, long long rows, long long ld, int type) {
 dim3 cast_grid(long long rows, long long cols, int span, int sms) {
     const long long spans = (cols + span - 1) / span;
     const long long most = std::max<long long>(1, (long long)sms * 16 / spans);   // sixteen blocks an SM in all
-    return dim3(unsigned(std::min((rows + kCastWarps - 1) / kCastWarps, most)), unsigned(spans));
+    return dim3(unsigned(spans), unsigned(std::min((rows + kCastWarps - 1) / kCastWarps, most)));
 }
 
 // --------------------------------------------------------------- product

@@ -146,6 +146,17 @@ def raw(ops, fn, *args):
     assert getattr(ops.azb200.lib(), fn)(*args, e, 1024) == 0, e.value
 
 
+@pytest.mark.parametrize("cols", [(1 << 26) - 5, 1 << 26])
+def test_longest_rows(ops, torch, cols):
+    """A row of 2^26 columns is the blocks of 2^16 rows of 1024."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(1 << 16, 1024, generator=g, device="cuda", dtype=torch.bfloat16)
+    x.view(-1)[cols:] = 0
+    a, b = ops.mx4_quantise(x.view(1, -1)[:, :cols]), ops.mx4_quantise(x)
+    assert torch.equal(a.codes.flatten(), b.codes.flatten())
+    assert torch.equal(ops.mx4_values(a, torch.bfloat16)[0], ops.mx4_values(b, torch.bfloat16).flatten()[:cols])
+
+
 def test_strided_outputs_leave_the_rest_alone(ops, torch):
     x, w = gpu(torch, normals(5, 9, 70), "float32"), gpu(torch, normals(6, 37, 70), "float32")
     qx, qw = ops.mx4_quantise(x), ops.mx4_quantise(w)
