@@ -8,6 +8,8 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <algorithm>
+#include <climits>
 #include <cstring>
 #include <string>
 
@@ -103,12 +105,17 @@ struct Matrix {
     const void* at;
 };
 
+// A gradient would be lost: there is no backward pass.
+void no_gradient(const at::Tensor& t, const char* what) {
+    require(!(t.requires_grad() && c10::GradMode::is_enabled()),
+            std::string(what) + " requires a gradient, and there is no backward pass (detach it)");
+}
+
 Matrix matrix(const at::Tensor& t, const char* what) {
     Matrix m{};
     m.type = elem_type(t.scalar_type(), what);
     require(t.dim() == 2, std::string(what) + ": a matrix is needed, not " + std::to_string(t.dim()) + " dimensions");
-    require(!(t.requires_grad() && c10::GradMode::is_enabled()),
-            std::string(what) + " requires a gradient, and there is no backward pass (detach it)");
+    no_gradient(t, what);
     m.rows = t.size(0);
     m.cols = t.size(1);
     require(m.cols >= 1, std::string(what) + ": at least one column is needed");
@@ -212,6 +219,7 @@ PyObject* mx4_product(PyObject*, PyObject* const* args, Py_ssize_t n) {
             require(fits, "bias: " + std::to_string(w.rows) + " adjacent float32 numbers are needed");
             const at::Tensor& b = THPVariable_Unpack(args[6]);
             require(b.device() == device, "x is on " + name_of(device) + ", bias on " + name_of(b.device()));
+            no_gradient(b, "bias");
             bias = static_cast<const float*>(b.const_data_ptr());
         }
         const int relu = PyObject_IsTrue(args[7]);
@@ -243,13 +251,15 @@ void setting(PyObject* o, const char* name, long long rows, const at::Device& de
              T* one, const T** each) {
     *each = nullptr;
     if (!THPVariable_Check(o)) {
-        *one = T(type == at::kInt ? double(whole(o)) : number(o));
+        if (type == at::kInt) *one = T(std::clamp<long long>(whole(o), INT_MIN, INT_MAX));
+        else *one = T(number(o));
         return;
     }
     const at::Tensor& t = THPVariable_Unpack(o);
     require(t.scalar_type() == type && t.dim() == 1 && t.size(0) == rows && t.device() == device && t.is_contiguous(),
             std::string(name) + ": a number, or " + std::to_string(rows) + " adjacent " + type_name + " numbers on " +
                 name_of(device));
+    no_gradient(t, name);
     *one = T(0);
     *each = static_cast<const T*>(t.const_data_ptr());
 }

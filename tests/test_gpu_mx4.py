@@ -284,6 +284,7 @@ def test_refusals(ops, torch):
         (lambda: ops.mx4_quantise(x[0]), "a matrix is needed"),
         (lambda: ops.mx4_quantise(x[:, :0]), "at least one column"),
         (lambda: ops.mx4_quantise(x.clone().requires_grad_()), "no backward pass"),
+        (lambda: ops.mx4_product(x, w, bias=x[0, :4].clone().requires_grad_()), "bias requires a gradient"),
         (lambda: ops.mx4_values(w, torch.float16), "float32 or bfloat16"),
         (lambda: ops.mx4_product(x[:, :32], w), "x has 32 columns, w 64"),
         (lambda: ops.mx4_product(x, x), "an Mx4 is needed"),

@@ -135,6 +135,21 @@ def test_wide_rows(ops, torch, cols, dtype):
     check(ops, torch, logits, noise, legal, dtype, top_k=3000, top_p=0.999)
 
 
+@pytest.mark.parametrize("cols", [600001, 900001])
+def test_widest_rows_bfloat16(ops, torch, cols):
+    """Slices beyond 16-bit places, and beyond shared memory, in the shorter type."""
+    logits, noise, r = data(cols, 2, cols)
+    for f in FILTERS:
+        check(ops, torch, logits, noise, None, "bfloat16", **f)
+
+
+def test_top_k_beyond_32_bits_is_off(ops, torch):
+    logits, noise, r = data(4, 6, 300)
+    for k in (300, 2 ** 31 - 1, 2 ** 31, 2 ** 40):
+        m, lp = run(ops, torch, logits, noise, top_k=k)
+        assert (m == run(ops, torch, logits, noise)[0]).all()
+
+
 @pytest.mark.parametrize("cols", [20000, 100001])
 def test_wide_rows_with_ties_and_infinities(ops, torch, cols):
     logits, noise, r = data(8, 4, cols, 1.0)
@@ -348,6 +363,7 @@ def test_refusals_and_empty(ops, torch):
     l, n = torch.zeros(3, 40, device="cuda"), torch.rand(3, 40, device="cuda")
     for call, text in [
         (lambda: ops.sample_moves(l.half(), n), "float32 or bfloat16"),
+        (lambda: ops.sample_moves(l, n, temperature=torch.ones(3, device="cuda").requires_grad_()), "no backward pass"),
         (lambda: ops.sample_moves(l.t(), n.t()), "columns must be adjacent"),
         (lambda: ops.sample_moves(l, n.double()), "noise: float32"),
         (lambda: ops.sample_moves(l, n[:, :39]), "noise: float32"),
