@@ -58,12 +58,10 @@ __device__ __forceinline__ void unpack_e2m1(uint32_t codes, float* v) {
     }
 }
 
-// kBytes (2 to 16) from global memory into the words at dst.
 template <int kBytes>
-__device__ __forceinline__ void load_piece(uint32_t* dst, const void* src) {
-    if constexpr (kBytes == 16) *reinterpret_cast<uint4*>(dst) = __ldcs(static_cast<const uint4*>(src));
-    else if constexpr (kBytes == 8) *reinterpret_cast<uint2*>(dst) = __ldcs(static_cast<const uint2*>(src));
-    else if constexpr (kBytes == 4) *dst = __ldcs(static_cast<const uint32_t*>(src));
+__device__ __forceinline__ void load_piece(uint32_t* dst, const uint32_t* src) {
+    if constexpr (kBytes == 16) *reinterpret_cast<uint4*>(dst) = __ldcs(reinterpret_cast<const uint4*>(src));
+    else *reinterpret_cast<uint2*>(dst) = __ldcs(reinterpret_cast<const uint2*>(src));
 }
 
 // kN neighbouring elements of a row as they lie in memory (kN T in words).
@@ -72,24 +70,51 @@ struct Run {
     static constexpr int kWords = kN * int(sizeof(T)) / 4;
     uint32_t u[kWords];
 
-    // Elements [c, c + kN), zeros past `cols`; kBytes: what the row's
-    // alignment lets one load take.
+    // Elements [c, c + kN), zeros past `cols`; c a multiple of kN. kBytes: 16
+    // or 8, of which the row starts at a multiple, or 0 (any row).
     template <int kBytes>
     __device__ __forceinline__ void load(const T* row, long long c, long long cols) {
-        if (kBytes >= 4 && c + kN <= cols) {
+        if constexpr (kBytes > 0) {
+            if (c + kN <= cols) {
 #pragma unroll
-            for (int i = 0; i < kWords; i += kBytes / 4)
-                load_piece<kBytes>(u + i, reinterpret_cast<const uint8_t*>(row + c) + 4 * i);
+                for (int i = 0; i < kWords; i += kBytes / 4)
+                    load_piece<kBytes>(u + i, reinterpret_cast<const uint32_t*>(row + c) + i);
+                return;
+            }
         } else {
+            // The run lies `off` bytes into its first 16: those and the ones
+            // after are read whole, where they are the row's, and shifted.
+            const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(row + c) & 15);
+            const long long first = c - off / int(sizeof(T)), end = first + kN + (off ? 16 / int(sizeof(T)) : 0);
+            if (first >= 0 && end <= cols) {
+                uint32_t w[kWords + 4];
+                const uint32_t* from = reinterpret_cast<const uint32_t*>(row + first);
 #pragma unroll
-            for (int i = 0; i < kWords; ++i) {
-                if constexpr (sizeof(T) == 4) {
-                    u[i] = c + i < cols ? __ldg(reinterpret_cast<const uint32_t*>(row + c) + i) : 0u;
-                } else {
-                    const uint16_t* h = reinterpret_cast<const uint16_t*>(row + c) + 2 * i;
-                    u[i] = c + 2 * i < cols ? __ldg(h) : 0u;
-                    if (c + 2 * i + 1 < cols) u[i] |= uint32_t(__ldg(h + 1)) << 16;
+                for (int i = 0; i < kWords; i += 4) load_piece<16>(w + i, from + i);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[kWords + i] = 0;
+                if (off) load_piece<16>(w + kWords, from + kWords);
+                if (off & 8) {
+#pragma unroll
+                    for (int i = 0; i < kWords + 2; ++i) w[i] = w[i + 2];
                 }
+                if (off & 4) {
+#pragma unroll
+                    for (int i = 0; i < kWords + 1; ++i) w[i] = w[i + 1];
+                }
+#pragma unroll
+                for (int i = 0; i < kWords; ++i) u[i] = sizeof(T) == 2 && (off & 2) ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
+                return;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                u[i] = c + i < cols ? __ldg(reinterpret_cast<const uint32_t*>(row + c) + i) : 0u;
+            } else {
+                const uint16_t* h = reinterpret_cast<const uint16_t*>(row + c) + 2 * i;
+                u[i] = c + 2 * i < cols ? __ldg(h) : 0u;
+                if (c + 2 * i + 1 < cols) u[i] |= uint32_t(__ldg(h + 1)) << 16;
             }
         }
     }
@@ -147,16 +172,22 @@ __device__ __forceinline__ size_t scale_offset(const MxShape& s, long long row, 
 // A thread takes 16 elements, two neighbours one block; a warp 512 neighbours
 // of a row at a time, kCastUnroll of those with all loads in flight before
 // the first is used. blockIdx.x: the span of columns (there may be more than
-// 65535); rows are shared out over blockIdx.y and the block's warps. Rows up to the next multiple of 128
-// and blocks up to the next multiple of 4 are visited too: their scales are
-// set to zero. kBytes: the widest load that every row's alignment allows.
+// 65535); rows are shared out over blockIdx.y and the block's warps. Rows up
+// to the next multiple of 128 and blocks up to the next multiple of 4 are
+// visited too: their scales are set to zero. Loads are of 16 bytes, shifted
+// into place where the rows do not start at multiples of 16 (16384 x 8191 of
+// fp32 108 us so and 277 us by elements, of bfloat16 67 and 150), but for
+// bfloat16 rows at multiples of 8, which take loads of 8 (59 us and 66).
 //
 // Bound by DRAM where the matrix is large: 16384 x 8192 of bfloat16 in 53 us
 // with nothing in L2 (5.4 TB/s of 268 MB read and the codes written). Five
 // blocks an SM (at most 51 registers) and two steps in flight: there and back
 // 113 us, with four blocks 3 us more. Few rows are bound by the launch: 3 us.
-constexpr int kCastThreads = 256, kCastWarps = kCastThreads / 32, kCastUnroll = 2, kCastStep = 512,
-              kCastSpan = kCastStep * kCastUnroll;
+constexpr int kCastThreads = 256, kCastWarps = kCastThreads / 32, kCastStep = 512;
+template <typename T>
+constexpr int kCastUnroll = sizeof(T) == 2 ? 2 : 1;   // as many as five blocks' registers hold
+template <typename T>
+constexpr int kCastSpan = kCastStep * kCastUnroll<T>;
 
 template <typename T, int kBytes>
 __global__ void __launch_bounds__(kCastThreads, 5) mx4_quantise_kernel(const MxCastArgs a) {
@@ -166,18 +197,18 @@ __global__ void __launch_bounds__(kCastThreads, 5) mx4_quantise_kernel(const MxC
     grid_launch_dependents();
     const MxShape s = a.shape;
     const int lane = threadIdx.x & 31;
-    const long long c0 = (long long)blockIdx.x * kCastSpan + lane * 16;
+    const long long c0 = (long long)blockIdx.x * kCastSpan<T> + lane * 16;
     const long long rows = s.row_tiles() * 128, blocks = s.blocks(), tiles = s.scale_tiles();
     for (long long row = (long long)blockIdx.y * kCastWarps + (threadIdx.x >> 5); row < rows; row += (long long)gridDim.y * kCastWarps) {
         const T* src = static_cast<const T*>(a.plain) + size_t(row) * size_t(a.ld);
         const long long cols = row < s.rows ? s.cols : 0;
-        Run<T, 16> v[kCastUnroll];
+        Run<T, 16> v[kCastUnroll<T>];
 #pragma unroll
-        for (int u = 0; u < kCastUnroll; ++u) v[u].template load<kBytes>(src, c0 + u * kCastStep, cols);
+        for (int u = 0; u < kCastUnroll<T>; ++u) v[u].template load<kBytes>(src, c0 + u * kCastStep, cols);
         uint8_t* codes = a.codes + size_t(row) * size_t(s.pitch());
         uint8_t* scales = a.scales + scale_offset(s, row, 0);
 #pragma unroll
-        for (int u = 0; u < kCastUnroll; ++u) {
+        for (int u = 0; u < kCastUnroll<T>; ++u) {
             const long long c = c0 + u * kCastStep, block = c >> 5;
             uint32_t field = v[u].top_field();
             field = max(field, __shfl_xor_sync(0xFFFFFFFFu, field, 1));
@@ -193,14 +224,24 @@ __global__ void __launch_bounds__(kCastThreads, 5) mx4_quantise_kernel(const MxC
 }
 
 // The inverse; a thread takes 8 elements, so that a warp's 16-byte stores of
-// bfloat16 are neighbours. A value is a code's magnitude times a
+// bfloat16 are neighbours (kBytes: what the rows are multiples of). Values of
+// fp32, and of bfloat16 in rows of odd places (kBytes 0), are exchanged so
+// that neighbouring lanes store neighbouring elements (16384 x 8192 of fp32 99
+// us, two stores of 16 bytes a lane 142; 16384 x 8191 108 us, by single
+// elements of a lane 518, of bfloat16 83 and 369). A value is a code's magnitude times a
 // power of two: exact in either type (the smallest, 2^-128, is a subnormal
 // that both hold). Bound by DRAM too: 16384 x 8192 into bfloat16 in 60 us
 // (5.7 TB/s of 71 MB read and 268 MB written).
 constexpr int kValuesUnroll = 4, kValuesStep = 256, kValuesSpan = kValuesStep * kValuesUnroll;
 
+// The magnitude's three bits on top of a float's significand and exponent are
+// that magnitude times 2^-126 (for 0.5 a subnormal).
+__device__ __forceinline__ float value_of(uint32_t code) {
+    return __uint_as_float((code & 8u) << 28 | (code & 7u) << 22) * 8.50705917e37f;
+}
+
 template <typename T, int kBytes>
-__global__ void __launch_bounds__(kCastThreads, 5) mx4_values_kernel(const MxCastArgs a) {
+__global__ void __launch_bounds__(kCastThreads, 6) mx4_values_kernel(const MxCastArgs a) {
     grid_dependency_wait();
     grid_launch_dependents();
     const MxShape s = a.shape;
@@ -221,44 +262,53 @@ __global__ void __launch_bounds__(kCastThreads, 5) mx4_values_kernel(const MxCas
 #pragma unroll
         for (int u = 0; u < kValuesUnroll; ++u) {
             const long long c = c0 + u * kValuesStep;
-            if (c >= s.cols) continue;
             // 2^(code - 127): code 0 is the subnormal 2^-127, code 255 NaN.
             const float x = __uint_as_float(scale[u] == 255 ? 0x7FC00000u : scale[u] ? scale[u] << 23 : 0x00400000u);
-            float v[8];
-            unpack_e2m1(q[u], v);
-            constexpr int kWords = 8 * int(sizeof(T)) / 4;
-            uint32_t w[kWords];
+            if constexpr (kBytes > 0) {
+                float v[8];
+                unpack_e2m1(q[u], v);
+                if (c + 8 <= s.cols) {
+                    uint32_t w[4];
 #pragma unroll
-            for (int i = 0; i < kWords; ++i) {
-                if constexpr (sizeof(T) == 4) {
-                    w[i] = __float_as_uint(v[i] * x);
+                    for (int i = 0; i < 4; ++i) {
+                        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i] * x, v[2 * i + 1] * x);
+                        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+                    }
+                    uint32_t* const to = reinterpret_cast<uint32_t*>(dst + c);
+                    if constexpr (kBytes == 16) {
+                        __stcs(reinterpret_cast<uint4*>(to), make_uint4(w[0], w[1], w[2], w[3]));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; i += kBytes / 4) {
+                            if constexpr (kBytes == 8) __stcs(reinterpret_cast<uint2*>(to + i), make_uint2(w[i], w[i + 1]));
+                            else __stcs(to + i, w[i]);
+                        }
+                    }
                 } else {
-                    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i] * x, v[2 * i + 1] * x);
-                    w[i] = *reinterpret_cast<const uint32_t*>(&h);
-                }
-            }
-            uint8_t* to = reinterpret_cast<uint8_t*>(dst + c);
-            if (kBytes >= 4 && c + 8 <= s.cols) {
 #pragma unroll
-                for (int i = 0; i < kWords; i += kBytes / 4) {
-                    if constexpr (kBytes == 16) __stcs(reinterpret_cast<uint4*>(to + 4 * i), make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]));
-                    else if constexpr (kBytes == 8) __stcs(reinterpret_cast<uint2*>(to + 4 * i), make_uint2(w[i], w[i + 1]));
-                    else __stcs(reinterpret_cast<uint32_t*>(to + 4 * i), w[i]);
+                    for (int i = 0; i < 8; ++i)
+                        if (c + i < s.cols) dst[c + i] = T(v[i] * x);
                 }
             } else {
+                const long long step = c - lane * 8;
+                const int left = int(min((long long)kValuesStep, s.cols - step)) - lane;
+                T* const to = dst + step + lane;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (c + i >= s.cols) break;
-                    if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(to)[i] = w[i];
-                    else reinterpret_cast<uint16_t*>(to)[i] = uint16_t(w[i >> 1] >> (i & 1 ? 16 : 0));
+                for (int j = 0; j < 8; ++j) {   // a block
+                    const uint32_t code = __shfl_sync(0xFFFFFFFFu, q[u], 4 * j + (lane >> 3)) >> (4 * (lane & 7));
+                    const float v = value_of(code) * __shfl_sync(0xFFFFFFFFu, x, 4 * j);
+                    if (32 * j < left) {
+                        if constexpr (sizeof(T) == 2)
+                            __stcs(reinterpret_cast<unsigned short*>(to + 32 * j), __bfloat16_as_ushort(__float2bfloat16_rn(v)));
+                        else __stcs(to + 32 * j, v);
+                    }
                 }
             }
         }
     }
 }
 
-// The widest load or store (16, 8, 4 bytes, or one 2-byte element) that the
-// alignment of every row allows.
+// The largest of 16, 8, 4 and 2 bytes of which every row starts at a multiple.
 int row_bytes(const void* p, long long rows, long long ld, int type) {
     const uintptr_t low = reinterpret_cast<uintptr_t>(p) | (rows > 1 ? uintptr_t(ld) * elem_size(type) : 0);
     return low % 16 == 0 ? 16 : low % 8 == 0 ? 8 : low % 4 == 0 ? 4 : 2;
@@ -302,7 +352,7 @@ struct ProductTile {
     int out_fours;         // four neighbouring outputs may be stored at once
     const void* x;         // plain x, where the kernel quantises it itself, and its rows
     long long x_ld;
-    int k, x_bytes;        // x_bytes: the widest load that its rows' alignment allows
+    int k, x_aligned;      // x_aligned: every row starts at a multiple of 16 bytes
 };
 
 constexpr int kPTile = 128, kPChunkBytes = 128, kPThreads = 192, kPMaxStages = 8, kPMaxSplits = 8;
@@ -412,14 +462,14 @@ __device__ __forceinline__ void load_four_of(uint32_t row, int lane, float (&v)[
 template <typename X>
 struct PlainBlock {
     Run<X, 16> a, b;
-    __device__ __forceinline__ void load(const X* row, long long c, long long cols, int bytes) {
-        if (bytes == 16) load_as<16>(row, c, cols);
-        else load_as<int(sizeof(X))>(row, c, cols);
-    }
-    template <int kBytes>
-    __device__ __forceinline__ void load_as(const X* row, long long c, long long cols) {
-        a.template load<kBytes>(row, c, cols);
-        b.template load<kBytes>(row, c + 16, cols);
+    __device__ __forceinline__ void load(const X* row, long long c, long long cols, bool aligned) {
+        if (aligned) {
+            a.template load<16>(row, c, cols);
+            b.template load<16>(row, c + 16, cols);
+        } else {
+            a.template load<0>(row, c, cols);
+            b.template load<0>(row, c + 16, cols);
+        }
     }
     __device__ __forceinline__ uint4 codes(uint32_t* code) const {
         *code = scale_code(max(a.top_field(), b.top_field()));
@@ -567,7 +617,7 @@ __global__ void __launch_bounds__(kPThreads)
             // m stay as they are: they reach no column that is stored.)
             const auto put = [&](int c, int s, int r, int b) {
                 PlainBlock<X> v;
-                v.load(static_cast<const X*>(p.x) + size_t(r) * size_t(p.x_ld), (long long)c * 256 + b * 32, p.k, p.x_bytes);
+                v.load(static_cast<const X*>(p.x) + size_t(r) * size_t(p.x_ld), (long long)c * 256 + b * 32, p.k, p.x_aligned != 0);
                 uint32_t code;
                 const uint4 q = v.codes(&code);
                 uint8_t* to = base + size_t(s) * stage + kPWBytes;
@@ -999,37 +1049,25 @@ cudaError_t launch_product_t(const CUtensorMap& mw, const CUtensorMap& mx, const
 }  // namespace
 
 cudaError_t launch_mx4_quantise(const MxCastArgs& a, int sms, cudaStream_t s) {
-    const dim3 grid = cast_grid(a.shape.row_tiles() * 128, a.shape.scale_tiles() * 128, kCastSpan, sms);
+    const int span = a.type == kElemBF16 ? kCastSpan<__nv_bfloat16> : kCastSpan<float>;
+    const dim3 grid = cast_grid(a.shape.row_tiles() * 128, a.shape.scale_tiles() * 128, span, sms);
     const int bytes = row_bytes(a.plain, a.shape.rows, a.ld, a.type);
-    cudaError_t e;
-    if (a.type == kElemBF16) {
-        if (bytes == 16) e = launch_pdl(mx4_quantise_kernel<__nv_bfloat16, 16>, grid, dim3(kCastThreads), 0, s, a);
-        else if (bytes == 8) e = launch_pdl(mx4_quantise_kernel<__nv_bfloat16, 8>, grid, dim3(kCastThreads), 0, s, a);
-        else if (bytes == 4) e = launch_pdl(mx4_quantise_kernel<__nv_bfloat16, 4>, grid, dim3(kCastThreads), 0, s, a);
-        else e = launch_pdl(mx4_quantise_kernel<__nv_bfloat16, 2>, grid, dim3(kCastThreads), 0, s, a);
-    } else {
-        if (bytes == 16) e = launch_pdl(mx4_quantise_kernel<float, 16>, grid, dim3(kCastThreads), 0, s, a);
-        else if (bytes == 8) e = launch_pdl(mx4_quantise_kernel<float, 8>, grid, dim3(kCastThreads), 0, s, a);
-        else e = launch_pdl(mx4_quantise_kernel<float, 4>, grid, dim3(kCastThreads), 0, s, a);
-    }
-    return e;
+    if (a.type == kElemBF16)
+        return bytes == 16  ? launch_pdl(mx4_quantise_kernel<__nv_bfloat16, 16>, grid, dim3(kCastThreads), 0, s, a)
+               : bytes == 8 ? launch_pdl(mx4_quantise_kernel<__nv_bfloat16, 8>, grid, dim3(kCastThreads), 0, s, a)
+                            : launch_pdl(mx4_quantise_kernel<__nv_bfloat16, 0>, grid, dim3(kCastThreads), 0, s, a);
+    return bytes == 16 ? launch_pdl(mx4_quantise_kernel<float, 16>, grid, dim3(kCastThreads), 0, s, a)
+                       : launch_pdl(mx4_quantise_kernel<float, 0>, grid, dim3(kCastThreads), 0, s, a);
 }
 
 cudaError_t launch_mx4_values(const MxCastArgs& a, int sms, cudaStream_t s) {
     const dim3 grid = cast_grid(a.shape.rows, a.shape.cols, kValuesSpan, sms);
     const int bytes = row_bytes(a.plain, a.shape.rows, a.ld, a.type);
-    cudaError_t e;
-    if (a.type == kElemBF16) {
-        if (bytes == 16) e = launch_pdl(mx4_values_kernel<__nv_bfloat16, 16>, grid, dim3(kCastThreads), 0, s, a);
-        else if (bytes == 8) e = launch_pdl(mx4_values_kernel<__nv_bfloat16, 8>, grid, dim3(kCastThreads), 0, s, a);
-        else if (bytes == 4) e = launch_pdl(mx4_values_kernel<__nv_bfloat16, 4>, grid, dim3(kCastThreads), 0, s, a);
-        else e = launch_pdl(mx4_values_kernel<__nv_bfloat16, 2>, grid, dim3(kCastThreads), 0, s, a);
-    } else {
-        if (bytes == 16) e = launch_pdl(mx4_values_kernel<float, 16>, grid, dim3(kCastThreads), 0, s, a);
-        else if (bytes == 8) e = launch_pdl(mx4_values_kernel<float, 8>, grid, dim3(kCastThreads), 0, s, a);
-        else e = launch_pdl(mx4_values_kernel<float, 4>, grid, dim3(kCastThreads), 0, s, a);
-    }
-    return e;
+    if (a.type == kElemF32) return launch_pdl(mx4_values_kernel<float, 0>, grid, dim3(kCastThreads), 0, s, a);
+    return bytes == 16  ? launch_pdl(mx4_values_kernel<__nv_bfloat16, 16>, grid, dim3(kCastThreads), 0, s, a)
+           : bytes == 8 ? launch_pdl(mx4_values_kernel<__nv_bfloat16, 8>, grid, dim3(kCastThreads), 0, s, a)
+           : bytes == 4 ? launch_pdl(mx4_values_kernel<__nv_bfloat16, 4>, grid, dim3(kCastThreads), 0, s, a)
+                        : launch_pdl(mx4_values_kernel<__nv_bfloat16, 0>, grid, dim3(kCastThreads), 0, s, a);
 }
 
 namespace {
@@ -1112,7 +1150,7 @@ cudaError_t launch_mx4_product(const MxProductArgs& a, int sms, cudaStream_t s) 
     p.x = a.x;
     p.x_ld = a.x_ld;
     p.k = int(a.k);
-    p.x_bytes = a.x ? row_bytes(a.x, a.m, a.x_ld, a.x_type) : 0;
+    p.x_aligned = a.x && row_bytes(a.x, a.m, a.x_ld, a.x_type) == 16;
     const CUtensorMap mw = make_byte_map(a.w_codes, uint64_t(ws.pitch()), uint64_t(a.n), kPTile);
     const CUtensorMap mx = a.x ? mw : make_byte_map(a.x_codes, uint64_t(xs.pitch()), uint64_t(a.m), uint32_t(p.tn));
     const dim3 grid(unsigned(plan.n_tiles * p.splits), unsigned(plan.x_tiles));
