@@ -361,6 +361,11 @@ __global__ void __launch_bounds__(128) sample_warp_kernel(const SampleArgs a) {
 // 178 us. (One CTA a row, its passes reading L2: 375 us, and one row 76 us
 // where a cluster takes 18.)
 //
+// Up to 64 (a warp each of a cluster) top-k needs no histogram: the k-th
+// largest of the warps' maxima bounds the k-th largest logit from below, and
+// what lies above it is the list (8 x 50001 with all filters 12.6 -> 11.2 us,
+// 512 x 131072 top-k 50 and top-p 211 -> 195 us).
+//
 // Lower bounds keep most logits out of the histogram: with k <= the number of
 // groups of threads that hold a logit, the k-th largest is at least the least
 // of the groups' maxima (groups of 1, 2, .. 32 threads: the largest that are
@@ -394,6 +399,7 @@ struct __align__(16) RowShared {
         struct {   // before that: of each warp's groups
             float low[kGroupSizes][kMaxRowWarps];
             int groups[kGroupSizes][kMaxRowWarps];
+            alignas(16) float warp_top[kMaxCluster][kMaxRowWarps];   // each CTA's warps' largest logits
         };
     };
     uint16_t upper[kUpper];                           // the slice's upper columns, a part for each warp
@@ -822,6 +828,11 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
 #pragma unroll
             for (int i = 0; i < int(sizeof(Part) / 4); ++i)
                 if (i < 3 || rp.first_k() > 0) put_u(to + uint32_t(i) * 4, words[i]);
+            if (rp.first_k() > 0) {
+                const uint32_t tops = crew.at(&sh.warp_top[rank][0], lane);
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) put_f(tops + uint32_t(w) * 4, sh.wf[w]);
+            }
         }
         crew.barrier();
         const Part& p = sh.part[lane < ranks ? lane : 0];
@@ -836,6 +847,28 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
                 all.groups[g] = int(__reduce_add_sync(0xFFFFFFFFu, in ? unsigned(p.groups[g]) : 0u));
             }
         }
+    }
+    // The k-th largest of the warps' largest, if k of them hold a logit: a
+    // bound of the k-th largest logit, above which about as many lie (50 of 64
+    // warps over 50001 columns: 100).
+    float kth = neg_inf();
+    static_assert(kSolo || (kWarps == kMaxRowWarps && kThreads == 4 * kMaxCluster * kMaxRowWarps), "four threads for each warp of a cluster");
+    if (!kSolo && rp.first_k() > 0 && rp.first_k() <= ranks * kWarps) {
+        // Four threads count what is above one of them.
+        const int tops = ranks * kWarps, v = t >> 2;
+        const float* const every = &sh.warp_top[0][0];
+        const float mine = v < tops ? every[v] : neg_inf();
+        int above = 0;
+        for (int j = t & 3; j < tops / 4; j += 4) {
+            const float4 f = reinterpret_cast<const float4*>(every)[j];
+            above += (f.x > mine) + (f.y > mine) + (f.z > mine) + (f.w > mine);
+        }
+        above += __shfl_xor_sync(0xFFFFFFFFu, above, 1);
+        above += __shfl_xor_sync(0xFFFFFFFFu, above, 2);
+        const uint32_t low = __reduce_min_sync(0xFFFFFFFFu, v < tops && above < rp.first_k() ? key_of(mine) : 0xFFFFFFFFu);
+        if (lane == 0) sh.wk[warp] = int(low);
+        __syncthreads();
+        kth = logit_of_key(__reduce_min_sync(0xFFFFFFFFu, lane < kWarps ? uint32_t(sh.wk[lane]) : 0xFFFFFFFFu));
     }
     m = all.top;
     int turn = 0;
@@ -860,6 +893,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
             all.valid = int(all.z);
 #pragma unroll
             for (int g = 0; g < kGroupSizes; ++g) all.low[g] = 0.0f;
+            kth = neg_inf();
         }
         const float* noise = a.noise + size_t(row) * size_t(a.noise_ld) + i0;
         const int k = rp.first_k();
@@ -940,6 +974,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
 #pragma unroll
                 for (int g = 0; g < kGroupSizes; ++g)
                     if (k <= all.groups[g]) l = all.low[g];
+                l = fmaxf(l, kth);
                 sure = low = fmaxf((l - m) * c, -40.0f);
             } else {
                 sure = fmaxf(__log2f((1.0f - rp.top_p) * 0.99f * all.z / float(a.cols)), -40.0f);
@@ -993,39 +1028,49 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
             // the mass that the cut is taken from. `final`: the last filter, so
             // that what lies above its cut is raced on the way. (sh.first,
             // sh.last and sh.list_n are at their starts before it.)
-            const auto settle = [&](int count, float target, bool final, float* kept) -> bool {
+            // direct: without a histogram, the logits of at least kth are the list.
+            const auto settle = [&](int count, float target, bool final, float* kept, bool direct) -> bool {
+                int first = 0, last = kBins;
+                bool whole = true;
+                if (!direct) {
 #pragma unroll
-                for (int j = 0; j < Sums<Crew>::kPer; ++j) {
-                    const int b = t * Sums<Crew>::kPer + j;
-                    if (count > 0) {
-                        if (upto.n[j] >= uint32_t(count) && upto.n[j] - upto.own_n[j] < uint32_t(count)) sh.first = sh.last = b;
-                    } else {
-                        // A fixed-point sum is off by half a unit a logit, and by
-                        // the masses' own rounding, a few 2^-22 of it.
-                        const float goal = target * fixed, slack = 0.5f * float(upto.n[j]) + 4096.0f, w = float(upto.w[j]);
-                        if (w + slack >= goal) atomicMin(&sh.first, b);
-                        if (w - slack >= goal) atomicMin(&sh.last, b);
+                    for (int j = 0; j < Sums<Crew>::kPer; ++j) {
+                        const int b = t * Sums<Crew>::kPer + j;
+                        if (count > 0) {
+                            if (upto.n[j] >= uint32_t(count) && upto.n[j] - upto.own_n[j] < uint32_t(count)) sh.first = sh.last = b;
+                        } else {
+                            // A fixed-point sum is off by half a unit a logit, and by
+                            // the masses' own rounding, a few 2^-22 of it.
+                            const float goal = target * fixed, slack = 0.5f * float(upto.n[j]) + 4096.0f, w = float(upto.w[j]);
+                            if (w + slack >= goal) atomicMin(&sh.first, b);
+                            if (w - slack >= goal) atomicMin(&sh.last, b);
+                        }
                     }
-                }
-                __syncthreads();
-                int first = sh.first;
-                const int last = sh.last;
-                if (last >= kBins) return false;
+                    __syncthreads();
+                    first = sh.first;
+                    last = sh.last;
+                    if (last >= kBins) return false;
 #pragma unroll
-                for (int j = 0; j < Sums<Crew>::kPer; ++j) {
-                    const int b = t * Sums<Crew>::kPer + j;
-                    if (b == last) sh.down = upto.n[j];
-                    if (b == first) sh.above = upto.n[j] - upto.own_n[j];
+                    for (int j = 0; j < Sums<Crew>::kPer; ++j) {
+                        const int b = t * Sums<Crew>::kPer + j;
+                        if (b == last) sh.down = upto.n[j];
+                        if (b == first) sh.above = upto.n[j] - upto.own_n[j];
+                    }
+                    __syncthreads();
+                    // Few enough down to the cut: all of them are listed, and raced there.
+                    whole = sh.down <= uint32_t(kList);
+                    if (!whole && sh.down - sh.above > uint32_t(kList)) return false;
+                    if (whole) first = 0;
                 }
-                __syncthreads();
-                // Few enough down to the cut: all of them are listed, and raced there.
-                const bool whole = sh.down <= uint32_t(kList);
-                if (!whole && sh.down - sh.above > uint32_t(kList)) return false;
-                if (whole) first = 0;
                 Weighed s{0, 0.0f};
                 // A column's bin against the cut's: above it is kept for certain
                 // (and raced if no filter follows).
                 const auto place_in = [&](float l, int i) -> bool {
+                    if (direct) {
+                        const unsigned to = atomicAdd(&sh.list_n, 1u);
+                        if (to < unsigned(kList)) list[to] = place_of(key_of(l), i0 + i);
+                        return false;
+                    }
                     const float y = (l - m) * c;
                     if (!(y >= low)) return false;
                     const int b = bin_of(y);
@@ -1038,7 +1083,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
                     return false;
                 };
                 if (upper_n < 0) {
-                    sl.each_above(logit_below(fmaxf(low, -float(last + 2) / steps)), [&](float l, int i) {
+                    sl.each_above(direct ? kth : logit_below(fmaxf(low, -float(last + 2) / steps)), [&](float l, int i) {
                         if (place_in(l, i)) run_race(l, i0 + i, __ldg(noise + i));
                     });
                 } else {
@@ -1073,6 +1118,13 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
 #pragma unroll
                 for (int r = 0; r < kMaxCluster; ++r)
                     if (r < ranks) of_rank[r] = int(get_u(crew.at(&sh.list_n, r)));
+                if (direct) {
+                    int all_lists = 0;
+#pragma unroll
+                    for (int r = 0; r < kMaxCluster; ++r)
+                        if (r < ranks) all_lists += min(of_rank[r], kList + 1);
+                    if (all_lists > kList) return false;
+                }
 #pragma unroll
                 for (int r = 0; r < kMaxCluster; ++r)
                     if (r < ranks) {
@@ -1163,17 +1215,24 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
             };
             float kept = all.z;
             bool settled = false, count_now = true, k_stage = by_k;
-            for (;;) {
+            if (!kSolo && by_k && kth > neg_inf()) {
+                if (t == 0) sh.list_n = 0;
+                upper_n = sl.list_above(kth, part);
+                __syncthreads();
+                settled = settle(k, 0.0f, true, &kept, true);
+                if (!settled) crew.barrier();   // every CTA is past its reads of this one's count
+            }
+            while (!settled) {
                 if (count_now) count_bins();
                 count_now = false;
-                settled = settle(k_stage ? k : 0, rp.top_p * kept, !k_stage || !by_p, &kept);
+                settled = settle(k_stage ? k : 0, rp.top_p * kept, !k_stage || !by_p, &kept, false);
                 if (!settled) {
                     if (k_stage || !(low > sure) || sh.last < kBins) break;
                     low = sure;   // the cut lies lower than was tried
                     count_now = true;
                 } else {
                     if (!k_stage || !by_p || raced) break;
-                    k_stage = false;
+                    settled = k_stage = false;
                 }
                 crew.barrier();   // every CTA is past its reads of this one's lists
                 if (t == 0) sh.first = sh.last = kBins, sh.list_n = 0;
