@@ -331,8 +331,8 @@ dim3 cast_grid(long long rows, long long cols, int span, int sms) {
 //
 // Few rows of x are bound by w's bytes and, at these sizes, by what comes
 // before and after them: 32 x 16384 x 4096 in 9.1 us with x's quantisation
-// (37 MB; 5.6 us at the rate of a copy), 1 x 4096 x 4096 in 5.0 us. Products
-// in between (333 x 1111 x 2501 in 12.5 us with x's quantisation) have too few
+// (37 MB; 5.6 us at the rate of a copy), 1 x 4096 x 4096 in 4.8 us. Products
+// in between (333 x 1111 x 2501 in 10.2 us with x's quantisation) have too few
 // tiles to fill the SMs and run at the latency of a tile's K.
 struct ProductTile {
     int m, n;              // rows of x, rows of w
@@ -479,9 +479,9 @@ struct PlainBlock {
 
 constexpr int kPEpiThreads = kPThreads - 64;
 // Up to so many rows, and chunks of K a CTA, a plain x is quantised by the
-// product's CTAs: 1 x 4096 x 4096 6.7 us so and 8.1 us with a launch before it
-// (16 rows: 8.4 and 8.8), and the launch's host time is saved. With 32 rows
-// 9.9 and 9.0, with 64 14.0 and 10.8.
+// product's CTAs: 1 x 4096 x 4096 4.8 us so and 6.3 us with a launch before it
+// (16 rows: 6.6 and 6.5), and the launch's host time is saved. With 32 rows
+// 8.9 and 7.0.
 constexpr int kPPlainRows = 16, kPPlainChunks = 8;
 
 // kGroups: scale tiles of 128 rows of x (tn <= 128: 1, else 2). X: void, or
@@ -539,8 +539,8 @@ __global__ void __launch_bounds__(kPThreads)
         if (p.early_w) grid_dependency_wait();
         // A call of one launch lets the next one's CTAs in at once (1 x 4096 x
         // 4096 5.0 us so, 5.7 without); behind a product with a quantisation
-        // before it the next quantisation's blocks would only hold SMs that
-        // this one's stores are waited on for (333 x 1111 x 2501 14.9, 12.5).
+        // before it the next quantisation's blocks only take up SMs (333 x 1111
+        // x 2501 11.0 us so, 10.2 without).
         if constexpr (kPlain) grid_launch_dependents();
         for (int i = 0; i < ahead; ++i) load_x(c_begin + i, i);
     }
@@ -748,8 +748,8 @@ struct PairTile {
 };
 
 // From so many tiles, and more than 128 rows on either side: 64 tiles of
-// 1024 x 4096 x 2048 9.9 us by pairs and 16.2 us without, 32 of 512 x 4096 x
-// 4096 12.5 and 10.7.
+// 1024 x 4096 x 2048 11.6 us by pairs and 16.9 us without, 32 of 512 x 4096 x
+// 4096 12.9 and 11.7 (with x's quantisation).
 constexpr int kPairFromTiles = 48;
 constexpr int kPairThreads = 320, kPairEpiWarps = 8, kPairStages = 5;
 constexpr uint32_t kPairBox = 32 * 128;   // an epilogue warp's rows on their way out
@@ -1097,10 +1097,10 @@ ProductPlan plan_of(long long m, long long n, long long k) {
     p.x_tiles = int((m + p.tn - 1) / p.tn);
     // Up to 64 columns a CTA takes half an SM's memory. K is shared by a
     // cluster of CTAs while there are SMs for them (over a long K two CTAs an
-    // SM, so that one's waits fill the other's: 1 x 8192 x 8192 8.2 us so, 8.9
-    // us with one; 64 x 4096 x 4096 9.0 and 7.6), every CTA keeps a chunk or
+    // SM, so that one's waits fill the other's: 1 x 8192 x 8192 6.9 us so, 10.3
+    // us with one; 64 x 4096 x 4096 9.2 and 7.9), every CTA keeps a chunk or
     // more and there are enough of them to pay for the exchange (1024 x 362 x
-    // 722, three chunks: 6.4 us in one piece, 8.7 us in two).
+    // 722, three chunks: 6.8 us in one piece, 9.1 us in two).
     const int slots = p.tn <= 64 && chunks >= 32 ? 2 * kSms : kSms;
     p.splits = 1;
     while (chunks >= 4 && p.splits < kPMaxSplits && (long long)p.n_tiles * p.x_tiles * p.splits * 2 <= slots &&
