@@ -16,7 +16,7 @@
 // weighing the logits at or above the middle, until one logit (or one group
 // of equal ones) is left in the range (rows beyond a warp: mostly from a
 // histogram). Counts are exact and sums run in a fixed order, so a row's move
-// does not depend on the batch or the run.
+// does not depend on the run or on the other rows.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -339,9 +339,9 @@ __global__ void __launch_bounds__(128) sample_warp_kernel(const SampleArgs a) {
 // More columns: a cluster of CTAs per row, each with a slice of the columns
 // in shared memory, so that the logits cross HBM once however many passes
 // the filters need. (A slice too long for that is read again from global
-// memory: kResident false.) The number of CTAs follows from the columns
-// alone, so a row's sums, and with them its result's bits, do not depend on
-// the batch.
+// memory: kResident false.) The number of CTAs follows from the columns, and
+// beyond 16384 from whether there are many rows: the only way in which the
+// order of a row's sums, and with it their last bits, depends on the batch.
 //
 // A filter's threshold is found from a histogram of the upper logits in
 // kBins equal steps of log w, each bin with its count and its mass in fixed
@@ -1371,6 +1371,8 @@ cudaError_t launch_rows(const SampleArgs& a, int ranks, int per, size_t smem, cu
     return cudaLaunchKernelEx(&cfg, kernel, a, ranks, per);
 }
 
+constexpr int kRowCtas = 384;   // that run at once: 48 clusters of eight
+
 template <typename T>
 cudaError_t launch_sample_t(const SampleArgs& a, cudaStream_t s) {
     const int grid = int((a.rows + 3) / 4);
@@ -1379,10 +1381,14 @@ cudaError_t launch_sample_t(const SampleArgs& a, cudaStream_t s) {
         if (a.cols <= 384) return launch_pdl(sample_warp_kernel<T, 12>, dim3(unsigned(grid)), dim3(128), 0, s, a);
         return launch_pdl(sample_warp_kernel<T, 32>, dim3(unsigned(grid)), dim3(128), 0, s, a);
     }
-    // Up to 16384 columns one CTA has the row (1024 rows of 16384: 45 us, with
-    // two of 8192 each 75 us); beyond, slices of at most 8192 while eight CTAs
-    // can hold the row so (8 rows of 50001: 13 us, with 16384 19 us).
-    const int ranks = a.cols <= 16384 ? 1 : a.cols <= 32768 ? 4 : kMaxCluster;
+    // Up to 16384 columns one CTA has the row (512 rows of 16384, top-p: 26 us,
+    // with two of 8192 each 42 us); beyond, slices of at most 8192 while eight
+    // CTAs can hold the row so (8 rows of 50001: 14 us, with 16384 16 us). Where
+    // not all of those run at once, up to 65536 columns, a row has half as many
+    // CTAs (512 rows of 50001: 174 us with eight, 102 us with four; 64 rows 30
+    // and 20), and its sums another order.
+    int ranks = a.cols <= 16384 ? 1 : a.cols <= 32768 ? 4 : kMaxCluster;
+    if (ranks > 1 && a.cols <= 65536 && a.rows * ranks > kRowCtas) ranks /= 2;
     const int per = (a.cols + ranks - 1) / ranks;
     const size_t smem = size_t(per) * sizeof(T) + 32;   // up to 16 bytes of alignment at either end
     if (a.cols <= 8192) return launch_rows<T, true, 128, true>(a, 1, per, smem, s);

@@ -316,7 +316,10 @@ int azb_mx4_linear(int device, const void* x, int x_type, long long m, long long
  * kept ones' distribution when the noise is uniform on (0, 1). logprob (may
  * be null) is x[move] - log(sum exp(x)) over all of l. A temperature of 0 or
  * less, or NaN, takes the first largest logit, logprob 0. A row without any l
- * gives -1 and -inf. A row's result does not depend on the other rows. */
+ * gives -1 and -inf. A row's result does not depend on the other rows; beyond
+ * 16384 columns its sums are taken in one order in small batches and in
+ * another in large ones (from 49 to 97 rows on), which may show in logprob's
+ * last bits and where two keys or a cut are as close. */
 typedef struct azb_sample_args {
     const void* logits;              /* [rows][cols], AZB_ELEM_* */
     int type;

@@ -135,6 +135,19 @@ def test_wide_rows(ops, torch, cols, dtype):
     check(ops, torch, logits, noise, legal, dtype, top_k=3000, top_p=0.999)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("cols", [16385, 32768, 50001, 65536])
+def test_many_wide_rows(ops, torch, cols, dtype):
+    """More rows than run at once: fewer CTAs a row."""
+    logits, noise, r = data(cols, 110, cols)
+    legal = r.random((110, cols)) < 0.6
+    legal[3], legal[7, 1:] = False, False
+    check(ops, torch, logits, noise, legal, dtype)
+    check(ops, torch, logits, noise, None, dtype, top_p=0.9)
+    check(ops, torch, logits, noise, legal, dtype, top_k=16, top_p=0.95, min_p=0.01, temperature=0.7)
+    check(ops, torch, logits, noise, None, dtype, top_k=40)
+
+
 @pytest.mark.parametrize("cols", [600001, 900001])
 def test_widest_rows_bfloat16(ops, torch, cols):
     """Slices beyond 16-bit places, and beyond shared memory, in the shorter type."""
