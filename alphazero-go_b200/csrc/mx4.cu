@@ -179,8 +179,8 @@ __device__ __forceinline__ size_t scale_offset(const MxShape& s, long long row, 
 // fp32 108 us so and 277 us by elements, of bfloat16 67 and 150), but for
 // bfloat16 rows at multiples of 8, which take loads of 8 (59 us and 66).
 //
-// Bound by DRAM where the matrix is large: 16384 x 8192 of bfloat16 in 53 us
-// with nothing in L2 (5.4 TB/s of 268 MB read and the codes written). Five
+// Bound by DRAM where the matrix is large: 16384 x 8192 of bfloat16 in 50 us
+// with nothing in L2 (5.8 TB/s of 268 MB read and the codes written). Five
 // blocks an SM (at most 51 registers) and two steps in flight: there and back
 // 113 us, with four blocks 3 us more. Few rows are bound by the launch: 3 us.
 constexpr int kCastThreads = 256, kCastWarps = kCastThreads / 32, kCastStep = 512;
@@ -228,10 +228,10 @@ __global__ void __launch_bounds__(kCastThreads, 5) mx4_quantise_kernel(const MxC
 // fp32, and of bfloat16 in rows of odd places (kBytes 0), are exchanged so
 // that neighbouring lanes store neighbouring elements (16384 x 8192 of fp32 99
 // us, two stores of 16 bytes a lane 142; 16384 x 8191 108 us, by single
-// elements of a lane 518, of bfloat16 83 and 369). A value is a code's magnitude times a
-// power of two: exact in either type (the smallest, 2^-128, is a subnormal
-// that both hold). Bound by DRAM too: 16384 x 8192 into bfloat16 in 60 us
-// (5.7 TB/s of 71 MB read and 268 MB written).
+// elements of a lane 518, of bfloat16 83 and 369). A value is a code's
+// magnitude times a power of two: exact in either type (the smallest, 2^-128,
+// is a subnormal that both hold). Bound by DRAM too: 16384 x 8192 into
+// bfloat16 in 56 us (6.1 TB/s of 71 MB read and 268 MB written).
 constexpr int kValuesUnroll = 4, kValuesStep = 256, kValuesSpan = kValuesStep * kValuesUnroll;
 
 // The magnitude's three bits on top of a float's significand and exponent are
