@@ -352,13 +352,13 @@ __global__ void __launch_bounds__(128) sample_warp_kernel(const SampleArgs a) {
 // above. Where the list would be longer (many equal logits, say) the range of
 // keys is halved as in find_threshold, over the listed upper logits.
 //
-// 512 rows of 131072 (fp32, top-p 0.9) take 270 us: 469 MB from DRAM (the
+// 512 rows of 131072 (fp32, top-p 0.9) take 268 us: 469 MB from DRAM (the
 // kept columns' numbers come in sectors of 32 bytes), a fifth of its rate. A
 // CTA lives 25 us, of which the load takes 3.4, the sum 1.9, the first
 // exchange 2.2, the list and histogram 5.1 with their exchange, the cut 9
 // with four more; three CTAs an SM (their slices fill it) overlap these, the
 // barriers of a cluster's eight being what is waited for. Without filters
-// 178 us. (One CTA a row, its passes reading L2: 375 us, and one row 76 us
+// 177 us. (One CTA a row, its passes reading L2: 375 us, and one row 76 us
 // where a cluster takes 18.)
 //
 // Up to 64 (a warp each of a cluster) top-k needs no histogram: the k-th
@@ -515,40 +515,60 @@ struct Slice {
     template <class F>
     __device__ __forceinline__ void load(F f) {
         if constexpr (kResident) {
-            const uint4* base = reinterpret_cast<const uint4*>(src - shift);
-            const int np = packs();
-            constexpr int kAhead = 8;
-            for (int v0 = int(threadIdx.x); v0 < np; v0 += kThreads * kAhead) {
-                P p[kAhead];
-#pragma unroll
-                for (int u = 0; u < kAhead; ++u) {
-                    const int v = v0 + u * kThreads, i = v * W - shift;
-                    if (v < np && i >= 0 && i + W <= n) p[u].q = __ldg(base + v);
-                }
-#pragma unroll
-                for (int u = 0; u < kAhead; ++u) {
-                    const int v = v0 + u * kThreads, i = v * W - shift;
-                    if (v >= np) continue;
-                    if (i < 0 || i + W > n) {
-#pragma unroll
-                        for (int e = 0; e < W; ++e) {
-                            p[u].drop(e);
-                            if (i + e >= 0 && i + e < n) reinterpret_cast<T*>(&p[u].q)[e] = src[i + e];
-                        }
-                    }
-                    p[u].clean();
-                    if (legal) {
-#pragma unroll
-                        for (int e = 0; e < W; ++e)
-                            if (i + e >= 0 && i + e < n && !legal[i + e]) p[u].drop(e);
-                    }
-                    mem[v] = p[u];
-#pragma unroll
-                    for (int e = 0; e < W; ++e) f(p[u].get(e));
-                }
-            }
+            if (legal) load_as<true>(f);
+            else load_as<false>(f);
         } else {
             for (int i = int(threadIdx.x); i < n; i += kThreads) f(direct(i));
+        }
+    }
+    template <bool kLegal, class F>
+    __device__ __forceinline__ void load_as(F f) {
+        const uint4* base = reinterpret_cast<const uint4*>(src - shift);
+        const int np = packs();
+        // Packs under way at once, and the words that hold a pack's legality
+        // (a byte each, at any place: one more word than their number).
+        constexpr int kAhead = kLegal ? 4 : 8, kFours = W / 4;
+        const int off = kLegal ? int(reinterpret_cast<uintptr_t>(legal - shift) & 3) : 0;
+        for (int v0 = int(threadIdx.x); v0 < np; v0 += kThreads * kAhead) {
+            P p[kAhead];
+            uint32_t open[kAhead][kFours + 1];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int v = v0 + u * kThreads, i = v * W - shift;
+                if (v < np && i >= 0 && i + W <= n) p[u].q = __ldg(base + v);
+                if (kLegal && v < np && i >= off && i - off + W + 4 <= n) {
+                    const uint32_t* words = reinterpret_cast<const uint32_t*>(legal + i - off);
+#pragma unroll
+                    for (int w = 0; w <= kFours; ++w) open[u][w] = __ldg(words + w);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int v = v0 + u * kThreads, i = v * W - shift;
+                if (v >= np) continue;
+                if (i < 0 || i + W > n) {
+#pragma unroll
+                    for (int e = 0; e < W; ++e) {
+                        p[u].drop(e);
+                        if (i + e >= 0 && i + e < n) reinterpret_cast<T*>(&p[u].q)[e] = src[i + e];
+                    }
+                }
+                p[u].clean();
+                if (kLegal && i >= off && i - off + W + 4 <= n) {
+#pragma unroll
+                    for (int e = 0; e < W; ++e) {
+                        const uint32_t four = __funnelshift_r(open[u][e / 4], open[u][e / 4 + 1], 8 * off);
+                        if (!(four >> (8 * (e & 3)) & 0xFFu)) p[u].drop(e);
+                    }
+                } else if (kLegal) {
+#pragma unroll
+                    for (int e = 0; e < W; ++e)
+                        if (i + e >= 0 && i + e < n && !legal[i + e]) p[u].drop(e);
+                }
+                mem[v] = p[u];
+#pragma unroll
+                for (int e = 0; e < W; ++e) f(p[u].get(e));
+            }
         }
     }
     // f(l, i) for this thread's logits (and some of -inf around the slice).
