@@ -921,15 +921,16 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
         uint64_t cut = place_of(kKeyLow, 0x7FFFFFFF);   // the last place kept
         bool raced = false;
         // A warp's race of kN columns a lane, those with a bit in `in`. With
-        // d = 1 - u: d <= -log u <= d / u, so that in log2 a column's key lies
-        // between reach and reach + lg2(u). The two logarithms (accurate, where
-        // the bounds' are approximate: the margins) are taken only where the
-        // upper bound reaches the warp's best so far, at first its best lower
-        // bound. ok(l, i): whether a column is in the race after all.
+        // d = 1 - u, u clamped as the key's is: d <= -log u <= d / u, so that in
+        // log2 a column's key lies between reach and reach + lg2(u). The two
+        // logarithms (accurate, where the bounds' are approximate: the margins)
+        // are taken only where the upper bound reaches the warp's best so far,
+        // at first its best lower bound. ok(l, i): whether a column is in the
+        // race after all.
         float lead = neg_inf();
         const auto race_some = [&](auto n, const float* l, const float* u, uint32_t in, auto column, auto ok) {
             constexpr int kN = decltype(n)::value;
-            const auto reach = [&](int g) { return (l[g] - m) * c - lg2(fmaxf(1.0f - u[g], 5.9604645e-8f)); };
+            const auto reach = [&](int g) { return (l[g] - m) * c - lg2(1.0f - clamped(u[g])); };
             if (lead == neg_inf()) {
                 float least = neg_inf();
 #pragma unroll

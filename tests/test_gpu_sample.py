@@ -392,3 +392,27 @@ def test_refusals_and_empty(ops, torch):
             call()
     m, lp = ops.sample_moves(l[:0], n[:0])
     assert m.shape == lp.shape == (0,)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("cols", [362, 1024, 5000, 16384, 50001, 450001])
+def test_noise_out_of_range_is_clamped(ops, torch, cols, dtype):
+    """Numbers outside (0, 1) are read as its ends, wherever they stand and
+    whatever stands beside them."""
+    logits, noise, r = data(cols + 1, 6, cols)
+    kind = r.random((6, cols))
+    for i, odd in enumerate((np.nan, -0.5, -20.0, -1e9, -np.inf)):
+        noise[(kind >= 0.15 * i) & (kind < 0.15 * i + 0.15)] = odd
+    at = r.integers(0, cols, 6)
+    noise[np.arange(6), at] = [1.0, 2.0, 1e9, np.inf, 0.0, 1.0]
+    logits[0], noise[0] = 0.0, -100.0                 # the same number everywhere: the largest logit
+    logits[0, cols - 3] = 1.0
+    logits[1, :] = -9.0                               # the largest logit's is the lowest, another's ordinary
+    noise[1, :] = np.nan
+    logits[1, [2, cols - 5]] = [0.0, -2.0]
+    noise[1, cols - 5] = 0.5
+    for f in (dict(), dict(top_k=40), dict(top_p=0.9), dict(min_p=0.05), dict(top_k=50, top_p=0.95, temperature=0.7)):
+        m, _ = check(ops, torch, logits, noise, None, dtype, **f)
+        assert m[0] == cols - 3
+        if f.get("top_p", 1.0) == 1.0:
+            assert m[1] == cols - 5
