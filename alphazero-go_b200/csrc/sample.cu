@@ -147,7 +147,7 @@ __device__ Threshold find_threshold(const RowParams& rp, uint32_t top, uint32_t 
             kept = above + (kept - above) * (float(th.ties) / float(clo - chi));
         }
     }
-    if (rp.filters_p()) {
+    if (rp.filters_p() && k != 1) {   // (a row with one logit, or a top-p of 0 or less, is settled)
         const float target = rp.top_p * kept;
         uint32_t lo = max(low_p, th.key), hi = top + 1;   // mass(lo) >= target > mass(hi)
         Weighed wlo = at(lo), whi{0, 0.0f};

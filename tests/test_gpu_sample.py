@@ -416,3 +416,16 @@ def test_noise_out_of_range_is_clamped(ops, torch, cols, dtype):
         assert m[0] == cols - 3
         if f.get("top_p", 1.0) == 1.0:
             assert m[1] == cols - 5
+
+
+@pytest.mark.parametrize("cols", [1, 5, 362, 1024, 1025, 5000, 50001])
+def test_per_row_top_p_below_zero_keeps_the_first(ops, torch, cols):
+    logits, noise, _ = data(cols, 10, cols)
+    legal = np.ones((10, cols), bool)
+    legal[:5] = False
+    legal[np.arange(5), [0, cols - 1, cols // 2, 0, cols - 1]] = True
+    p = np.tile(np.array([-0.5, -5.0, -1e30, -np.inf, 0.0], np.float32), 2)
+    for k in (0, 1, 7):
+        m, lp = run(ops, torch, logits, noise, legal, top_p=p, top_k=k)
+        assert np.array_equal(m, np.where(legal, logits, -np.inf).argmax(1)), (k, m)
+        assert (lp[:5] == 0).all()
