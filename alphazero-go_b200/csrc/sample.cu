@@ -61,9 +61,12 @@ __device__ __forceinline__ float lg2(float x) {   // x >= 2^-25
     return r;
 }
 
-// w = 2^((l - m) c). The bounds keep 0 * c and -inf * c what they should be
+// w = 2^((l - m) c). The bounds (the least positive number, and what a
+// temperature of 5e-39 gives) keep 0 * c and -inf * c what they should be
 // whatever the temperature.
-__device__ __forceinline__ float log2_scale(float temperature) { return fminf(fmaxf(kLog2e / temperature, 1e-38f), 3e38f); }
+__device__ __forceinline__ float log2_scale(float temperature) {
+    return fminf(fmaxf(kLog2e / temperature, __uint_as_float(1u)), 3e38f);
+}
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll

@@ -306,20 +306,21 @@ int azb_mx4_linear(int device, const void* x, int x_type, long long m, long long
                    void* workspace, size_t workspace_bytes, void* stream, char* err, size_t err_cap);
 
 /* One move per row of logits. With l the legal, non-NaN logits above -inf and
- * m their maximum: x = 0 where l = m, else (l - m) / temperature. In
- * descending order of l (ties: lower column first) top_k keeps the first k
- * (0 or less: off), top_p of those the shortest prefix whose share of their
- * mass sum exp(x) reaches p (1 or more: off), min_p those with exp(x) >=
- * min_p (0 or less: off); the first is always kept. The move is the kept
- * column with the largest x - log(-log u), u its noise clamped into [2^-25,
- * 1 - 2^-24] (a NaN: the lowest), ties to the lower column: a draw from the
- * kept ones' distribution when the noise is uniform on (0, 1). logprob (may
- * be null) is x[move] - log(sum exp(x)) over all of l. A temperature of 0 or
- * less, or NaN, takes the first largest logit, logprob 0. A row without any l
- * gives -1 and -inf. A row's result does not depend on the other rows; beyond
- * 16384 columns its sums are taken in one order in small batches and in
- * another in large ones (from 49 to 97 rows on), which may show in logprob's
- * last bits and where two keys or a cut are as close. */
+ * m their maximum: x = 0 where l = m, else (l - m) / temperature (l - m in
+ * fp32; a temperature below 5e-39 counts as that). In descending order of l
+ * (ties: lower column first) top_k keeps the first k (0 or less: off), top_p
+ * of those the shortest prefix whose share of their mass sum exp(x) reaches p
+ * (1 or more: off), min_p those with exp(x) >= min_p (0 or less: off); the
+ * first is always kept. The move is the kept column with the largest
+ * x - log(-log u), u its noise clamped into [2^-25, 1 - 2^-24] (a NaN: the
+ * lowest), ties to the lower column: a draw from the kept ones' distribution
+ * when the noise is uniform on (0, 1). logprob (may be null) is
+ * x[move] - log(sum exp(x)) over all of l. A temperature of 0 or less, or NaN,
+ * takes the first largest logit, logprob 0. A row without any l gives -1 and
+ * -inf. A row's result does not depend on the other rows; beyond 16384 columns
+ * its sums are taken in one order in small batches and in another in large
+ * ones (from 49 to 97 rows on), which may show in logprob's last bits and
+ * where two keys or a cut are as close. */
 typedef struct azb_sample_args {
     const void* logits;              /* [rows][cols], AZB_ELEM_* */
     int type;

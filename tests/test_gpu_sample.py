@@ -429,3 +429,22 @@ def test_per_row_top_p_below_zero_keeps_the_first(ops, torch, cols):
         m, lp = run(ops, torch, logits, noise, legal, top_p=p, top_k=k)
         assert np.array_equal(m, np.where(legal, logits, -np.inf).argmax(1)), (k, m)
         assert (lp[:5] == 0).all()
+
+
+@pytest.mark.parametrize("cols", [40, 362, 3000, 20000])
+def test_extreme_temperatures(ops, torch, cols):
+    """Temperatures near the type's ends, with logits as far apart."""
+    r = np.random.default_rng(cols)
+    noise = r.random((6, cols), np.float32)
+    unit = r.standard_normal((6, cols)).astype(np.float32)
+    unit = np.clip(unit, -3, 3) / 3
+    for t, scale in ((3.4e38, 1.6e38), (2e38, 1.6e38), (1.5e38, 1e38), (1e37, 1e37), (1e-30, 1e-30), (2e-37, 1e-36)):
+        for f in (dict(), dict(top_k=5), dict(top_p=0.8), dict(min_p=0.5)):
+            check(ops, torch, unit * np.float32(scale), noise, temperature=t, **f)
+    inf = np.array([np.inf, 1.0, np.inf, 1.0, np.inf, np.inf], np.float32)   # per row: every logit the same
+    logits = np.where(r.random((6, cols)) < 0.5, np.float32(-np.inf), unit)
+    m, lp = run(ops, torch, logits, noise, temperature=inf)
+    for i in np.flatnonzero(np.isinf(inf)):
+        n = np.isfinite(logits[i]).sum()
+        assert np.isfinite(logits[i, m[i]]) and abs(lp[i] + np.log(n)) <= 1e-5
+        assert m[i] == np.where(np.isfinite(logits[i]), noise[i], -1).argmax()
