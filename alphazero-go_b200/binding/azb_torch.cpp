@@ -15,6 +15,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -105,9 +106,11 @@ struct Matrix {
     const void* at;
 };
 
-// A gradient would be lost: there is no backward pass.
+// A gradient, or a forward-mode tangent, would be lost: there is no backward
+// pass.
 void no_gradient(const at::Tensor& t, const char* what) {
-    require(!(t.requires_grad() && c10::GradMode::is_enabled()),
+    const bool tangent = t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode();
+    require(!tangent && !(t.requires_grad() && c10::GradMode::is_enabled()),
             std::string(what) + " requires a gradient, and there is no backward pass (detach it)");
 }
 
@@ -275,6 +278,7 @@ const void* beside(PyObject* o, const char* name, const at::Tensor& logits, cons
     require((t.size(1) == 1 || t.stride(1) == 1) && t.device() == logits.device(),
             std::string(name) + ": adjacent columns on " + name_of(logits.device()) + " are needed (stride " +
                 std::to_string(t.stride(1)) + "; it is on " + name_of(t.device()) + ")");
+    no_gradient(t, name);
     *ld = t.stride(0);
     return t.const_data_ptr();
 }

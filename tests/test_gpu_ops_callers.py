@@ -1,0 +1,38 @@
+"""Callers of the device operators (include/azb200.h, "device operators")
+beside the plain one: torch's ways of following a computation, which these
+calls cannot take part in and therefore refuse."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops(engine):
+    import azb_ops
+
+    return azb_ops
+
+
+def test_a_lost_gradient_is_refused(ops):
+    """Forward-mode tangents and the noise's gradient as any other gradient."""
+    import torch
+    import torch.autograd.forward_ad as fw
+
+    x, b = torch.ones(4, 64, device="cuda"), torch.ones(4, device="cuda")
+    w = ops.mx4_quantise(x)
+    noise = torch.rand(4, 64, device="cuda")
+    with fw.dual_level():
+        d = fw.make_dual(x, torch.ones_like(x))
+        for call in (lambda: ops.mx4_quantise(d), lambda: ops.mx4_product(d, w), lambda: ops.mx4_product(d[0], w),
+                     lambda: ops.mx4_product(x, w, bias=fw.make_dual(b, b)), lambda: ops.sample_moves(d, noise),
+                     lambda: ops.sample_moves(x, noise, temperature=fw.make_dual(b, b)),
+                     lambda: ops.sample_moves(x, fw.make_dual(noise, noise))):
+            with pytest.raises(ValueError, match="no backward pass"):
+                call()
+        ops.mx4_product(fw.unpack_dual(d).primal, w)
+        with fw._set_fwd_grad_enabled(False):
+            ops.mx4_quantise(d)
+    with pytest.raises(ValueError, match="noise requires a gradient"):
+        ops.sample_moves(x, noise.clone().requires_grad_())
+    with torch.no_grad():
+        ops.sample_moves(x, noise.clone().requires_grad_())
