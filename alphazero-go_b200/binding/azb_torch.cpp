@@ -106,19 +106,20 @@ struct Matrix {
     const void* at;
 };
 
-// A gradient, or a forward-mode tangent, would be lost: there is no backward
-// pass.
-void no_gradient(const at::Tensor& t, const char* what) {
+// That a tensor's memory holds its values, and that nothing follows them. A
+// gradient, or a forward-mode tangent, would be lost: there is no backward pass.
+void check_source(const at::Tensor& t, const char* what) {
     const bool tangent = t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode();
     require(!tangent && !(t.requires_grad() && c10::GradMode::is_enabled()),
             std::string(what) + " requires a gradient, and there is no backward pass (detach it)");
+    require(!t.is_neg(), std::string(what) + " is a view of negated memory (resolve_neg it)");
 }
 
 Matrix matrix(const at::Tensor& t, const char* what) {
     Matrix m{};
     m.type = elem_type(t.scalar_type(), what);
     require(t.dim() == 2, std::string(what) + ": a matrix is needed, not " + std::to_string(t.dim()) + " dimensions");
-    no_gradient(t, what);
+    check_source(t, what);
     m.rows = t.size(0);
     m.cols = t.size(1);
     require(m.cols >= 1, std::string(what) + ": at least one column is needed");
@@ -222,7 +223,7 @@ PyObject* mx4_product(PyObject*, PyObject* const* args, Py_ssize_t n) {
             require(fits, "bias: " + std::to_string(w.rows) + " adjacent float32 numbers are needed");
             const at::Tensor& b = THPVariable_Unpack(args[6]);
             require(b.device() == device, "x is on " + name_of(device) + ", bias on " + name_of(b.device()));
-            no_gradient(b, "bias");
+            check_source(b, "bias");
             bias = static_cast<const float*>(b.const_data_ptr());
         }
         const int relu = PyObject_IsTrue(args[7]);
@@ -262,7 +263,7 @@ void setting(PyObject* o, const char* name, long long rows, const at::Device& de
     require(t.scalar_type() == type && t.dim() == 1 && t.size(0) == rows && t.device() == device && t.is_contiguous(),
             std::string(name) + ": a number, or " + std::to_string(rows) + " adjacent " + type_name + " numbers on " +
                 name_of(device));
-    no_gradient(t, name);
+    check_source(t, name);
     *one = T(0);
     *each = static_cast<const T*>(t.const_data_ptr());
 }
@@ -278,7 +279,7 @@ const void* beside(PyObject* o, const char* name, const at::Tensor& logits, cons
     require((t.size(1) == 1 || t.stride(1) == 1) && t.device() == logits.device(),
             std::string(name) + ": adjacent columns on " + name_of(logits.device()) + " are needed (stride " +
                 std::to_string(t.stride(1)) + "; it is on " + name_of(t.device()) + ")");
-    no_gradient(t, name);
+    check_source(t, name);
     *ld = t.stride(0);
     return t.const_data_ptr();
 }

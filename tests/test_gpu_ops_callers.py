@@ -36,3 +36,18 @@ def test_a_lost_gradient_is_refused(ops):
         ops.sample_moves(x, noise.clone().requires_grad_())
     with torch.no_grad():
         ops.sample_moves(x, noise.clone().requires_grad_())
+
+
+def test_a_negated_view_is_refused(ops):
+    """A view whose values are its memory's, negated."""
+    import torch
+
+    x = torch.ones(4, 64, device="cuda")
+    n = torch._neg_view(x)
+    w = ops.mx4_quantise(x)
+    for call in (lambda: ops.mx4_quantise(n), lambda: ops.mx4_product(n, w), lambda: ops.mx4_product(n[0], w),
+                 lambda: ops.mx4_product(x, w, bias=torch._neg_view(x[0, :4])), lambda: ops.sample_moves(n, x),
+                 lambda: ops.sample_moves(x, n), lambda: ops.sample_moves(x, x, temperature=torch._neg_view(x[:, 0].clone()))):
+        with pytest.raises(ValueError, match="resolve_neg"):
+            call()
+    assert bool((ops.mx4_values(ops.mx4_quantise(n.resolve_neg())) == -1).all())
