@@ -11,8 +11,9 @@ synchronise and can be captured into a CUDA graph after a first call on the
 device. Tensors are float32 or bfloat16; a matrix's rows may be any distance
 apart (0 for a broadcast source), its columns are adjacent. There is no
 backward pass: an argument that requires a gradient or carries a forward-mode
-tangent is refused. Bad arguments raise ValueError, failures of the device
-azb200.CudaError.
+tangent is refused, and so are a negated view, a tensor that stands for others
+and a call under a trace (the calls run below torch's dispatcher). Bad
+arguments raise ValueError, failures of the device azb200.CudaError.
 
 The calls go through _azb_torch.so (binding/azb_torch.cpp); importing this
 module fails loudly when it is missing.

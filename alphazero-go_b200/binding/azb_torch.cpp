@@ -17,8 +17,10 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <azb200.h>
 
@@ -113,6 +115,20 @@ void check_source(const at::Tensor& t, const char* what) {
     require(!tangent && !(t.requires_grad() && c10::GradMode::is_enabled()),
             std::string(what) + " requires a gradient, and there is no backward pass (detach it)");
     require(!t.is_neg(), std::string(what) + " is a view of negated memory (resolve_neg it)");
+    require(!t.key_set().has(c10::DispatchKey::Python),
+            std::string(what) + " is of a tensor subclass with a dispatch of its own, which these calls would bypass");
+    require(t.has_storage(), std::string(what) + " stands for other tensors (a transform's, say) and has no memory to read");
+}
+
+// These calls run below torch's dispatcher: a trace would hold their results
+// as constants.
+void check_untraced() {
+    using Mode = c10::impl::TorchDispatchModeKey;
+    using Modes = c10::impl::TorchDispatchModeTLS;
+    const bool traced = torch::jit::tracer::isTracing() ||
+                        (Modes::any_modes_set() && (Modes::get_mode(Mode::FAKE) || Modes::get_mode(Mode::PROXY) ||
+                                                    Modes::get_mode(Mode::FUNCTIONAL)));
+    require(!traced, "these calls cannot be traced (capture them into a CUDA graph instead)");
 }
 
 Matrix matrix(const at::Tensor& t, const char* what) {
@@ -158,6 +174,7 @@ const uint8_t* quantised_data(const at::Tensor& data, const Quantised& q, const 
 PyObject* mx4_quantise(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         want(n, 1);
+        check_untraced();
         const at::Tensor& x = tensor(args[0], "x");
         const Matrix m = matrix(x, "x");
         const Quantised q{m.rows, m.cols};
@@ -181,6 +198,7 @@ PyObject* mx4_quantise(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* mx4_values(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         want(n, 4);
+        check_untraced();
         const at::Tensor& data = tensor(args[0], "q");
         const Quantised q{whole(args[1]), whole(args[2])};
         const uint8_t* p = quantised_data(data, q, "q");
@@ -199,6 +217,7 @@ PyObject* mx4_values(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* mx4_product(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         want(n, 9);
+        check_untraced();
         const long long x_rows = whole(args[1]);
         const bool plain = x_rows < 0;
         at::Tensor x = tensor(args[0], "x");
@@ -289,6 +308,7 @@ const void* beside(PyObject* o, const char* name, const at::Tensor& logits, cons
 PyObject* sample_moves(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         want(n, 7);
+        check_untraced();
         const at::Tensor& logits = tensor(args[0], "logits");
         const Matrix m = matrix(logits, "logits");
         const at::Device device = logits.device();

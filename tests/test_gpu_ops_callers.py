@@ -51,3 +51,43 @@ def test_a_negated_view_is_refused(ops):
         with pytest.raises(ValueError, match="resolve_neg"):
             call()
     assert bool((ops.mx4_values(ops.mx4_quantise(n.resolve_neg())) == -1).all())
+
+
+def test_traces_and_wrapped_tensors_are_refused(ops):
+    """The calls run below torch's dispatcher: a trace would hold their results
+    as constants, and a tensor that stands for others has no memory to read."""
+    import torch
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    x = torch.ones(4, 64, device="cuda")
+    w = ops.mx4_quantise(x)
+    calls = (lambda x: ops.mx4_values(ops.mx4_quantise(x)), lambda x: ops.mx4_product(x, w), lambda x: ops.sample_moves(x, x)[0])
+    for call in calls:
+        with pytest.raises(ValueError, match="trac"):
+            make_fx(call)(x)
+        with pytest.raises(ValueError, match="trac"):
+            torch.jit.trace(call, x)
+        with pytest.raises(ValueError):
+            torch.func.vmap(call)(x[None])
+        with pytest.raises(ValueError):
+            torch.func.grad(lambda x: call(x).sum())(x)
+        with FakeTensorMode() as mode, pytest.raises(ValueError):
+            call(mode.from_tensor(x))
+
+    class Wrapped(torch.Tensor):
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            raise AssertionError("not reached")
+
+    with pytest.raises(ValueError, match="subclass"):
+        ops.mx4_quantise(torch.Tensor._make_subclass(Wrapped, x))
+
+    class Counting(TorchDispatchMode):   # looks on, and is no trace
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    with Counting():
+        assert torch.equal(ops.mx4_product(x, w), torch.full((4, 4), 64.0, device="cuda"))
+    assert torch.equal(ops.mx4_product(torch.nn.Parameter(x, requires_grad=False), w), torch.full((4, 4), 64.0, device="cuda"))
