@@ -331,9 +331,17 @@ CUtensorMap make_map_2d(CUtensorMapDataType type, const void* base, uint64_t inn
     const cuuint64_t strides[1] = {row_bytes};
     const cuuint32_t box[2] = {box_inner, box_rows};
     const cuuint32_t estr[2] = {1, 1};
-    const CUresult r = encode_tiled()(&m, type, 2, const_cast<void*>(base), dims, strides, box, estr,
-                                      CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const auto encode = [&] {
+        return encode_tiled()(&m, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = encode();
+    if (r == CUDA_ERROR_INVALID_CONTEXT) {   // the host thread's first call: no context is current on it yet
+        int device = 0;
+        check(cudaGetDevice(&device), "cudaGetDevice");
+        check(cudaSetDevice(device), "cudaSetDevice");
+        r = encode();
+    }
     if (r != CUDA_SUCCESS) throw std::runtime_error("cuda: cuTensorMapEncodeTiled failed (" + std::to_string(int(r)) + ")");
     return m;
 }

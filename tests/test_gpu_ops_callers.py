@@ -1,6 +1,9 @@
 """Callers of the device operators (include/azb200.h, "device operators")
-beside the plain one: torch's ways of following a computation, which these
-calls cannot take part in and therefore refuse."""
+beside the plain one: several host threads, and torch's ways of following a
+computation, which these calls cannot take part in and therefore refuse."""
+import ctypes as C
+import threading
+
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -91,3 +94,36 @@ def test_traces_and_wrapped_tensors_are_refused(ops):
     with Counting():
         assert torch.equal(ops.mx4_product(x, w), torch.full((4, 4), 64.0, device="cuda"))
     assert torch.equal(ops.mx4_product(torch.nn.Parameter(x, requires_grad=False), w), torch.full((4, 4), 64.0, device="cuda"))
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 100, 300), (40, 100, 300), (2000, 2000, 64)])
+def test_a_host_threads_first_call_may_be_a_product(ops, m, n, k):
+    """No call of that thread has touched the device before."""
+    import torch
+
+    x, w = ops.mx4_quantise(torch.ones(m, k, device="cuda")), ops.mx4_quantise(torch.ones(n, k, device="cuda"))
+    plain = torch.ones(m, k, device="cuda")
+    out = torch.zeros(m, n, device="cuda")
+    torch.cuda.synchronize()
+    got = {}
+
+    def through_c():
+        e = C.create_string_buffer(1024)
+        rc = ops.azb200.lib().azb_mx4_product(0, *x.pointers(), m, *w.pointers(), n, k, None, 0, out.data_ptr(), 0, n, None, e, 1024)
+        got["c"] = (rc, e.value)
+
+    def through_python(name, x):
+        try:
+            got[name] = ops.mx4_product(x, w, dtype=torch.float32)
+        except Exception as e:
+            got[name] = e
+
+    for target, args in ((through_c, ()), (through_python, ("mx4", x)), (through_python, ("plain", plain))):
+        t = threading.Thread(target=target, args=args)
+        t.start()
+        t.join()
+    torch.cuda.synchronize()
+    ref = torch.full((m, n), float(k), device="cuda")
+    assert got["c"] == (0, b"") and torch.equal(out, ref)
+    for name in ("mx4", "plain"):
+        assert isinstance(got[name], torch.Tensor) and torch.equal(got[name], ref), got[name]
