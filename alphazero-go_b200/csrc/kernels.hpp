@@ -15,6 +15,7 @@
 #include <cstdint>
 #include <cuda.h>
 #include <cuda_runtime.h>
+#include <mutex>
 
 namespace azb {
 
@@ -38,20 +39,22 @@ cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t s
 
 // Lets `Kernel` use `bytes` of dynamic shared memory on the current device.
 // The attribute belongs to the device, so each device is opened once (and
-// again for a larger size): one process may launch on several GPUs.
+// again for a larger size): one process may launch on several GPUs. The
+// attribute only grows: host threads that ask at once take turns, and what
+// `opened` says has been set.
 constexpr int kMaxDevices = 64;
 template <auto Kernel>
 cudaError_t open_smem(size_t bytes) {
     static std::atomic<size_t> opened[kMaxDevices];
+    static std::mutex turn;
     int dev = 0;
     if (const cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
-    if (dev >= 0 && dev < kMaxDevices && bytes <= opened[dev].load()) return cudaSuccess;
+    if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+    if (bytes <= opened[dev].load()) return cudaSuccess;
+    const std::lock_guard<std::mutex> lock(turn);
+    if (bytes <= opened[dev].load()) return cudaSuccess;
     const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
-    if (e == cudaSuccess && dev >= 0 && dev < kMaxDevices) {
-        size_t seen = opened[dev].load();
-        while (seen < bytes && !opened[dev].compare_exchange_weak(seen, bytes)) {
-        }
-    }
+    if (e == cudaSuccess) opened[dev].store(bytes);
     return e;
 }
 

@@ -2,6 +2,9 @@
 beside the plain one: several host threads, and torch's ways of following a
 computation, which these calls cannot take part in and therefore refuse."""
 import ctypes as C
+import os
+import subprocess
+import sys
 import threading
 
 import pytest
@@ -127,3 +130,60 @@ def test_a_host_threads_first_call_may_be_a_product(ops, m, n, k):
     assert got["c"] == (0, b"") and torch.equal(out, ref)
     for name in ("mx4", "plain"):
         assert isinstance(got[name], torch.Tensor) and torch.equal(got[name], ref), got[name]
+
+
+def child(text):
+    """Runs Python code in a process of its own, whose first calls are its."""
+    env = dict(os.environ, PYTHONPATH=os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "alphazero-go_b200"))
+    r = subprocess.run([sys.executable, "-c", text], env=env, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-2000:]
+    return r.stdout
+
+
+FIRST_CALLS = """
+import ctypes as C, threading
+import torch, azb200 as E
+L = E.lib()
+logits = torch.zeros(1, 1 << 17, device="cuda")
+noise = torch.full((1, 1 << 17), 0.5, device="cuda")
+moves = torch.zeros(64, dtype=torch.int64, device="cuda")
+data = torch.zeros(1 << 22, dtype=torch.uint8, device="cuda")
+out = torch.zeros(1 << 14, device="cuda")
+torch.cuda.synchronize()
+
+def sample(cols, type):
+    a = E.SampleArgs(logits=logits.data_ptr(), type=type, rows=1, cols=cols, ld=cols, noise=noise.data_ptr(), noise_ld=cols,
+                     temperature=1.0, top_p=1.0, moves=moves.data_ptr())
+    e = C.create_string_buffer(1024)
+    return L.azb_sample_moves(0, C.byref(a), None, e, 1024), cols, type, e.value
+
+def product(k, m):
+    p = data.data_ptr()
+    e = C.create_string_buffer(1024)
+    return L.azb_mx4_product(0, p, p, m, p, p, 100, k, None, 0, out.data_ptr(), 0, 100, None, e, 1024), k, m, e.value
+
+sets = [[(sample, c, t) for c in sizes] for t in (0, 1)
+        for sizes in ([1100, 8192, 2000, 5000, 3000, 7000, 4000, 6000], [8200, 16384, 9000, 12000, 10000, 15000, 11000, 13000],
+                      [16400, 32768, 40000, 65536, 20000, 60000, 50000, 30000])]
+sets += [[(product, k, m) for k in (768, 512, 256, 600) for m in (1, 128)]]
+failed = []
+for calls in sets:
+    ready = threading.Barrier(len(calls))
+    def one(f, *args):
+        ready.wait()
+        r = f(*args)
+        if r[0]: failed.append(r)
+    threads = [threading.Thread(target=one, args=c) for c in calls]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    failed += [r for r in (c[0](*c[1:]) for c in calls) if r[0]]
+torch.cuda.synchronize()
+assert not failed, failed
+"""
+
+
+def test_first_calls_from_several_threads():
+    """Every call of a kernel's first ones, of different sizes at once, and
+    each of those sizes afterwards."""
+    for _ in range(2):
+        child(FIRST_CALLS)
