@@ -165,6 +165,7 @@ def lib() -> C.CDLL:
             L.azb_probe_fill.argtypes = [C.c_int, _F, s, C.c_float, s] + err
             L.azb_probe_tanh.argtypes = [C.c_int, _F, s] + err
             L.azb_probe_bounded_wait.argtypes = [C.c_int, C.c_ulonglong] + err
+            L.azb_probe_ops_wait.argtypes = [C.c_int, C.c_ulonglong] + err
             L.azb_probe_umma.argtypes = [C.c_int] * 7 + [_F, _F, _F] + err
             L.azb_synth_network.argtypes = [D, C.c_uint64, C.c_int, _F, _F]
             L.azb_synth_positions.argtypes = [D, C.c_uint64, C.c_long, C.c_int, _F]
@@ -689,6 +690,13 @@ class cuda_probe:
         if code < 0:
             raise CudaError(e.value.decode())
         return code
+
+    @staticmethod
+    def ops_wait(limit_ns: int, device: int = 0):
+        """A wait that runs out as a product kernel's would; azb_ops.check reports it for the rest of the process."""
+        e = _err()
+        if lib().azb_probe_ops_wait(device, limit_ns, e, 1024) != 0:
+            raise CudaError(e.value.decode())
 
     @staticmethod
     def umma(precision: int, n_out: int, halo_rows: int, shift: int, k_chunks: int, a: np.ndarray, w: np.ndarray,

@@ -136,7 +136,8 @@ def sample_moves(logits: torch.Tensor, noise: torch.Tensor | None, *, legal: tor
 
 
 def check(device: int = 0) -> None:
-    """Waits for the device; raises CudaError if a product kernel's bounded wait ran out since the last check."""
+    """Waits for the device; raises CudaError if a product kernel's bounded wait ever ran out on it (and again in every
+    later call: that product's outputs are not valid, whoever's they were)."""
     e = azb200._err()
     if azb200.lib().azb_ops_check(device, e, 1024) != 0:
         raise CudaError(e.value.decode())

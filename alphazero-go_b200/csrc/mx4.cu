@@ -21,7 +21,7 @@ namespace azb {
 
 namespace {
 
-__device__ int g_mx4_error;   // KernelError of a product whose bounded wait ran out
+__device__ int g_mx4_error;   // KernelError of the first product whose bounded wait ran out; never cleared
 
 // ---------------------------------------------------------- conversions
 
@@ -1164,13 +1164,16 @@ cudaError_t launch_mx4_product(const MxProductArgs& a, int sms, cudaStream_t s) 
     return a.type == kElemBF16 ? launch(__nv_bfloat16()) : launch(0.0f);
 }
 
-cudaError_t mx4_take_error(int* code) {
+cudaError_t mx4_error(int* code) {
     *code = 0;
-    cudaError_t e = cudaDeviceSynchronize();
-    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(code, g_mx4_error, sizeof(int));
-    const int zero = 0;
-    if (e == cudaSuccess && *code) e = cudaMemcpyToSymbol(g_mx4_error, &zero, sizeof(int));
-    return e;
+    const cudaError_t e = cudaDeviceSynchronize();
+    return e == cudaSuccess ? cudaMemcpyFromSymbol(code, g_mx4_error, sizeof(int)) : e;
+}
+
+cudaError_t mx4_error_probe(unsigned long long limit_ns) {
+    void* word = nullptr;
+    const cudaError_t e = cudaGetSymbolAddress(&word, g_mx4_error);
+    return e == cudaSuccess ? launch_bounded_wait_probe(static_cast<int*>(word), limit_ns, nullptr) : e;
 }
 
 }  // namespace azb

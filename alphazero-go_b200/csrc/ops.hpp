@@ -68,8 +68,10 @@ struct MxProductArgs {
 bool mx4_product_quantises(long long m, long long n, long long k);
 cudaError_t launch_mx4_product(const MxProductArgs& a, int sms, cudaStream_t s);
 // The product kernels' error word on the current device (KernelError; 0:
-// none), read and cleared after waiting for the device.
-cudaError_t mx4_take_error(int* code);
+// none), read after waiting for the device.
+cudaError_t mx4_error(int* code);
+// A wait of limit_ns that runs out and is recorded there.
+cudaError_t mx4_error_probe(unsigned long long limit_ns);
 
 // ------------------------------------------------------------ move sampler
 

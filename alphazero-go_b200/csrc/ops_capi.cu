@@ -223,8 +223,15 @@ int azb_ops_check(int device, char* err, size_t err_cap) {
     return guarded(err, err_cap, "", [&] {
         const OnDevice on(device);
         int code = 0;
-        check(mx4_take_error(&code), "azb_ops_check");
+        check(mx4_error(&code), "azb_ops_check");
         if (code) throw std::runtime_error("cuda: " + kernel_error_text(code));
+    });
+}
+
+int azb_probe_ops_wait(int device, unsigned long long limit_ns, char* err, size_t err_cap) {
+    return guarded(err, err_cap, "", [&] {
+        const OnDevice on(device);
+        check(mx4_error_probe(limit_ns), "azb_probe_ops_wait");
     });
 }
 

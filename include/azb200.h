@@ -341,8 +341,9 @@ typedef struct azb_sample_args {
 int azb_sample_moves(int device, const azb_sample_args* args, void* stream, char* err, size_t err_cap);
 
 /* Waits for the device and reports whether a bounded wait inside a product
- * kernel ran out since the last call (its outputs are then not valid): 0, or
- * -1 with "cuda: ...". */
+ * kernel ever ran out on it (that product's outputs are then not valid): 0, or
+ * -1 with "cuda: ...". Like a CUDA error that sticks, it is reported to every
+ * caller from then on, whoever asked before. The calls above do not report it. */
 int azb_ops_check(int device, char* err, size_t err_cap);
 
 /* ------------------------------------------------------- memory checks */
@@ -418,6 +419,9 @@ int azb_probe_tanh(int device, float* data, size_t n, char* err, size_t err_cap)
 /* A kernel that waits on a barrier nothing arrives on: returns the kernel's
  * error word (5: its wait ran out after limit_ns) with the context intact. */
 int azb_probe_bounded_wait(int device, unsigned long long limit_ns, char* err, size_t err_cap);
+/* A wait of limit_ns that runs out as a product kernel's would, for
+ * azb_ops_check to report for the rest of the process. */
+int azb_probe_ops_wait(int device, unsigned long long limit_ns, char* err, size_t err_cap);
 /* The tensor-core path alone on one CTA: D[128][n_out] = A[shift .. shift+127]
  * . W^T over k_chunks 128-byte chunks, A [halo_rows][chunk*k_chunks] and W
  * [n_out][9*chunk*k_chunks] given as host fp32 (converted per precision);

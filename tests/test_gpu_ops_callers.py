@@ -1,6 +1,7 @@
 """Callers of the device operators (include/azb200.h, "device operators")
-beside the plain one: several host threads, and torch's ways of following a
-computation, which these calls cannot take part in and therefore refuse."""
+beside the plain one: several host threads, several users of one device's error
+word, and torch's ways of following a computation, which these calls cannot
+take part in and therefore refuse."""
 import ctypes as C
 import os
 import subprocess
@@ -187,3 +188,21 @@ def test_first_calls_from_several_threads():
     each of those sizes afterwards."""
     for _ in range(2):
         child(FIRST_CALLS)
+
+
+def test_every_user_learns_of_a_wait_that_ran_out():
+    """Whoever asks first, and after other products that went well."""
+    out = child("""
+import torch, azb200 as E, azb_ops as A
+w = A.mx4_quantise(torch.ones(4, 64, device="cuda"))
+A.check(0)
+E.cuda_probe.ops_wait(1000000)
+for user in ("first", "second"):
+    try:
+        A.check(0)
+        print(user, "no error")
+    except E.CudaError as e:
+        print(user, e)
+    assert bool((A.mx4_product(torch.ones(3, 64, device="cuda"), w) == 64).all())
+""")
+    assert [line.split(" ", 1) for line in out.splitlines()] == [[u, "cuda: bounded wait ran out"] for u in ("first", "second")]
