@@ -537,11 +537,6 @@ __global__ void __launch_bounds__(kPThreads)
         if (!p.early_w) grid_dependency_wait();
         for (int i = 0; i < ahead; ++i) load_w(c_begin + i, i);
         if (p.early_w) grid_dependency_wait();
-        // A call of one launch lets the next one's CTAs in at once (1 x 4096 x
-        // 4096 5.0 us so, 5.7 without); behind a product with a quantisation
-        // before it the next quantisation's blocks only take up SMs (333 x 1111
-        // x 2501 11.0 us so, 10.2 without).
-        if constexpr (kPlain) grid_launch_dependents();
         for (int i = 0; i < ahead; ++i) load_x(c_begin + i, i);
     }
     if (warp == 1) tmem_alloc(&tmem_slot, p.tmem_cols);
@@ -549,6 +544,12 @@ __global__ void __launch_bounds__(kPThreads)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
+    // A call of one launch lets the next one's CTAs in at once (1 x 4096 x 4096
+    // 5.0 us so, 5.7 without); behind a product with a quantisation before it
+    // the next quantisation's blocks only take up SMs (333 x 1111 x 2501 11.0
+    // us so, 10.2 without). Not before this CTA has its TMEM: a CTA let in
+    // sooner could take it first, and keep it until this one is done.
+    if constexpr (kPlain) grid_launch_dependents();
 
     if (warp == 0 && elect_one()) {
         Ring r;

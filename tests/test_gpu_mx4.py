@@ -297,3 +297,16 @@ def test_refusals(ops, torch):
         with pytest.raises(ValueError, match=text):
             call()
     ops.check(0)
+
+
+def test_products_that_fill_the_accumulators_follow_at_once(ops, torch):
+    """A small product of plain x lets the next launch in early; the next here
+    takes the whole of the tensor core's memory on every SM."""
+    m, n, k = 40000, 100, 256
+    x, w = ops.mx4_quantise(gpu(torch, normals(1, m, k), "bfloat16")), ops.mx4_quantise(gpu(torch, normals(2, n, k), "bfloat16"))
+    one, v = gpu(torch, normals(3, 1, k), "float32"), ops.mx4_quantise(gpu(torch, normals(4, 3000, k), "float32"))
+    ref, small = ops.mx4_product(x, w), ops.mx4_product(one, v)
+    torch.cuda.synchronize()
+    got = [(ops.mx4_product(one, v), ops.mx4_product(x, w)) for _ in range(50)]
+    assert all(torch.equal(a, small) and torch.equal(b, ref) for a, b in got)
+    ops.check(0)
