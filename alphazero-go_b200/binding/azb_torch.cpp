@@ -111,13 +111,14 @@ struct Matrix {
 // That a tensor's memory holds its values, and that nothing follows them. A
 // gradient, or a forward-mode tangent, would be lost: there is no backward pass.
 void check_source(const at::Tensor& t, const char* what) {
-    const bool tangent = t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode();
-    require(!tangent && !(t.requires_grad() && c10::GradMode::is_enabled()),
-            std::string(what) + " requires a gradient, and there is no backward pass (detach it)");
-    require(!t.is_neg(), std::string(what) + " is a view of negated memory (resolve_neg it)");
-    require(!t.key_set().has(c10::DispatchKey::Python),
-            std::string(what) + " is of a tensor subclass with a dispatch of its own, which these calls would bypass");
-    require(t.has_storage(), std::string(what) + " stands for other tensors (a transform's, say) and has no memory to read");
+    const auto refuse = [&](const char* why) { throw Refused{std::string(what) + why}; };
+    if ((t.requires_grad() && c10::GradMode::is_enabled()) ||
+        (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode()))
+        refuse(" requires a gradient, and there is no backward pass (detach it)");
+    if (t.is_neg()) refuse(" is a view of negated memory (resolve_neg it)");
+    if (t.key_set().has(c10::DispatchKey::Python))
+        refuse(" is of a tensor subclass with a dispatch of its own, which these calls would bypass");
+    if (!t.has_storage()) refuse(" stands for other tensors (a transform's, say) and has no memory to read");
 }
 
 // These calls run below torch's dispatcher: a trace would hold their results
@@ -125,10 +126,9 @@ void check_source(const at::Tensor& t, const char* what) {
 void check_untraced() {
     using Mode = c10::impl::TorchDispatchModeKey;
     using Modes = c10::impl::TorchDispatchModeTLS;
-    const bool traced = torch::jit::tracer::isTracing() ||
-                        (Modes::any_modes_set() && (Modes::get_mode(Mode::FAKE) || Modes::get_mode(Mode::PROXY) ||
-                                                    Modes::get_mode(Mode::FUNCTIONAL)));
-    require(!traced, "these calls cannot be traced (capture them into a CUDA graph instead)");
+    if (torch::jit::tracer::isTracing() || (Modes::any_modes_set() && (Modes::get_mode(Mode::FAKE) || Modes::get_mode(Mode::PROXY) ||
+                                                                       Modes::get_mode(Mode::FUNCTIONAL))))
+        throw Refused{"these calls cannot be traced (capture them into a CUDA graph instead)"};
 }
 
 Matrix matrix(const at::Tensor& t, const char* what) {
