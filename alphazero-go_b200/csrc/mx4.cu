@@ -637,10 +637,12 @@ __global__ void __launch_bounds__(kPThreads)
                 mbar_arrive(&full[r.idx]);
                 r.next(uint32_t(p.stages));
             }
+            __syncwarp();
         }
     }
     if (warp >= 2) {
         mbar_wait(&done, 0, &g_mx4_error, kErrWaitEpilogue);
+        __syncwarp();   // the lanes poll each for itself; the loads from TMEM are the warp's
         tc_fence_after();
         // The accumulator into shared memory (the stages are done with), a
         // row of x after the other: from there a warp stores a row's 128
@@ -688,6 +690,7 @@ __global__ void __launch_bounds__(kPThreads)
     }
     // The parts' sum, in order of K (the same bits on every run): CTA `split`
     // finishes rows split, split + splits, ... of the tile.
+    __syncwarp();
     cluster_sync();
     constexpr int kAhead = 4;   // rows whose parts are all asked for before the first sum
     const int step = p.splits * (kPThreads / 32);
@@ -898,7 +901,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         float* const bias_of = reinterpret_cast<float*>(boxes + kPairEpiWarps * kPairBox) + (warp - 2) * 128;   // of its columns
         uint32_t j = 0;
         for (int tile = int(blockIdx.x) >> 1; tile < p.tiles; tile += pairs, ++j) {
-            if (!mbar_wait(&acc_full, j & 1u, &g_mx4_error, kErrWaitEpilogue)) break;
+            // The lanes poll each for itself; the loads from TMEM are the warp's.
+            if (!__all_sync(0xFFFFFFFFu, mbar_wait(&acc_full, j & 1u, &g_mx4_error, kErrWaitEpilogue))) break;
             tc_fence_after();
             uint32_t v[4][32];
 #pragma unroll
@@ -952,14 +956,14 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                     if (lane == 0) bulk_commit();
                 }
             } else {
-                if (l >= p.lanes) continue;
-                const float bias = p.bias ? __ldg(p.bias + l) : 0.0f;
+                const bool in = l < p.lanes;
+                const float bias = p.bias && in ? __ldg(p.bias + l) : 0.0f;
                 T* dst = out + size_t(c0) * size_t(p.ld) + l;
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
-                        if (c0 + q * 32 + i < p.cols) *dst = T(act(v[q][i], bias));
+                        if (in && c0 + q * 32 + i < p.cols) *dst = T(act(v[q][i], bias));
                         dst += p.ld;
                     }
             }

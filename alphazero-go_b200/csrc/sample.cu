@@ -831,6 +831,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3)
         s.count = int(__reduce_add_sync(0xFFFFFFFFu, unsigned(s.count)));
         if (lane == 0) sh.wh[warp] = s.mass, sh.wk[warp] = s.count;
     }
+    __syncwarp();
     if constexpr (!kSolo) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // every CTA runs
     __syncthreads();
     Part all;   // (every warp, from its own reads; the sums' order is fixed)

@@ -310,3 +310,32 @@ def test_products_that_fill_the_accumulators_follow_at_once(ops, torch):
     got = [(ops.mx4_product(one, v), ops.mx4_product(x, w)) for _ in range(50)]
     assert all(torch.equal(a, small) and torch.equal(b, ref) for a, b in got)
     ops.check(0)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("m,n,ld", [(15400, 257, 257), (15400, 257, 301), (257, 15401, 15401), (15401, 264, 264), (15401, 264, 304),
+                                    (300, 15400, 15416)])
+def test_large_products_with_tails_and_strides(ops, torch, m, n, ld, dtype):
+    """Several tiles of 256 x 256 a pair of CTAs, the last ones with a few rows
+    or columns, output rows at multiples of 16 bytes and elsewhere, and rows
+    and columns that are NaN. Integers leave no room for rounding."""
+    r = np.random.default_rng(m + n)
+    values = np.array([-6, -4, -3, -2, -1, 0, 1, 2, 3, 4, 6], np.float32)
+    k = 70
+    x, w, bias = r.choice(values, (m, k)), r.choice(values, (n, k)), r.integers(-9, 10, n).astype(np.float32)
+    x[:, ::32], w[:, ::32] = 4, -4   # every block's scale is 1
+    ref = x.astype(np.float64) @ w.astype(np.float64).T + bias
+    bad_rows, bad_cols = [0, 255, 256, m - 1], [3, n - 1]
+    x[bad_rows, [1, 33, 66, 69]] = [np.inf, np.nan, -np.inf, np.nan]
+    w[bad_cols, [5, 68]] = [np.nan, np.inf]
+    ref[bad_rows], ref[:, bad_cols] = np.nan, np.nan
+    qx, qw = ops.mx4_quantise(gpu(torch, x, "float32")), ops.mx4_quantise(gpu(torch, w, "float32"))
+    b = gpu(torch, bias, "float32")
+    for relu in (0, 1):
+        out = gpu(torch, np.full((m, ld), -7.0), dtype)
+        raw(ops, "azb_mx4_product", 0, *qx.pointers(), m, *qw.pointers(), n, k, b.data_ptr(), relu, out.data_ptr(),
+            int(dtype == "bfloat16"), ld, None)
+        want = torch.as_tensor(np.maximum(ref, 0) if relu else ref, device="cuda").to(out.dtype)
+        assert torch.equal(out[:, :n].isnan(), want.isnan()) and torch.equal(out[:, :n].nan_to_num(0.5), want.nan_to_num(0.5))
+        assert bool((out[:, n:] == -7).all())
+    ops.check(0)
