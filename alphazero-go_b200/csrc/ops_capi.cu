@@ -62,8 +62,8 @@ void check_ld(long long ld, long long cols, long long rows, const char* fn) {
 }
 
 void check_aligned(const void* p, size_t to, const char* what, const char* fn) {
-    require(reinterpret_cast<uintptr_t>(p) % to == 0,
-            std::string(fn) + ": " + what + " must be aligned to " + std::to_string(to) + " bytes");
+    if (reinterpret_cast<uintptr_t>(p) % to != 0)
+        throw std::invalid_argument(std::string(fn) + ": " + what + " must be aligned to " + std::to_string(to) + " bytes");
 }
 
 // A quantised operand's two arrays.
@@ -135,6 +135,7 @@ int azb_mx4_product(int device, const void* x_codes, const void* x_scales, long 
         if (m == 0 || n == 0) return;
         require(out, std::string(fn) + ": null out");
         check_aligned(out, elem_size(type), "out", fn);
+        check_aligned(bias, 4, "bias", fn);
         check_mx(x_codes, x_scales, "x", fn);
         check_mx(w_codes, w_scales, "w", fn);
         const OnDevice on(device);
@@ -166,6 +167,7 @@ int azb_mx4_linear(int device, const void* x, int x_type, long long m, long long
         require(x && out, std::string(fn) + ": null x or out");
         check_aligned(x, elem_size(x_type), "x", fn);
         check_aligned(out, elem_size(type), "out", fn);
+        check_aligned(bias, 4, "bias", fn);
         check_mx(w_codes, w_scales, "w", fn);
         if (mx4_product_quantises(m, n, k)) {
             const OnDevice on(device);
@@ -211,6 +213,10 @@ int azb_sample_moves(int device, const azb_sample_args* p, void* stream, char* e
         check_aligned(p->noise, 4, "noise", fn);
         check_aligned(p->moves, 8, "moves", fn);
         check_aligned(p->logprob, 4, "logprob", fn);
+        check_aligned(p->temperature_rows, 4, "temperature_rows", fn);
+        check_aligned(p->top_p_rows, 4, "top_p_rows", fn);
+        check_aligned(p->min_p_rows, 4, "min_p_rows", fn);
+        check_aligned(p->top_k_rows, 4, "top_k_rows", fn);
         const SampleArgs a{p->logits, p->type, p->rows, p->ld, int(p->cols), p->noise, p->noise_ld, p->legal, p->legal_ld,
                            p->temperature, p->top_p, p->min_p, p->top_k, p->temperature_rows, p->top_p_rows,
                            p->min_p_rows, p->top_k_rows, reinterpret_cast<long long*>(p->moves), p->logprob};

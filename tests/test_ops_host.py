@@ -125,3 +125,17 @@ def test_python_refuses_host_tensors():
         A.mx4_product(x, x)
     with pytest.raises(ValueError, match="bytes of codes"):
         A.Mx4(torch.zeros(2, 16, dtype=torch.uint8), torch.zeros(4, dtype=torch.uint8), 2, 8)
+
+
+@pytest.mark.parametrize("call_", [
+    lambda at: product(bias=at),
+    lambda at: call("azb_mx4_linear", 0, P, 0, 2, 8, 8, P, P, 3, at, 0, P, 0, 3, P, 1 << 20, None),
+    lambda at: call("azb_mx4_linear", 0, P, 0, 2000, 8, 8, P, P, 3000, at, 0, P, 0, 3000, P, 1 << 20, None),
+    lambda at: sample(temperature_rows=at), lambda at: sample(top_p_rows=at), lambda at: sample(min_p_rows=at),
+    lambda at: sample(top_k_rows=at),
+])
+def test_misaligned_numbers_are_refused(call_):
+    """The kernels read the bias and the per-row settings as whole 4-byte numbers."""
+    for off in (1, 2, 3):
+        rc, msg = call_(P + off)
+        assert rc == -1 and "must be aligned to 4 bytes" in msg, msg
