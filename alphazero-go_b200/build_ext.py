@@ -130,10 +130,18 @@ BINDING_OUT = os.path.join(HERE, "_azb_torch.so")
 
 
 def _build_binding(force: bool, verbose: bool) -> None:
-    """_azb_torch.so, rebuilt when its source, the C ABI, torch or Python changes."""
+    """_azb_torch.so, rebuilt when its source, the C ABI, torch or Python changes.
+    The engine needs none of it: without a torch that has CUDA it is left out
+    (azb_ops, its only user, says so on import)."""
     import sysconfig
 
-    import torch
+    try:
+        import torch
+    except ImportError:
+        torch = None
+    if torch is None or torch.version.cuda is None:
+        print("build_ext: no torch with CUDA here: _azb_torch.so is not built (azb_ops needs it)", file=sys.stderr)
+        return
 
     root = os.path.dirname(torch.__file__)
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
