@@ -81,3 +81,24 @@ def test_the_engines_logits_sampled_in_place(fitted, engine):
 
     ref, _ = A.sample_moves(torch.as_tensor(logits, device="cuda"), noise)
     assert torch.equal(moves, ref)
+
+
+def test_every_logit_is_its_layers_product(fitted):
+    """Each layer against 64 bits on the layer's own input, so that no rounding
+    of the one before carries over: an fp32 sum of K exact terms, the bias and
+    the output's rounding (bfloat16's half a unit is 2^-8 of the value)."""
+    import azb_ops as A
+    import torch
+
+    desc, _, x, policy = fitted
+    h = torch.as_tensor(x.reshape(600, -1), device="cuda")
+    logits = policy.logits(h)
+    for i, (w, b) in enumerate(policy.layers):
+        xq, wq = A.mx4_values(A.mx4_quantise(h)).double(), A.mx4_values(w).double()
+        y, size = xq @ wq.t() + b.double(), xq.abs() @ wq.abs().t() + b.double().abs()
+        y = y.clamp(min=0) if i < 2 else y
+        out = A.mx4_product(h, w, bias=b, relu=i < 2, dtype=torch.bfloat16 if i < 2 else torch.float32)
+        tol = (h.shape[1] + 1) * 2.0 ** -23 * size + (2.0 ** -8 if i < 2 else 2.0 ** -24) * y.abs() + 2.0 ** -133
+        assert bool(((out.double() - y).abs() <= tol * (1 + 2.0 ** -8)).all())
+        h = out
+    assert torch.equal(logits, h)

@@ -339,3 +339,51 @@ def test_large_products_with_tails_and_strides(ops, torch, m, n, ld, dtype):
         assert torch.equal(out[:, :n].isnan(), want.isnan()) and torch.equal(out[:, :n].nan_to_num(0.5), want.nan_to_num(0.5))
         assert bool((out[:, n:] == -7).all())
     ops.check(0)
+
+
+def test_rounding_edges_and_special_blocks_of_bfloat16(ops, torch):
+    """As of float32, whose sources have code of their own: ties, the numbers
+    next to them, subnormals, the largest number, infinities and NaN."""
+    ties = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
+    edges = np.concatenate([[6.0, -0.0, 7.96875, -7.96875], ties, -ties, ties * (1 - 2.0 ** -8), ties * (1 + 2.0 ** -7)])
+    rows = [np.pad(edges * 2.0 ** e, (0, 32 - edges.size)) for e in (-130, -126, -124, -60, 0, 60, 124)]
+    special = np.zeros((9, 32))
+    special[1, 5] = np.inf
+    special[2, 31] = -np.inf
+    special[3, 0] = np.nan
+    special[4, :] = 2.0 ** -133                      # the least subnormal
+    special[5, :] = float(torch.finfo(torch.bfloat16).max)
+    special[6, 3] = -float(torch.finfo(torch.bfloat16).max)
+    special[7, :] = 2.0 ** -126
+    special[8, :] = np.where(np.arange(32) % 2, 2.0 ** -133 * 100, -(2.0 ** -126))
+    x = np.concatenate([np.stack(rows), special])
+    x = np.concatenate([x, x[::-1]], 1)              # a bad block next to a good one
+    x = torch.as_tensor(x, device="cuda").to(torch.bfloat16)
+    w = np.eye(64, dtype=np.float32)
+    for cols, pad in ((64, 0), (64, 1), (64, 4), (61, 3)):
+        v = torch.nn.functional.pad(x, (pad, 9))[:, pad:pad + cols]
+        ref = quantised(v.float().cpu().numpy())
+        q = ops.mx4_quantise(v)
+        assert same(host(ops.mx4_values(q, torch.float32)), ref) and same(host(ops.mx4_values(q, torch.bfloat16)), ref)
+        for m in (1, 16):                            # quantised by the product's own CTAs: a row of the identity each
+            y = host(ops.mx4_product(v[:m], ops.mx4_quantise(gpu(torch, w[:, :cols], "float32")), dtype=torch.float32))
+            bad = np.isnan(ref[:m]).any(1)
+            assert np.isnan(y[bad]).all() and np.array_equal(y[~bad][:, :cols], ref[:m][~bad])
+
+
+def test_two_streams_at_once(ops, torch):
+    """Products of every kind on two streams, with nothing between them."""
+    shapes = [(1, 4096, 4096), (16, 1000, 2000), (40, 3000, 700), (333, 1111, 2501), (3000, 2000, 300), (3001, 2001, 300)]
+    x = [gpu(torch, normals(m, m, k), "bfloat16") for m, n, k in shapes]
+    w = [ops.mx4_quantise(gpu(torch, normals(n, n, k), "bfloat16")) for m, n, k in shapes]
+    ref = [ops.mx4_product(a, b) for a, b in zip(x, w)]
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    order = np.random.default_rng(5)
+    for _ in range(300):
+        i, s = int(order.integers(len(shapes))), streams[int(order.integers(2))]
+        with torch.cuda.stream(s):
+            got.append((i, ops.mx4_product(x[i], w[i])))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, ref[i]) for i, y in got)
+    ops.check(0)

@@ -448,3 +448,22 @@ def test_extreme_temperatures(ops, torch, cols):
         n = np.isfinite(logits[i]).sum()
         assert np.isfinite(logits[i, m[i]]) and abs(lp[i] + np.log(n)) <= 1e-5
         assert m[i] == np.where(np.isfinite(logits[i]), noise[i], -1).argmax()
+
+
+def test_two_streams_at_once(ops, torch):
+    """Rows of every kernel on two streams, with nothing between them."""
+    cases = []
+    for rows, cols in ((300, 362), (40, 5000), (64, 16384), (9, 50001), (200, 50001), (2, 131072)):
+        logits, noise, _ = data(cols, rows, cols)
+        cases.append((torch.as_tensor(logits, device="cuda"), torch.as_tensor(noise, device="cuda"),
+                      dict(top_k=50, top_p=0.9) if rows % 2 else dict(top_p=0.8)))
+    ref = [ops.sample_moves(l, n, **f) for l, n, f in cases]
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    order = np.random.default_rng(6)
+    for _ in range(300):
+        i, s = int(order.integers(len(cases))), streams[int(order.integers(2))]
+        with torch.cuda.stream(s):
+            got.append((i, ops.sample_moves(cases[i][0], cases[i][1], **cases[i][2])))
+    torch.cuda.synchronize()
+    assert all(torch.equal(m, ref[i][0]) and torch.equal(lp, ref[i][1]) for i, (m, lp) in got)
