@@ -1023,9 +1023,12 @@ cudaError_t launch_pair(const MxProductArgs& a, int sms, cudaStream_t s) {
     return cudaLaunchKernelEx(&cfg, mx4_pair_kernel<T, kRowsOnLanes>, ml, mc, sl, sc, mo, p);
 }
 
-// Whether TMA can store rows of `out`.
+// Whether TMA can store rows of `out`: they start at multiples of 16 bytes and
+// end at such. (Of a row that ends elsewhere it writes the last 16 bytes whole,
+// into what lies between the caller's rows.)
 bool out_aligned(const MxProductArgs& a) {
-    return reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && size_t(a.ld) * elem_size(a.type) % 16 == 0;
+    const size_t es = elem_size(a.type);
+    return reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && size_t(a.ld) * es % 16 == 0 && size_t(a.n) * es % 16 == 0;
 }
 
 template <typename T, int kGroups, typename X>

@@ -387,3 +387,14 @@ def test_two_streams_at_once(ops, torch):
     torch.cuda.synchronize()
     assert all(torch.equal(y, ref[i]) for i, y in got)
     ops.check(0)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("n", [4097, 4098, 4099, 4100, 4103, 4104])
+def test_large_products_write_no_further_than_their_rows(ops, torch, n, dtype):
+    """Output rows that start at multiples of 16 bytes and end elsewhere."""
+    m, k, ld = 800, 64, 4112
+    x, w = ops.mx4_quantise(gpu(torch, normals(1, m, k), "float32")), ops.mx4_quantise(gpu(torch, normals(2, n, k), "float32"))
+    out = gpu(torch, np.full((m, ld), -7.0), dtype)
+    raw(ops, "azb_mx4_product", 0, *x.pointers(), m, *w.pointers(), n, k, None, 0, out.data_ptr(), int(dtype == "bfloat16"), ld, None)
+    assert torch.equal(out[:, :n], ops.mx4_product(x, w, dtype=out.dtype)) and bool((out[:, n:] == -7).all())
