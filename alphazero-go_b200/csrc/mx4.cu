@@ -330,9 +330,9 @@ dim3 cast_grid(long long rows, long long cols, int span, int sms) {
 // 32x128b.warpx4 form writes TMEM's scale columns).
 //
 // Few rows of x are bound by w's bytes and, at these sizes, by what comes
-// before and after them: 32 x 16384 x 4096 in 9.1 us with x's quantisation
-// (37 MB; 5.6 us at the rate of a copy), 1 x 4096 x 4096 in 4.8 us. Products
-// in between (333 x 1111 x 2501 in 10.2 us with x's quantisation) have too few
+// before and after them: 32 x 16384 x 4096 in 9.3 us with x's quantisation
+// (37 MB; 5.6 us at the rate of a copy), 1 x 4096 x 4096 in 4.9 us. Products
+// in between (333 x 1111 x 2501 in 10.5 us with x's quantisation) have too few
 // tiles to fill the SMs and run at the latency of a tile's K.
 struct ProductTile {
     int m, n;              // rows of x, rows of w
@@ -732,15 +732,16 @@ __global__ void __launch_bounds__(kPThreads)
 // every (number of pairs)-th tile, and its copies run ahead into the next
 // tile while the epilogue drains. The epilogue's eight warps read their whole
 // share of the accumulator into registers and free it before converting and
-// storing. 8192^3 in 185 us: 5.9 PFLOP/s, at which the GPU is at its power
-// limit (1.5 GHz); 4096^3, 3.5 tiles a pair, in 34 us.
+// storing. 8192^3 in 178 to 185 us: 5.9 to 6.2 PFLOP/s, at which the GPU is at
+// its power limit (1.5 GHz); 4096^3, 3.5 tiles a pair, in 31 us.
 //
 // kRowsOnLanes: TMEM's lanes are rows of x, so a thread holds neighbouring
 // outputs of one row; its warp lays them out in shared memory, 32 rows of 128
 // bytes at a time, and TMA stores them (where `out` is aligned for it; 16-byte
 // stores of 32 lanes into 32 rows took 6600 cycles a tile). Otherwise the
 // lanes are rows of w and a warp stores 32 neighbouring outputs at a time,
-// whatever the alignment.
+// whatever the alignment (6000 x 2049 x 64 into bfloat16 in 19 us, 6000 x 2048
+// x 64 by boxes in 13; 4096 x 4097 x 4096 37 us, x 4096 30).
 struct PairTile {
     int lanes, cols;                 // rows of the operand on the lanes and of the other
     int lane_tiles, tiles;           // tiles along the lanes, and in all

@@ -185,9 +185,9 @@ __device__ Threshold find_threshold(const RowParams& rp, uint32_t top, uint32_t 
 // and the race's two accurate logarithms are taken only for the columns that
 // cheap bounds of their keys leave in it.
 //
-// Bound by the latency of its steps: one row of 362 in 2.9 us, with top-k and
-// top-p, whose halvings follow one another, 5.9 us; 1024 rows of 362 with all
-// filters 8.7 us, 27% of the issue slots used. (Masses in fixed point, one
+// Bound by the latency of its steps: one row of 362 in 3.0 us, with top-k and
+// top-p, whose halvings follow one another, 6.0 us; 1024 rows of 362 with all
+// filters 8.7 us, 21% of the issue slots used. (Masses in fixed point, one
 // instruction a sum instead of five exchanges: 8.5 us, but 1024 rows of 1000
 // 19.4 instead of 18.6.)
 template <typename T, int kPer>
@@ -355,13 +355,13 @@ __global__ void __launch_bounds__(128) sample_warp_kernel(const SampleArgs a) {
 // above. Where the list would be longer (many equal logits, say) the range of
 // keys is halved as in find_threshold, over the listed upper logits.
 //
-// 512 rows of 131072 (fp32, top-p 0.9) take 268 us: 469 MB from DRAM (the
+// 512 rows of 131072 (fp32, top-p 0.9) take 270 us: 469 MB from DRAM (the
 // kept columns' numbers come in sectors of 32 bytes), a fifth of its rate. A
 // CTA lives 25 us, of which the load takes 3.4, the sum 1.9, the first
 // exchange 2.2, the list and histogram 5.1 with their exchange, the cut 9
 // with four more; three CTAs an SM (their slices fill it) overlap these, the
 // barriers of a cluster's eight being what is waited for. Without filters
-// 177 us. (One CTA a row, its passes reading L2: 375 us, and one row 76 us
+// 179 us. (One CTA a row, its passes reading L2: 375 us, and one row 76 us
 // where a cluster takes 18.)
 //
 // Up to 64 (a warp each of a cluster) top-k needs no histogram: the k-th
@@ -1406,12 +1406,12 @@ cudaError_t launch_sample_t(const SampleArgs& a, cudaStream_t s) {
         if (a.cols <= 384) return launch_pdl(sample_warp_kernel<T, 12>, dim3(unsigned(grid)), dim3(128), 0, s, a);
         return launch_pdl(sample_warp_kernel<T, 32>, dim3(unsigned(grid)), dim3(128), 0, s, a);
     }
-    // Up to 16384 columns one CTA has the row (512 rows of 16384, top-p: 26 us,
+    // Up to 16384 columns one CTA has the row (512 rows of 16384, top-p: 27 us,
     // with two of 8192 each 42 us); beyond, slices of at most 8192 while eight
-    // CTAs can hold the row so (8 rows of 50001: 14 us, with 16384 16 us). Where
+    // CTAs can hold the row so (8 rows of 50001, top-p: 14 us, with 16384 16 us). Where
     // not all of those run at once, up to 65536 columns, a row has half as many
-    // CTAs (512 rows of 50001: 174 us with eight, 102 us with four; 64 rows 30
-    // and 20), and its sums another order.
+    // CTAs (512 rows of 50001: 174 us with eight, 101 us with four; 64 rows 30
+    // and 19), and its sums another order.
     int ranks = a.cols <= 16384 ? 1 : a.cols <= 32768 ? 4 : kMaxCluster;
     if (ranks > 1 && a.cols <= 65536 && a.rows * ranks > kRowCtas) ranks /= 2;
     const int per = (a.cols + ranks - 1) / ranks;

@@ -282,8 +282,9 @@ enum { AZB_ELEM_F32 = 0, AZB_ELEM_BF16 = 1 };
  * 2i in the low half of byte i, zero past cols. scales: exponent + 127 (255:
  * NaN), one byte per block, in tiles of 128 rows x 4 blocks of 512 bytes: row
  * r, block b at ((r / 128) * ceil(blocks / 4) + b / 4) * 512 + (r % 32) * 16
- * + (r % 128 / 32) * 4 + b % 4. Both 16-byte aligned. azb_mx4_sizes gives
- * their sizes in bytes (rows 0..2^22, cols 1..2^26). */
+ * + (r % 128 / 32) * 4 + b % 4, zero outside the matrix (the product reads
+ * that too). Both 16-byte aligned. azb_mx4_sizes gives their sizes in bytes
+ * (rows 0..2^22, cols 1..2^26). */
 int azb_mx4_sizes(long long rows, long long cols, size_t* code_bytes, size_t* scale_bytes, char* err, size_t err_cap);
 int azb_mx4_quantise(int device, const void* x, int type, long long rows, long long cols, long long ld, void* codes,
                      void* scales, void* stream, char* err, size_t err_cap);
@@ -292,7 +293,9 @@ int azb_mx4_values(int device, const void* codes, const void* scales, long long 
                    long long ld, void* stream, char* err, size_t err_cap);
 /* out[i][j] = act(sum_k x[i][k] w[j][k] + bias[j]): x is m x k, w n x k, out
  * m x n, act ReLU (a NaN stays NaN) or nothing, bias fp32 or null. Products
- * are exact and summed in fp32. */
+ * are exact and summed in fp32, in an order that m, n and k decide: the same
+ * bits on every run, but a row's last bits may differ in a batch of another
+ * size. */
 int azb_mx4_product(int device, const void* x_codes, const void* x_scales, long long m, const void* w_codes,
                     const void* w_scales, long long n, long long k, const float* bias, int relu, void* out, int type,
                     long long ld, void* stream, char* err, size_t err_cap);
@@ -307,11 +310,11 @@ int azb_mx4_linear(int device, const void* x, int x_type, long long m, long long
 
 /* One move per row of logits. With l the legal, non-NaN logits above -inf and
  * m their maximum: x = 0 where l = m, else (l - m) / temperature (l - m in
- * fp32; a temperature below 5e-39 counts as that). In descending order of l
- * (ties: lower column first) top_k keeps the first k (0 or less: off), top_p
- * of those the shortest prefix whose share of their mass sum exp(x) reaches p
- * (1 or more: off), min_p those with exp(x) >= min_p (0 or less: off); the
- * first is always kept. The move is the kept column with the largest
+ * fp32; a temperature below 5e-39 counts as that, an infinite one as 1e45).
+ * In descending order of l (ties: lower column first) top_k keeps the first k
+ * (0 or less: off), top_p of those the shortest prefix whose share of their
+ * mass sum exp(x) reaches p (1 or more: off; 0 or less: the first alone),
+ * min_p those with exp(x) >= min_p (0 or less: off); the first is always kept. The move is the kept column with the largest
  * x - log(-log u), u its noise clamped into [2^-25, 1 - 2^-24] (a NaN: the
  * lowest), ties to the lower column: a draw from the kept ones' distribution
  * when the noise is uniform on (0, 1). logprob (may be null) is
